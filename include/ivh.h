@@ -212,6 +212,121 @@ int ivh_softmax_f16(const void * x, void * y, int outer, int axis, int inner, in
 int ivh_bmm_f16(const void * a, const void * b, void * y, int bb, int m, int k, int n, int batch,
                 void * stream);
 
+/* ---------------------------------------------------------------- sequence operators
+ * What a language or image-text model needs around its matrix products (no counterpart in the
+ * reference, whose attention is the bmm and softmax nodes of a plan): rotary positions, a paged
+ * key/value cache and attention.  Caller-owned device buffers and a stream as above; operands
+ * must be memory of the current device and the stream one of its own.  Nothing is allocated, and a call
+ * may be captured into a HIP graph; what differs from replay to replay (lengths, page numbers,
+ * positions) is read from device memory.  16-bit storage in either type, fp32 sums.
+ *
+ * Token rows are [tokens][heads][dim] with the strides of a token and of a head given in
+ * elements (a head's channels are contiguous); rows start at multiples of 8 bytes (rope, append)
+ * or 16 bytes (attention).  `cu` [batch + 1] are the first rows of the sequences, which lie one behind
+ * the other: sequence b has rows cu[b] .. cu[b + 1] - 1, possibly none; rows behind cu[batch] belong to no
+ * sequence and are neither read nor written.
+ */
+#define IVH_F16 0
+#define IVH_BF16 1
+
+/* Rotary positions: frequency f < rot / 2 turns a pair of a head's first rot channels by
+   pos[axis(f)][token] * freq[f] radians: (a, b) -> (a cos - b sin, b cos + a sin).  Channels from rot on
+   stay.  Angles are formed in 64 bits, the rotation in fp32, rounded once. */
+typedef struct ivh_rotation {
+  int rot;                  /* rotated channels of a head, a multiple of 8 */
+  int adjacent;             /* pairs: 0 channels (f, f + rot / 2), 1 channels (2 f, 2 f + 1) */
+  int axes;                 /* position axes, 1 to 4 (time, height, width, ..) */
+  int section[4];           /* frequencies of each axis, 0 for axes that are not there; sum rot / 2 */
+  int dealt;                /* 0: axis 0 has the first section[0] frequencies, then axis 1, ..;
+                               1: frequency f is axis f % axes' if that is not 0 and f / axes < its
+                               section, else axis 0's */
+} ivh_rotation;
+
+typedef struct ivh_rope_desc {
+  int type;                 /* IVH_F16 or IVH_BF16 */
+  int heads, dim;           /* dim: a multiple of 8, at most 1024 */
+  ivh_rotation rotation;
+  int64_t x_token, x_head, y_token, y_head;
+  int64_t pos_axis;         /* elements between two axes' positions */
+} ivh_rope_desc;
+
+/* y = rotated x; y may be x with the same strides, else the two must not overlap.  pos [axes][tokens],
+   freq [rot / 2]. */
+int ivh_rope(const ivh_rope_desc * d, const void * x, const int32_t * pos, const float * freq, void * y, int tokens,
+             void * stream);
+
+/* A paged key/value cache.  A page holds `page` tokens of every head; with E = 16 bytes' worth of
+   elements (16 codes of 8 bits, 8 values of 16) keys are stored as
+   [pages][heads][page / 4][dim / E][4][E], values as [pages][heads][page / E][dim][E]: the order in
+   which the attention's fragments want them.  8-bit pages hold e4m3 codes and two positive fp32
+   scales for each page and head.  `table` [batch][table_width] has the page of a sequence's tokens
+   0 .. page - 1, the next page, ..; a page number outside [0, pages) holds nothing: what is
+   appended there is dropped and attention passes over it. */
+typedef struct ivh_cache_desc {
+  int type;                 /* of keys, values and queries: IVH_F16 or IVH_BF16 */
+  int bits;                 /* 16: that type; 8: e4m3 with scales */
+  int heads, dim;           /* key heads; dim: a multiple of 16, at most 256 */
+  int page;                 /* tokens of a page: 16, 32, 64 or 128 */
+  int pages;                /* pages of the cache */
+  int table_width;          /* pages of a sequence at most */
+} ivh_cache_desc;
+
+/* bytes of each of the two page buffers, and of each of the two scale buffers (0 for 16 bits) */
+int ivh_cache_bytes(const ivh_cache_desc * d, size_t * pages, size_t * scales);
+
+typedef struct ivh_append_desc {
+  ivh_cache_desc cache;
+  ivh_rotation rotation;    /* of the keys; rot 0: none (pos and freq are not read) */
+  int64_t k_token, k_head, v_token, v_head;
+  int64_t pos_axis;
+} ivh_append_desc;
+
+/* Appends the new rows k, v (`tokens` of them at most) of every sequence; keys are rotated on the
+   way.  lens [batch] counts a sequence's tokens with the new ones: row i of sequence b becomes its token
+   lens[b] - (cu[b + 1] - cu[b]) + i.  An 8-bit page's scale is the smallest power of two s with
+   max |x| <= 448 s over the page's new values of a head, at least 2^-32 and at least the scale of
+   older tokens in the page; when it grows, the page's other codes of that head are rounded to it
+   (nearest, ties to even).  Infinities are stored as +-448 s, NaN as NaN; neither counts for s.  A page that gets tokens must belong to one
+   sequence alone; ks and vs of a page without tokens need no value. */
+int ivh_kv_append(const ivh_append_desc * d, const void * k, const void * v, const int32_t * pos, const float * freq,
+                  const int32_t * cu, const int32_t * lens, const int32_t * table, void * kc, void * vc, float * ks,
+                  float * vs, int batch, int tokens, void * stream);
+
+typedef struct ivh_paged_attn_desc {
+  ivh_cache_desc cache;
+  int heads;                /* query heads; heads / cache.heads share a key head */
+  float scale;              /* of q . k */
+  int window, sinks;        /* window 0: a token sees every earlier one and itself; else the last
+                               `window` tokens with itself, and the sequence's first `sinks` */
+  int64_t q_token, q_head, o_token, o_head;
+  int max_new, max_len;     /* new and cached tokens of a sequence at most, 0: unknown.  They steer
+                               how the call is split; results hold for any lengths */
+} ivh_paged_attn_desc;
+
+/* workspace of a call: partial sums where few rows meet many keys.  Calls that may run at the
+   same time need one each; its contents before a call do not matter */
+int ivh_paged_attention_workspace(const ivh_paged_attn_desc * d, int batch, int tokens, size_t * bytes);
+/* o = softmax(scale q k^T) v over the cached tokens of each row's sequence; lens, cu as for the append
+   that stored the rows' own tokens.  A row that sees no key is zero. */
+int ivh_paged_attention(const ivh_paged_attn_desc * d, const void * q, const void * kc, const void * vc, const float * ks,
+                        const float * vs, const int32_t * cu, const int32_t * lens, const int32_t * table, void * o,
+                        int batch, int tokens, void * workspace, size_t workspace_bytes, void * stream);
+
+typedef struct ivh_attn_desc {
+  int type;                 /* IVH_F16 or IVH_BF16 */
+  int heads, kv_heads, dim; /* dim: a multiple of 8, at most 256 */
+  float scale;
+  int causal;               /* row i of nq stands at place i + nk - nq of its nk keys; 1: it sees no later key */
+  int window, sinks;        /* window 0: all; else keys less than `window` places away, and the first `sinks` */
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head;
+  int max_q;                /* rows of a sequence at most, 0: unknown (steers the grid alone) */
+} ivh_attn_desc;
+
+/* The same over contiguous rows: sequence b's queries are rows cu_q[b] .., its keys and values rows
+   cu_k[b] .. (cu_q and cu_k may be one array). */
+int ivh_attention(const ivh_attn_desc * d, const void * q, const void * k, const void * v, const int32_t * cu_q,
+                  const int32_t * cu_k, void * o, int batch, int tokens_q, int tokens_k, void * stream);
+
 #ifdef __cplusplus
 }
 #endif

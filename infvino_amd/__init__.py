@@ -54,6 +54,42 @@ class ConvDesc(C.Structure):
                                        "has_bias", "channels_last")]
 
 
+class Rotation(C.Structure):
+    """ivh_rotation (include/ivh.h)."""
+    _fields_ = [("rot", C.c_int), ("adjacent", C.c_int), ("axes", C.c_int), ("section", C.c_int * 4), ("dealt", C.c_int)]
+
+
+class RopeDesc(C.Structure):
+    """ivh_rope_desc."""
+    _fields_ = [("type", C.c_int), ("heads", C.c_int), ("dim", C.c_int), ("rotation", Rotation)] + \
+        [(n, C.c_int64) for n in ("x_token", "x_head", "y_token", "y_head", "pos_axis")]
+
+
+class CacheDesc(C.Structure):
+    """ivh_cache_desc."""
+    _fields_ = [(n, C.c_int) for n in ("type", "bits", "heads", "dim", "page", "pages", "table_width")]
+
+
+class AppendDesc(C.Structure):
+    """ivh_append_desc."""
+    _fields_ = [("cache", CacheDesc), ("rotation", Rotation)] + \
+        [(n, C.c_int64) for n in ("k_token", "k_head", "v_token", "v_head", "pos_axis")]
+
+
+class PagedAttentionDesc(C.Structure):
+    """ivh_paged_attn_desc."""
+    _fields_ = [("cache", CacheDesc), ("heads", C.c_int), ("scale", C.c_float), ("window", C.c_int), ("sinks", C.c_int)] + \
+        [(n, C.c_int64) for n in ("q_token", "q_head", "o_token", "o_head")] + [("max_new", C.c_int), ("max_len", C.c_int)]
+
+
+class AttentionDesc(C.Structure):
+    """ivh_attn_desc."""
+    _fields_ = [(n, C.c_int) for n in ("type", "heads", "kv_heads", "dim")] + [("scale", C.c_float)] + \
+        [(n, C.c_int) for n in ("causal", "window", "sinks")] + \
+        [(n, C.c_int64) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "o_token", "o_head")] + \
+        [("max_q", C.c_int)]
+
+
 _cdp = C.POINTER(ConvDesc)
 
 SIGNATURES = {
@@ -98,6 +134,13 @@ SIGNATURES = {
     "ivh_pool_f16": (_i, [_i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "ivh_softmax_f16": (_i, [_vp, _vp, _i, _i, _i, _i, _vp]),
     "ivh_bmm_f16": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
+    # sequence operators
+    "ivh_rope": (_i, [C.POINTER(RopeDesc), _vp, _vp, _vp, _vp, _i, _vp]),
+    "ivh_cache_bytes": (_i, [C.POINTER(CacheDesc), _szp, _szp]),
+    "ivh_kv_append": (_i, [C.POINTER(AppendDesc)] + [_vp] * 11 + [_i, _i, _vp]),
+    "ivh_paged_attention_workspace": (_i, [C.POINTER(PagedAttentionDesc), _i, _i, _szp]),
+    "ivh_paged_attention": (_i, [C.POINTER(PagedAttentionDesc)] + [_vp] * 9 + [_i, _i, _vp, _sz, _vp]),
+    "ivh_attention": (_i, [C.POINTER(AttentionDesc)] + [_vp] * 6 + [_i, _i, _i, _vp]),
 }
 
 _lib = None

@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "../../include/ivh.h"
+#include "capi_guard.hpp"
 #include "conv_pack.hpp"
 #include "executor.hpp"
 #include "kernels.hpp"
@@ -20,29 +21,17 @@ struct ivh_model {
   ivh::Model * m = nullptr;
 };
 
-namespace {
-thread_local std::string g_err;
-
-template <class F>
-int guard(F && f)
+namespace ivh {
+std::string & last_error()
 {
-  try {
-    f();
-    return IVH_OK;
-  } catch (const std::invalid_argument & e) {
-    g_err = e.what();
-    return IVH_ERR_INVALID;
-  } catch (const std::runtime_error & e) {
-    g_err = e.what();
-    return std::strncmp(e.what(), "HIP error", 9) == 0 ? IVH_ERR_DEVICE : IVH_ERR_INVALID;
-  } catch (const std::exception & e) {
-    g_err = e.what();
-    return IVH_ERR_INTERNAL;
-  } catch (...) {
-    g_err = "unknown error";
-    return IVH_ERR_INTERNAL;
-  }
+  thread_local std::string e;
+  return e;
 }
+}  // namespace ivh
+
+namespace {
+using ivh::check_launch;
+using ivh::guard;
 
 ivh::Model & M(const ivh_model * m)
 {
@@ -102,12 +91,6 @@ ivh::View tensor_view(const void * ptr, int C, int H, int W, bool nhwc)
   return v;
 }
 
-void check_launch(const char * what)
-{
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) throw std::runtime_error(std::string("HIP error in ") + what + ": " + hipGetErrorString(e));
-}
-
 void check_batch(int batch)
 {
   if (batch < 1 || batch > 65535) throw std::invalid_argument("batch must be in [1, 65535]");
@@ -162,7 +145,7 @@ ivh::View flat_view(const void * ptr, long n)
 
 extern "C" {
 
-const char * ivh_last_error(void) { return g_err.c_str(); }
+const char * ivh_last_error(void) { return ivh::last_error().c_str(); }
 
 int ivh_version(int * major, int * minor)
 {
