@@ -64,29 +64,31 @@ __device__ __forceinline__ u2v read_transposed(const void * at)
 #endif
 }
 
+// What a query at place i sees: keys lo..hi and the first `sinks`.
 struct RaggedMask {
-  int nk, causal, window, sinks;
-  __device__ __forceinline__ bool operator()(int i, int j) const
+  int nk, causal, window, sinks;  // sinks 0 without a window
+  __device__ __forceinline__ int lo(int i) const { return window ? i - window + 1 : 0; }
+  __device__ __forceinline__ int hi(int i) const
   {
-    return j < nk && (!causal || j <= i) && (window == 0 || (i - j < window && j - i < window) || j < sinks);
+    const int h = causal ? i : window ? (int)min((long)i + window - 1, (long)nk) : nk;
+    return min(h, nk - 1);
   }
+  __device__ __forceinline__ bool operator()(int i, int j) const { return (j >= lo(i) && j <= hi(i)) || (j < sinks && (!causal || j <= i) && j < nk); }
   // whether rows imin..imax see all of keys j0..j1, or none of them
   __device__ __forceinline__ bool all(int imin, int imax, int j0, int j1) const
   {
-    return j1 < nk && (!causal || j1 <= imin) &&
-           (window == 0 || (imax - j0 < window && j1 - imin < window) || j1 < sinks);
+    return j1 <= (causal ? min(imin, nk - 1) : nk - 1) && ((j0 >= lo(imax) && j1 <= hi(imin)) || j1 < sinks);
   }
   __device__ __forceinline__ bool none(int imin, int imax, int j0, int j1) const
   {
-    return j0 >= nk || (causal && j0 > imax) ||
-           (window != 0 && j0 >= sinks && (imin - j1 >= window || j0 - imax >= window));
+    return j0 >= nk || (causal && j0 > imax) || (j0 >= sinks && (j1 < lo(imin) || j0 > hi(imax)));
   }
 };
 
 }  // namespace
 
 template <int TYPE, int DP>
-__global__ void __launch_bounds__(256) ragged_attn_kernel(const RaggedParams p, int slots)
+__global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) ragged_attn_kernel(const RaggedParams p, int slots, int round)
 {
   using T = St<TYPE>;
   typedef typename T::e E;
@@ -101,15 +103,27 @@ __global__ void __launch_bounds__(256) ragged_attn_kernel(const RaggedParams p, 
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = lane & 31, hi = lane >> 5;
-  int w = xcd_tile(blockIdx.x, gridDim.x);
-  const int slot = w % slots;
-  w /= slots;
-  const int head = w % p.heads, b = w / p.heads, kvh = head / p.group;
+  // The work-groups of a unit (sequence and key head) run on one XCD, whose L2 they share keys and values in.
+  // Units go round the XCDs where that is even, so that each gets its share of long and short
+  // sequences; a few units are cut into equal runs of work-groups instead.
+  const int unit_wgs = p.group * slots, units = p.batch * (p.heads / p.group);
+  int w = blockIdx.x, unit;
+  if (round) {
+    unit = w / kXcds / unit_wgs * kXcds + w % kXcds;
+    w = w / kXcds % unit_wgs;
+    if (unit >= units) return;
+  } else {
+    w = xcd_tile(w, gridDim.x);
+    unit = w / unit_wgs;
+    w -= unit * unit_wgs;
+  }
+  const int kv_heads = p.heads / p.group, b = unit / kv_heads, kvh = unit - b * kv_heads;
+  const int slot = w % slots, head = kvh * p.group + w / slots;
 
   const int q0 = min(max(p.cu_q[b], 0), p.tokens_q), q1 = min(max(p.cu_q[b + 1], q0), p.tokens_q);
   const int k0 = min(max(p.cu_k[b], 0), p.tokens_k), k1 = min(max(p.cu_k[b + 1], k0), p.tokens_k);
   const int nq = q1 - q0, nk = k1 - k0;
-  const RaggedMask see = {nk, p.causal, p.window, p.sinks};
+  const RaggedMask see = {nk, p.causal, p.window, p.window ? p.sinks : 0};
   const E * kp = static_cast<const E *>(p.k) + (long)k0 * p.k_token + (long)kvh * p.k_head;
   const E * vp = static_cast<const E *>(p.v) + (long)k0 * p.v_token + (long)kvh * p.v_head;
 
@@ -125,6 +139,10 @@ __global__ void __launch_bounds__(256) ragged_attn_kernel(const RaggedParams p, 
     voff[i] = vc * 8 < p.dim ? (unsigned)(row * (int)p.v_token + vc * 8) * 2u : kBufOOB;
   }
 
+  // a negative scale turns the queries' signs, so that the largest score has the largest exponent
+  const float scale = fmaxf(fabsf(p.scale_log2), 1.2e-38f);  // not 0: masked scores stay -inf
+  const unsigned flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
+
   const int nqb = (nq + kRows - 1) / kRows;
   for (int t = slot; t < nqb; t += slots) {
     const int qb = nqb - 1 - t;  // the longest first
@@ -133,13 +151,13 @@ __global__ void __launch_bounds__(256) ragged_attn_kernel(const RaggedParams p, 
     const int wmin = imin + 32 * wave, wmax = min(imax, wmin + 31);  // this wave's rows (none where wmax < wmin)
     const int row = qb * kRows + 32 * wave + col;
     const bool live = row < nq;
-    const int place = live ? row + shift : INT32_MIN / 2;
+    const int place = live ? row + shift : -(1 << 27);
     const E * q = static_cast<const E *>(p.q) + (long)(q0 + row) * p.q_token + (long)head * p.q_head;
     u4v qf[NS];
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       const int ch = 16 * s + 8 * hi;
-      qf[s] = live && ch < p.dim ? *reinterpret_cast<const u4v *>(q + ch) : u4v{0, 0, 0, 0};
+      qf[s] = live && ch < p.dim ? *reinterpret_cast<const u4v *>(q + ch) ^ flip : u4v{0, 0, 0, 0};
     }
 
     // steps: `first` over the first tokens, the others from step `from` on
@@ -162,12 +180,22 @@ __global__ void __launch_bounds__(256) ragged_attn_kernel(const RaggedParams p, 
         copy_to_lds(vs, crow[i] < left ? voff[i] : kBufOOB, V + st * STAGE + 512 * (wave + 4 * i));
     };
 
+    // what this lane's row sees, less the lane's first key of a 32-key block
+    const int seen_lo = see.lo(place) - 4 * hi, seen_n = see.hi(place) - see.lo(place);
+    const int seen_first = min(see.sinks, see.causal ? place + 1 : see.nk) - 4 * hi;
+
     f16v o[NB];
+    float M, L;
+    // An infinity or NaN among the values reaches rows that do not see it, as 0 x inf, and stays in
+    // their sums.  So rows are first taken as they come; only if a result is not finite are they taken again
+    // with such values left out of the product and added to the rows that do see them.
+    for (int careful = 0; careful < 2; ++careful) {
 #pragma unroll
     for (int j = 0; j < NB; ++j) o[j] = f16v{};
-    float M = kLowest, L = 0.0f;
+    M = kLowest;
+    L = 0.0f;
 
-    __syncthreads();  // the last row block's stages are no longer read
+    __syncthreads();  // the last rows' stages are no longer read
     if (total > 0) copy(0);
     for (int n = 0; n < total; ++n) {
       __builtin_amdgcn_s_waitcnt(vm_wait(0));
@@ -190,17 +218,22 @@ __global__ void __launch_bounds__(256) ragged_attn_kernel(const RaggedParams p, 
           s[kb] = T::mma32(a, qf[i], s[kb]);
         }
       }
+      if (!inner) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const int j = key0 + 32 * kb + 8 * (v / 4) + v % 4;
+            const bool ok = (seen_n >= 0 && (unsigned)j - (unsigned)seen_lo <= (unsigned)seen_n) || j < seen_first;
+            s[kb][v] = ok ? s[kb][v] : -__builtin_inff();
+          }
+      }
       float top = -__builtin_inff();
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          float x = s[kb][v] * p.scale_log2;
-          if (!inner && !see(place, key0 + 32 * kb + 8 * (v / 4) + 4 * hi + v % 4)) x = -__builtin_inff();
-          s[kb][v] = x;
-          top = fmaxf(top, x);
-        }
-      top = across32(top, MaxOp());
+        for (int v = 0; v < 16; ++v) top = fmaxf(top, s[kb][v]);
+      top = across32(top, MaxOp()) * scale;
       // the reference exponent follows the maximum only when that is 2^8 above it: weights up to
       // 2^8 lose nothing in either 16-bit type
       if (__any(top > M + 8.0f)) {
@@ -218,7 +251,8 @@ __global__ void __launch_bounds__(256) ragged_attn_kernel(const RaggedParams p, 
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int v = 0; v < 16; v += 2) {
-          const float x = __builtin_amdgcn_exp2f(s[kb][v] - M), y = __builtin_amdgcn_exp2f(s[kb][v + 1] - M);
+          const float x = __builtin_amdgcn_exp2f(fmaf(s[kb][v], scale, -M));
+          const float y = __builtin_amdgcn_exp2f(fmaf(s[kb][v + 1], scale, -M));
           sum += x + y;
           pf[2 * kb + v / 8][v % 8 / 2] = pack2<TYPE>(x, y);
         }
@@ -238,15 +272,12 @@ __global__ void __launch_bounds__(256) ragged_attn_kernel(const RaggedParams p, 
         }
         return a;
       };
-      if (inner) {
+      if (inner || !careful) {
 #pragma unroll
         for (int sl = 0; sl < 4; ++sl)
 #pragma unroll
           for (int j = 0; j < NB; ++j) o[j] = T::mma32(values(sl, j), pf[sl], o[j]);
       } else {
-        // some row does not see some key: an infinity or NaN among the values would reach rows
-        // that do not see it, as 0 x inf.  Such values are left out of the product and added to
-        // the rows that do.
         unsigned odd = 0;
 #pragma unroll
         for (int sl = 0; sl < 4; ++sl)
@@ -278,6 +309,13 @@ __global__ void __launch_bounds__(256) ragged_attn_kernel(const RaggedParams p, 
     }
 
     L = across32(L, SumOp());
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) odd = odd || !(fabsf(o[j][v]) < __builtin_inff());
+    if (!__syncthreads_or(odd)) break;
+    }
     if (live) {
       const float inv = L != 0.0f ? 1.0f / L : 0.0f;  // a row that saw nothing is zero (NaN stays)
       E * out = static_cast<E *>(p.o) + (long)(q0 + row) * p.o_token + (long)head * p.o_head;
@@ -307,9 +345,11 @@ template <int TYPE, int DP> void launch_ragged(const RaggedParams & p, hipStream
   // max_q only sizes the grid: a work-group takes every slots-th row block of its sequence.  A
   // launch holds 2^24 work-groups of 256 lanes.
   const long heads = (long)p.batch * p.heads;
-  const int slots = (int)std::min<long>((std::max(1, std::min(p.max_q, p.tokens_q)) + kRows - 1) / kRows, (1L << 24) / heads);
-  const long wgs = heads * slots;
-  hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(256), lds, s, p, slots);
+  const int slots = (int)std::min<long>((std::max(1, std::min(p.max_q, p.tokens_q)) + kRows - 1) / kRows, (1L << 24) / (heads + kXcds * p.group));
+  const long units = heads / p.group;
+  const int round = units % kXcds == 0 || units >= 4 * kXcds;
+  const long wgs = (round ? (units + kXcds - 1) / kXcds * kXcds : units) * p.group * slots;
+  hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(256), lds, s, p, slots, round);
 }
 
 template <int TYPE> void launch_ragged_dim(const RaggedParams & p, hipStream_t s)

@@ -2,6 +2,7 @@
 // is checked before anything is enqueued.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <initializer_list>
@@ -96,6 +97,8 @@ ivh::RotParams rotation(const ivh_rotation & r, int dim, const int32_t * pos, in
 }
 
 constexpr int kMaxTokens = 1 << 26, kMaxBatch = 1 << 20;
+// a larger window hides nothing either; with it a place less the window stays within 32 bits
+constexpr int kMaxWindow = INT32_MAX - 2 * kMaxTokens;
 
 void check_counts(int batch, int tokens)
 {
@@ -158,7 +161,7 @@ ivh::PagedParams paged(const ivh_paged_attn_desc * d, int batch, int tokens, siz
   p.heads = d->heads;
   p.group = d->heads / d->cache.heads;
   p.scale_log2 = d->scale * kLog2E;
-  p.window = d->window;
+  p.window = std::min(d->window, kMaxWindow);
   p.sinks = d->sinks;
   const int max_new = d->max_new ? d->max_new : tokens;
   const int max_len = d->max_len ? d->max_len : d->cache.table_width * d->cache.page;
@@ -307,7 +310,7 @@ int ivh_attention(const ivh_attn_desc * d, const void * q, const void * k, const
     p.tokens_k = tokens_k;
     p.max_q = d->max_q ? d->max_q : tokens_q;
     p.causal = d->causal != 0;
-    p.window = d->window;
+    p.window = std::min(d->window, kMaxWindow);
     p.sinks = d->sinks;
     p.scale_log2 = d->scale * kLog2E;
     p.q = q;
