@@ -30,7 +30,6 @@ typedef __attribute__((address_space(3))) void lds_ptr;
 typedef short s4v __attribute__((ext_vector_type(4)));
 
 constexpr int kKeys = 64;   // keys of a step
-constexpr int kRows = 128;  // rows of a work-group
 
 // position of 16-byte piece c of row r in a row of DP / 8 pieces (its own inverse)
 template <int DP> __device__ __forceinline__ int key_piece(int r, int c)
@@ -46,10 +45,10 @@ template <int DP> __device__ __forceinline__ int value_piece(int r, int c)
   return c;
 }
 
-// 64 x 16 bytes straight into LDS: lane i's from base + its offset (zeros where that is kBufOOB) to lds + 16 i
-__device__ __forceinline__ void copy_to_lds(const void * base, unsigned off, void * lds)
+// 64 x 16 bytes straight into LDS: lane i's from base + its offset, zeros from `bytes` on, to lds + 16 i
+__device__ __forceinline__ void copy_to_lds(const void * base, unsigned bytes, unsigned off, void * lds)
 {
-  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), (short)0, 0x7fffffff, kBufDword3);
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), (short)0, (int)bytes, kBufDword3);
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr *)lds, 16, (int)off, 0, 0, 0);
 }
 
@@ -62,6 +61,26 @@ __device__ __forceinline__ u2v read_transposed(const void * at)
 #else
   return u2v{};
 #endif
+}
+
+// LDS byte offsets of a lane's fragment pieces: of channels 16 i + 8 (lane / 32) of a key row, and
+// of channel block j of a value row.  The permuted bits lie below a row's, so pieces differ by an
+// exclusive or of those and a constant.
+template <int DP> __device__ __forceinline__ unsigned key_at(unsigned base, int i)
+{
+  constexpr int BITS = DP % 128 == 0 ? 4 : DP % 64 == 0 ? 3 : 2;
+  return (base ^ (32u * (i & ((1 << (BITS - 1)) - 1)))) + (unsigned)(2 * i >> BITS) * (16u << BITS);
+}
+template <int DP> __device__ __forceinline__ unsigned value_at(unsigned base, int j)
+{
+  constexpr int BITS = DP % 128 == 0 ? 2 : DP % 64 == 0 ? 1 : 0;
+  return (base ^ (64u * (j & ((1 << BITS) - 1)))) + (unsigned)(j >> BITS) * (64u << BITS);
+}
+
+// the largest of three, NaN if one is: one instruction
+__device__ __forceinline__ float top_of(float a, float b, float c)
+{
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 
 // What a query at place i sees: keys lo..hi and the first `sinks`.
@@ -85,23 +104,30 @@ struct RaggedMask {
   }
 };
 
+// waves per SIMD that the registers of a build are to allow
+constexpr int ragged_waves(int dp, int qt) { return qt == 1 ? (dp <= 32 ? 3 : dp <= 128 ? 2 : 1) : dp <= 64 ? 2 : 1; }
+
 }  // namespace
 
-template <int TYPE, int DP>
-__global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) ragged_attn_kernel(const RaggedParams p, int slots, int round)
+// QT: 32-row tiles of a wave.
+template <int TYPE, int DP, int QT>
+__global__ void __launch_bounds__(256, ragged_waves(DP, QT)) ragged_attn_kernel(const RaggedParams p, int slots, int round)
 {
   using T = St<TYPE>;
   typedef typename T::e E;
   constexpr int NS = DP / 16;          // 16-channel slices of the first product
   constexpr int NB = DP / 32;          // 32-channel blocks of the second
   constexpr int PR = DP / 8;           // 16-byte pieces of a row
-  constexpr int NI = kKeys * PR / 256; // copies of a wave, keys or values of a step
-  constexpr int STAGE = kKeys * DP;
-  extern __shared__ __attribute__((aligned(16))) unsigned char lds_raw[];
-  E * const K = reinterpret_cast<E *>(lds_raw);  // [2][64][DP]
-  E * const V = K + 2 * STAGE;
+  constexpr int VI = kKeys * PR / 256; // copies of a wave: values of a step,
+  constexpr int KC = 32 * PR / 64, KI = (KC + 3) / 4;  // keys of a block (KC in all)
+  constexpr int STAGE = kKeys * DP, BLOCK = 32 * DP;
+  constexpr int WR = 32 * QT, kRows = 4 * WR;  // rows of a wave, of the work-group
+  // keys: a ring of four 32-key blocks; values: two stages of 64.  Arrays of their own, so that the
+  // compiler sees that a copy into one does not touch the others and leaves it in flight.
+  __shared__ __attribute__((aligned(16))) unsigned char K0[BLOCK * 2], K1[BLOCK * 2], K2[BLOCK * 2], K3[BLOCK * 2];
+  __shared__ __attribute__((aligned(16))) unsigned char V0[STAGE * 2], V1[STAGE * 2];
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, hi = lane >> 5;
   // The work-groups of a unit (sequence and key head) run on one XCD, whose L2 they share keys and values in.
   // Units go round the XCDs where that is even, so that each gets its share of long and short
@@ -128,36 +154,42 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) ragged_
   const E * vp = static_cast<const E *>(p.v) + (long)k0 * p.v_token + (long)kvh * p.v_head;
 
   // what this lane copies: position pos of row `row` of the stage holds a piece of the key's row
-  unsigned koff[NI], voff[NI];
-  int crow[NI];
+  unsigned koff[KI], voff[VI];
 #pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    const int s = 64 * (wave + 4 * i) + lane, row = s / PR, pos = s - row * PR;
-    const int kc = key_piece<DP>(row, pos), vc = value_piece<DP>(row, pos);
-    crow[i] = row;
-    koff[i] = kc * 8 < p.dim ? (unsigned)(row * (int)p.k_token + kc * 8) * 2u : kBufOOB;
-    voff[i] = vc * 8 < p.dim ? (unsigned)(row * (int)p.v_token + vc * 8) * 2u : kBufOOB;
+  for (int i = 0; i < KI; ++i) {
+    const int s = 64 * (wave + 4 * i) + lane, row = s / PR, c = key_piece<DP>(row, s - row * PR);
+    koff[i] = c * 8 < p.dim ? (unsigned)(row * (int)p.k_token + c * 8) * 2u : kBufOOB;
   }
-
+#pragma unroll
+  for (int i = 0; i < VI; ++i) {
+    const int s = 64 * (wave + 4 * i) + lane, row = s / PR, c = value_piece<DP>(row, s - row * PR);
+    voff[i] = c * 8 < p.dim ? (unsigned)(row * (int)p.v_token + c * 8) * 2u : kBufOOB;
+  }
   // a negative scale turns the queries' signs, so that the largest score has the largest exponent
   const float scale = fmaxf(fabsf(p.scale_log2), 1.2e-38f);  // not 0: masked scores stay -inf
   const unsigned flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
+
+  const unsigned kaddr = (unsigned)(col * DP + key_piece<DP>(col, hi) * 8) * 2u;
+  const int tr = (lane & 15) >> 2;
+  const unsigned vaddr =
+      (unsigned)((4 * hi + tr) * DP + value_piece<DP>(tr, 2 * (lane >> 4 & 1) + ((lane & 3) >> 1)) * 8 + (lane & 1) * 4) * 2u;
 
   const int nqb = (nq + kRows - 1) / kRows;
   for (int t = slot; t < nqb; t += slots) {
     const int qb = nqb - 1 - t;  // the longest first
     const int shift = nk - nq;
     const int imin = qb * kRows + shift, imax = min(nq - 1, qb * kRows + kRows - 1) + shift;
-    const int wmin = imin + 32 * wave, wmax = min(imax, wmin + 31);  // this wave's rows (none where wmax < wmin)
-    const int row = qb * kRows + 32 * wave + col;
-    const bool live = row < nq;
-    const int place = live ? row + shift : -(1 << 27);
-    const E * q = static_cast<const E *>(p.q) + (long)(q0 + row) * p.q_token + (long)head * p.q_head;
-    u4v qf[NS];
+    const int wmin = imin + WR * wave, wmax = min(imax, wmin + WR - 1);  // this wave's rows (none where wmax < wmin)
+    const int row = qb * kRows + WR * wave + col;                        // this lane's in each tile: row + 32 u
+    u4v qf[QT][NS];
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      const int ch = 16 * s + 8 * hi;
-      qf[s] = live && ch < p.dim ? *reinterpret_cast<const u4v *>(q + ch) ^ flip : u4v{0, 0, 0, 0};
+    for (int u = 0; u < QT; ++u) {
+      const E * q = static_cast<const E *>(p.q) + (long)(q0 + row + 32 * u) * p.q_token + (long)head * p.q_head;
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const int ch = 16 * s + 8 * hi;
+        qf[u][s] = row + 32 * u < nq && ch < p.dim ? *reinterpret_cast<const u4v *>(q + ch) ^ flip : u4v{0, 0, 0, 0};
+      }
     }
 
     // steps: `first` over the first tokens, the others from step `from` on
@@ -169,163 +201,257 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) ragged_
     const int total = end > 0 ? first + (end + kKeys - 1) / kKeys - from : 0;
     auto key_of = [&](int n) { return kKeys * (n < first ? n : from + n - first); };
 
-    auto copy = [&](int n) __attribute__((always_inline)) {
-      const int key0 = key_of(n), left = nk - key0, st = n & 1;
-      const E * ks = kp + (long)key0 * p.k_token, * vs = vp + (long)key0 * p.v_token;
+    // keys of block g (32 of step g / 2) into slot sl of the ring; values of step n into stage st
+    auto copy_keys = [&](int g, auto sl) __attribute__((always_inline)) {
+      if (g >= 2 * total) return;
+      const int key = key_of(g >> 1) + 32 * (g & 1), left = min(nk - key, 32);
+      const unsigned bytes = left > 0 ? (unsigned)((left - 1) * (int)p.k_token + p.dim) * 2u : 0u;  // none behind the last key
+      const E * at = kp + (long)key * p.k_token;
+      unsigned char * to = sl == 0 ? K0 : sl == 1 ? K1 : sl == 2 ? K2 : K3;
 #pragma unroll
-      for (int i = 0; i < NI; ++i)
-        copy_to_lds(ks, crow[i] < left ? koff[i] : kBufOOB, K + st * STAGE + 512 * (wave + 4 * i));
-#pragma unroll
-      for (int i = 0; i < NI; ++i)
-        copy_to_lds(vs, crow[i] < left ? voff[i] : kBufOOB, V + st * STAGE + 512 * (wave + 4 * i));
+      for (int i = 0; i < KI; ++i)
+        if (4 * i + 3 < KC || wave + 4 * i < KC) copy_to_lds(at, bytes, koff[i], to + 1024 * (wave + 4 * i));
     };
-
-    // what this lane's row sees, less the lane's first key of a 32-key block
-    const int seen_lo = see.lo(place) - 4 * hi, seen_n = see.hi(place) - see.lo(place);
-    const int seen_first = min(see.sinks, see.causal ? place + 1 : see.nk) - 4 * hi;
-
-    f16v o[NB];
-    float M, L;
-    // An infinity or NaN among the values reaches rows that do not see it, as 0 x inf, and stays in
-    // their sums.  So rows are first taken as they come; only if a result is not finite are they taken again
-    // with such values left out of the product and added to the rows that do see them.
-    for (int careful = 0; careful < 2; ++careful) {
+    auto copy_values = [&](int n, auto st) __attribute__((always_inline)) {
+      if (n >= total) return;
+      const unsigned bytes = (unsigned)((min(nk - key_of(n), kKeys) - 1) * (int)p.v_token + p.dim) * 2u;
+      const E * at = vp + (long)key_of(n) * p.v_token;
 #pragma unroll
-    for (int j = 0; j < NB; ++j) o[j] = f16v{};
-    M = kLowest;
-    L = 0.0f;
-
-    __syncthreads();  // the last rows' stages are no longer read
-    if (total > 0) copy(0);
-    for (int n = 0; n < total; ++n) {
-      __builtin_amdgcn_s_waitcnt(vm_wait(0));
-      __syncthreads();
-      if (n + 1 < total) copy(n + 1);
-      const int key0 = key_of(n);
-      if (wmax < wmin || see.none(wmin, wmax, key0, key0 + kKeys - 1)) continue;
-      const bool inner = see.all(wmin, wmax, key0, key0 + kKeys - 1);
-      const E * Ks = K + (n & 1) * STAGE;
-      const E * Vs = V + (n & 1) * STAGE;
-
-      f16v s[2];
+      for (int i = 0; i < VI; ++i)
+        copy_to_lds(at, bytes, voff[i], (st ? V1 : V0) + 1024 * (wave + 4 * i));
+    };
+    // what this lane's rows see, less the lane's first key of a 32-key block
+    int seen_lo[QT], seen_n[QT], seen_first[QT];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        s[kb] = f16v{};
-        const int r = 32 * kb + col;
+    for (int u = 0; u < QT; ++u) {
+      const int place = row + 32 * u < nq ? row + 32 * u + shift : -(1 << 27);
+      seen_lo[u] = see.lo(place) - 4 * hi;
+      seen_n[u] = see.hi(place) - see.lo(place);
+      seen_first[u] = min(see.sinks, see.causal ? place + 1 : see.nk) - 4 * hi;
+    }
+    auto none_of = [&](int n) { return wmax < wmin || see.none(wmin, wmax, key_of(n), key_of(n) + kKeys - 1); };
+
+    f16v o[QT][NB], s0[QT], s1[QT];
+    float M[QT], L[QT];
+    auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < NS; ++i) {
-          const u4v a = *reinterpret_cast<const u4v *>(Ks + r * DP + key_piece<DP>(r, 2 * i + hi) * 8);
-          s[kb] = T::mma32(a, qf[i], s[kb]);
-        }
+      for (int u = 0; u < QT; ++u) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) o[u][j] = f16v{};
+        M[u] = kLowest;
+        L[u] = 0.0f;
       }
+    };
+    // fragment of channels 16 i .. of the keys in ring slot sl; of the values of keys 16 q .. and channels
+    // 32 j .. in stage st, two transposing loads of 4 keys each
+    auto key_piece_of = [&](auto sl, int i) __attribute__((always_inline)) {
+      return *reinterpret_cast<const u4v *>((sl == 0 ? K0 : sl == 1 ? K1 : sl == 2 ? K2 : K3) + key_at<DP>(kaddr, i));
+    };
+    auto value_piece_of = [&](auto st, int q, int j) __attribute__((always_inline)) {
+      const unsigned char * at = (st ? V1 : V0) + value_at<DP>(vaddr, j) + 32 * q * DP;
+      const u2v x = read_transposed(at), y = read_transposed(at + 16 * DP);
+      return u4v{x[0], x[1], y[0], y[1]};
+    };
+    // S^T of the 32 keys in slot sl
+    auto scores = [&](auto sl, f16v (&s)[QT]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        const u4v a = key_piece_of(sl, i);
+#pragma unroll
+        for (int u = 0; u < QT; ++u) s[u] = T::mma32(a, qf[u][i], i ? s[u] : f16v{});
+      }
+    };
+    // scores of keys (from key0 on) that a row does not see become -inf; the reference exponent follows the
+    // running maximum only when that is 2^8 above it: weights up to 2^8 lose nothing in either 16-bit type
+    auto settle = [&](int key0, bool inner, f16v (&s)[QT]) __attribute__((always_inline)) {
       if (!inner) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int u = 0; u < QT; ++u)
 #pragma unroll
           for (int v = 0; v < 16; ++v) {
-            const int j = key0 + 32 * kb + 8 * (v / 4) + v % 4;
-            const bool ok = (seen_n >= 0 && (unsigned)j - (unsigned)seen_lo <= (unsigned)seen_n) || j < seen_first;
-            s[kb][v] = ok ? s[kb][v] : -__builtin_inff();
+            const int j = key0 + 8 * (v / 4) + v % 4;
+            const bool ok = (seen_n[u] >= 0 && (unsigned)j - (unsigned)seen_lo[u] <= (unsigned)seen_n[u]) || j < seen_first[u];
+            s[u][v] = ok ? s[u][v] : -__builtin_inff();
           }
       }
-      float top = -__builtin_inff();
+      float top[QT];
+      bool grow = false;
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+      for (int u = 0; u < QT; ++u) {
+        float a = s[u][0], b = s[u][1];
 #pragma unroll
-        for (int v = 0; v < 16; ++v) top = fmaxf(top, s[kb][v]);
-      top = across32(top, MaxOp()) * scale;
-      // the reference exponent follows the maximum only when that is 2^8 above it: weights up to
-      // 2^8 lose nothing in either 16-bit type
-      if (__any(top > M + 8.0f)) {
-        const float m = fmaxf(M, top), a = __builtin_amdgcn_exp2f(M - m);
-        M = m;
-        L *= a;
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) o[j][v] *= a;
+        for (int v = 2; v < 16; v += 4) {
+          a = top_of(a, s[u][v], s[u][v + 1]);
+          if (v + 2 < 16) b = top_of(b, s[u][v + 2], s[u][v + 3]);
+        }
+        top[u] = across32(top_of(a, b, b), MaxOp()) * scale;
+        grow = grow || top[u] > M[u] + 8.0f;
       }
-      u4v pf[4];
-      float sum = 0.0f;
+      if (__any(grow)) {
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+        for (int u = 0; u < QT; ++u) {
+          const float m = fmaxf(M[u], top[u]), a = __builtin_amdgcn_exp2f(M[u] - m);
+          M[u] = m;
+          L[u] *= a;
 #pragma unroll
-        for (int v = 0; v < 16; v += 2) {
-          const float x = __builtin_amdgcn_exp2f(fmaf(s[kb][v], scale, -M));
-          const float y = __builtin_amdgcn_exp2f(fmaf(s[kb][v + 1], scale, -M));
-          sum += x + y;
-          pf[2 * kb + v / 8][v % 8 / 2] = pack2<TYPE>(x, y);
+          for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[u][j][v] *= a;
         }
-      L += sum;
-
-      // V^T fragment of 16 keys and 32 channels: two transposing loads of 4 keys each
-      auto values = [&](int sl, int j) __attribute__((always_inline)) {
-        u4v a;
+      }
+    };
+    // weights of score pairs [from, to) of the tiles' 8 each, two 16-bit values a pair; their sum is of
+    // the rounded ones, which are what the values get
+    auto weights = [&](const f16v (&s)[QT], u4v (&pf)[QT][2], int from, int to) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int r = 16 * sl + 8 * u + 4 * hi + ((lane & 15) >> 2);
-          const int pc = 4 * j + 2 * (lane >> 4 & 1) + ((lane & 3) >> 1);
-          const E * at = Vs + r * DP + value_piece<DP>(r, pc) * 8 + (lane & 1) * 4;
-          const u2v y = read_transposed(at);
-          a[2 * u] = y[0];
-          a[2 * u + 1] = y[1];
-        }
-        return a;
+      for (int k = from; k < to; ++k) {
+        const int u = k % QT, i = k / QT;
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[u][2 * i], scale, -M[u]));
+        const float y = __builtin_amdgcn_exp2f(fmaf(s[u][2 * i + 1], scale, -M[u]));
+        const unsigned w = pack2<TYPE>(x, y);
+        L[u] = T::add2(w, L[u]);
+        pf[u][i / 4][i % 4] = w;
+      }
+    };
+    // 32 keys, half kb of the step in stage st.  The matrix cores form the scores of the next 32 (in
+    // slot nsl) while the vector unit turns these into weights, then take the values.  The order is
+    // pinned slot by slot, with fragments read ahead.
+    auto block = [&](auto st, auto kb, auto nsl, int key0, bool inner, f16v (&s)[QT], f16v (&next)[QT]) __attribute__((always_inline)) {
+      // slots: the next keys' products, then the values'; fragment i is read R - 1 slots before its slot
+      constexpr int Q = NS, W = 2 * NB, R = 5;
+      u4v pf[QT][2], f[R];
+      auto read = [&](auto i) __attribute__((always_inline)) {
+        if constexpr (i < Q) f[i % R] = key_piece_of(nsl, i);
+        else if constexpr (i < Q + W) f[i % R] = value_piece_of(st, 2 * kb + (i - Q) / NB, (i - Q) % NB);
       };
-      if (inner || !careful) {
-#pragma unroll
-        for (int sl = 0; sl < 4; ++sl)
-#pragma unroll
-          for (int j = 0; j < NB; ++j) o[j] = T::mma32(values(sl, j), pf[sl], o[j]);
-      } else {
-        unsigned odd = 0;
-#pragma unroll
-        for (int sl = 0; sl < 4; ++sl)
-#pragma unroll
-          for (int j = 0; j < NB; ++j) {
-            u4v a = values(sl, j);
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const unsigned d = T::odd_bits(a[x]);
-              odd |= d;
-              a[x] &= ~((d >> 15) * 0xffffu);
-            }
-            o[j] = T::mma32(a, pf[sl], o[j]);
-          }
-        if (__any(odd != 0)) {
-          for (int r = 0; r < kKeys; ++r) {
-            const bool mine = see(place, key0 + r);
-#pragma unroll
-            for (int j = 0; j < NB; ++j)
-#pragma unroll
-              for (int v = 0; v < 16; ++v) {
-                const int ch = 32 * j + 8 * (v / 4) + 4 * hi + v % 4;
-                const float x = (float)Vs[r * DP + value_piece<DP>(r, ch / 8) * 8 + ch % 8];
-                if (mine && !(fabsf(x) < __builtin_inff())) o[j][v] += x;
-              }
-          }
-        }
+      static_for<0, R - 1>(read);
+      settle(key0, inner, s);
+      __builtin_amdgcn_sched_barrier(0);
+      static_for<0, Q>([&](auto i) __attribute__((always_inline)) {
+        read(std::integral_constant<int, i + R - 1>{});
+        static_for<0, QT>([&](auto u) __attribute__((always_inline)) {
+          if constexpr (i == 0) next[u] = T::mma32(f[0], qf[u][0], f16v{});
+          else next[u] = T::mma32(f[i % R], qf[u][i], next[u]);
+          constexpr int at = i * QT + u;
+          weights(s, pf, at * 8 / Q, (at + 1) * 8 / Q);
+          __builtin_amdgcn_sched_barrier(0);
+        });
+      });
+      static_for<0, W>([&](auto i) __attribute__((always_inline)) {
+        read(std::integral_constant<int, Q + i + R - 1>{});
+        static_for<0, QT>([&](auto u) __attribute__((always_inline)) {
+          o[u][i % NB] = T::mma32(f[(Q + i) % R], pf[u][i / NB], o[u][i % NB]);
+        });
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    };
+    constexpr std::integral_constant<int, 0> c0{};
+    constexpr std::integral_constant<int, 1> c1{};
+    constexpr std::integral_constant<int, 2> c2{};
+    constexpr std::integral_constant<int, 3> c3{};
+    // Step n in value stage st, whose first 32 scores are there; x, y: ring slots of the two key blocks
+    // it multiplies, behind the ones it weighs; z, w: the slots that take the two after those.
+    auto step = [&](int n, auto st, auto nst, auto x, auto y, auto z, auto w) __attribute__((always_inline)) {
+      __builtin_amdgcn_s_waitcnt(vm_wait(0));
+      __syncthreads();
+      copy_keys(2 * n + 3, z);
+      copy_keys(2 * n + 4, w);
+      copy_values(n + 1, nst);
+      const int key0 = key_of(n);
+      const bool inner = see.all(wmin, wmax, key0, key0 + kKeys - 1);
+      block(st, c0, x, key0, inner, s0, s1);
+      block(st, c1, y, key0 + 32, inner, s1, s0);  // after the last step s0 is of no use (whatever the slot holds)
+    };
+
+    __syncthreads();  // the last rows' stages are no longer read
+    clear();
+    if (total > 0) {
+      copy_keys(0, c0);
+      __builtin_amdgcn_s_waitcnt(vm_wait(0));
+      __syncthreads();
+      copy_keys(1, c1);
+      copy_keys(2, c2);
+      copy_values(0, c0);
+      scores(c0, s0);
+      for (int n = 0; n < total; n += 2) {
+        step(n, c0, c1, c1, c2, c3, c0);
+        if (n + 1 < total) step(n + 1, c1, c0, c3, c0, c1, c2);
       }
     }
 
-    L = across32(L, SumOp());
+    // An infinity or NaN among the values reaches rows that do not see it, as 0 x inf, and stays
+    // in their sums.  If a result is not finite the rows are taken again, one step at a time, with such
+    // values left out of the product and added to the rows that do see them.
     bool odd = false;
 #pragma unroll
-    for (int j = 0; j < NB; ++j)
+    for (int u = 0; u < QT; ++u)
 #pragma unroll
-      for (int v = 0; v < 16; ++v) odd = odd || !(fabsf(o[j][v]) < __builtin_inff());
-    if (!__syncthreads_or(odd)) break;
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) odd = odd || !(fabsf(o[u][j][v]) < __builtin_inff());
+    if (__syncthreads_or(odd)) {
+      clear();
+      for (int n = 0; n < total; ++n) {
+        __syncthreads();
+        copy_keys(2 * n, c0);
+        copy_keys(2 * n + 1, c1);
+        copy_values(n, c0);
+        __builtin_amdgcn_s_waitcnt(vm_wait(0));
+        __syncthreads();
+        if (none_of(n)) continue;
+        const bool inner = see.all(wmin, wmax, key_of(n), key_of(n) + kKeys - 1);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          u4v pf[QT][2];
+          if (kb) scores(c1, s0);
+          else scores(c0, s0);
+          settle(key_of(n) + 32 * kb, inner, s0);
+          weights(s0, pf, 0, 8 * QT);
+#pragma unroll
+          for (int sl = 0; sl < 2; ++sl)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+              u4v a = value_piece_of(c0, 2 * kb + sl, j);
+#pragma unroll
+              for (int x = 0; x < 4; ++x) a[x] &= ~((T::odd_bits(a[x]) >> 15) * 0xffffu);
+#pragma unroll
+              for (int u = 0; u < QT; ++u) o[u][j] = T::mma32(a, pf[u][sl], o[u][j]);
+            }
+        }
+        const E * Vs = reinterpret_cast<const E *>(V0);
+        for (int r = 0; r < kKeys; ++r) {
+          bool mine[QT];
+#pragma unroll
+          for (int u = 0; u < QT; ++u) mine[u] = row + 32 * u < nq && see(row + 32 * u + shift, key_of(n) + r);
+#pragma unroll
+          for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+              const int ch = 32 * j + 8 * (v / 4) + 4 * hi + v % 4;
+              const float x = (float)Vs[r * DP + value_piece<DP>(r, ch / 8) * 8 + ch % 8];
+              if (fabsf(x) < __builtin_inff()) continue;
+#pragma unroll
+              for (int u = 0; u < QT; ++u)
+                if (mine[u]) o[u][j][v] += x;
+            }
+        }
+      }
     }
-    if (live) {
-      const float inv = L != 0.0f ? 1.0f / L : 0.0f;  // a row that saw nothing is zero (NaN stays)
-      E * out = static_cast<E *>(p.o) + (long)(q0 + row) * p.o_token + (long)head * p.o_head;
+
+#pragma unroll
+    for (int u = 0; u < QT; ++u) {
+      const float sum = across32(L[u], SumOp());
+      if (row + 32 * u >= nq) continue;
+      const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;  // a row that saw nothing is zero (NaN stays)
+      E * out = static_cast<E *>(p.o) + (long)(q0 + row + 32 * u) * p.o_token + (long)head * p.o_head;
 #pragma unroll
       for (int j = 0; j < NB; ++j)
 #pragma unroll
         for (int v = 0; v < 16; v += 4) {
           const int ch = 32 * j + 2 * v + 4 * hi;
           if (ch >= p.dim) continue;
-          const u2v y = {pack2<TYPE>(o[j][v] * inv, o[j][v + 1] * inv), pack2<TYPE>(o[j][v + 2] * inv, o[j][v + 3] * inv)};
+          const f16v & x = o[u][j];
+          const u2v y = {pack2<TYPE>(x[v] * inv, x[v + 1] * inv), pack2<TYPE>(x[v + 2] * inv, x[v + 3] * inv)};
           *reinterpret_cast<u2v *>(out + ch) = y;
         }
     }
@@ -334,14 +460,9 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) ragged_
 
 namespace {
 
-template <int TYPE, int DP> void launch_ragged(const RaggedParams & p, hipStream_t s)
+template <int TYPE, int DP, int QT> void launch_ragged(const RaggedParams & p, hipStream_t s)
 {
-  auto kern = ragged_attn_kernel<TYPE, DP>;
-  const size_t lds = (size_t)4 * kKeys * DP * 2;
-  if (lds > 65536) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) throw std::runtime_error(std::string("HIP error: ") + hipGetErrorString(e));
-  }
+  constexpr int kRows = 128 * QT;
   // max_q only sizes the grid: a work-group takes every slots-th row block of its sequence.  A
   // launch holds 2^24 work-groups of 256 lanes.
   const long heads = (long)p.batch * p.heads;
@@ -349,17 +470,18 @@ template <int TYPE, int DP> void launch_ragged(const RaggedParams & p, hipStream
   const long units = heads / p.group;
   const int round = units % kXcds == 0 || units >= 4 * kXcds;
   const long wgs = (round ? (units + kXcds - 1) / kXcds * kXcds : units) * p.group * slots;
-  hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(256), lds, s, p, slots, round);
+  hipLaunchKernelGGL((ragged_attn_kernel<TYPE, DP, QT>), dim3((unsigned)wgs), dim3(256), 0, s, p, slots, round);
 }
 
 template <int TYPE> void launch_ragged_dim(const RaggedParams & p, hipStream_t s)
 {
-  if (p.dim <= 32) launch_ragged<TYPE, 32>(p, s);
-  else if (p.dim <= 64) launch_ragged<TYPE, 64>(p, s);
-  else if (p.dim <= 96) launch_ragged<TYPE, 96>(p, s);
-  else if (p.dim <= 128) launch_ragged<TYPE, 128>(p, s);
-  else if (p.dim <= 192) launch_ragged<TYPE, 192>(p, s);
-  else launch_ragged<TYPE, 256>(p, s);
+  const bool wide = getenv("QT2") != nullptr;
+  if (p.dim <= 32) launch_ragged<TYPE, 32, 1>(p, s);
+  else if (p.dim <= 64) wide ? launch_ragged<TYPE, 64, 2>(p, s) : launch_ragged<TYPE, 64, 1>(p, s);
+  else if (p.dim <= 96) wide ? launch_ragged<TYPE, 96, 2>(p, s) : launch_ragged<TYPE, 96, 1>(p, s);
+  else if (p.dim <= 128) wide ? launch_ragged<TYPE, 128, 2>(p, s) : launch_ragged<TYPE, 128, 1>(p, s);
+  else if (p.dim <= 192) launch_ragged<TYPE, 192, 1>(p, s);
+  else launch_ragged<TYPE, 256, 1>(p, s);
 }
 
 }  // namespace

@@ -37,6 +37,10 @@ template <> struct St<kSeqF16> {
   {
     return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, true));
   }
+  static __device__ __forceinline__ float add2(unsigned x, float c)  // c + both halves
+  {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(e2, x), __builtin_bit_cast(e2, 0x3c003c00u), c, false);
+  }
   // which halves of x are infinite or NaN: their top bits
   static __device__ __forceinline__ unsigned odd_bits(unsigned x) { return ((x & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }
 };
@@ -59,6 +63,10 @@ template <> struct St<kSeqBF16> {
   static __device__ __forceinline__ unsigned fp8_hi(unsigned x)
   {
     return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, true));
+  }
+  static __device__ __forceinline__ float add2(unsigned x, float c)
+  {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(e2, x), __builtin_bit_cast(e2, 0x3f803f80u), c, false);
   }
   static __device__ __forceinline__ unsigned odd_bits(unsigned x) { return ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
 };
