@@ -30,6 +30,7 @@ typedef __attribute__((address_space(3))) void lds_ptr;
 typedef short s4v __attribute__((ext_vector_type(4)));
 
 constexpr int kKeys = 64;   // keys of a step
+constexpr int kRows = 128;  // rows of a work-group
 
 // position of 16-byte piece c of row r in a row of DP / 8 pieces (its own inverse)
 template <int DP> __device__ __forceinline__ int key_piece(int r, int c)
@@ -93,35 +94,26 @@ struct RaggedMask {
     return min(h, nk - 1);
   }
   __device__ __forceinline__ bool operator()(int i, int j) const { return (j >= lo(i) && j <= hi(i)) || (j < sinks && (!causal || j <= i) && j < nk); }
-  // whether rows imin..imax see all of keys j0..j1, or none of them
+  // whether rows imin..imax see all of keys j0..j1
   __device__ __forceinline__ bool all(int imin, int imax, int j0, int j1) const
   {
     return j1 <= (causal ? min(imin, nk - 1) : nk - 1) && ((j0 >= lo(imax) && j1 <= hi(imin)) || j1 < sinks);
   }
-  __device__ __forceinline__ bool none(int imin, int imax, int j0, int j1) const
-  {
-    return j0 >= nk || (causal && j0 > imax) || (j0 >= sinks && (j1 < lo(imin) || j0 > hi(imax)));
-  }
 };
-
-// waves per SIMD that the registers of a build are to allow
-constexpr int ragged_waves(int dp, int qt) { return qt == 1 ? (dp <= 32 ? 3 : dp <= 128 ? 2 : 1) : dp <= 64 ? 2 : 1; }
 
 }  // namespace
 
-// QT: 32-row tiles of a wave.
-template <int TYPE, int DP, int QT>
-__global__ void __launch_bounds__(256, ragged_waves(DP, QT)) ragged_attn_kernel(const RaggedParams p, int slots, int round)
+// NS: 16-channel slices of the head size, DP: that rounded up to a build's rows.
+template <int TYPE, int DP, int NS>
+__global__ void __launch_bounds__(256, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) ragged_attn_kernel(const RaggedParams p, int slots, int round)
 {
   using T = St<TYPE>;
   typedef typename T::e E;
-  constexpr int NS = DP / 16;          // 16-channel slices of the first product
   constexpr int NB = DP / 32;          // 32-channel blocks of the second
   constexpr int PR = DP / 8;           // 16-byte pieces of a row
   constexpr int VI = kKeys * PR / 256; // copies of a wave: values of a step,
   constexpr int KC = 32 * PR / 64, KI = (KC + 3) / 4;  // keys of a block (KC in all)
   constexpr int STAGE = kKeys * DP, BLOCK = 32 * DP;
-  constexpr int WR = 32 * QT, kRows = 4 * WR;  // rows of a wave, of the work-group
   // keys: a ring of four 32-key blocks; values: two stages of 64.  Arrays of their own, so that the
   // compiler sees that a copy into one does not touch the others and leaves it in flight.
   __shared__ __attribute__((aligned(16))) unsigned char K0[BLOCK * 2], K1[BLOCK * 2], K2[BLOCK * 2], K3[BLOCK * 2];
@@ -179,17 +171,14 @@ __global__ void __launch_bounds__(256, ragged_waves(DP, QT)) ragged_attn_kernel(
     const int qb = nqb - 1 - t;  // the longest first
     const int shift = nk - nq;
     const int imin = qb * kRows + shift, imax = min(nq - 1, qb * kRows + kRows - 1) + shift;
-    const int wmin = imin + WR * wave, wmax = min(imax, wmin + WR - 1);  // this wave's rows (none where wmax < wmin)
-    const int row = qb * kRows + WR * wave + col;                        // this lane's in each tile: row + 32 u
-    u4v qf[QT][NS];
+    const int wmin = imin + 32 * wave, wmax = min(imax, wmin + 31);  // this wave's rows (none where wmax < wmin)
+    const int row = qb * kRows + 32 * wave + col;
+    const E * q = static_cast<const E *>(p.q) + (long)(q0 + row) * p.q_token + (long)head * p.q_head;
+    u4v qf[NS];
 #pragma unroll
-    for (int u = 0; u < QT; ++u) {
-      const E * q = static_cast<const E *>(p.q) + (long)(q0 + row + 32 * u) * p.q_token + (long)head * p.q_head;
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const int ch = 16 * s + 8 * hi;
-        qf[u][s] = row + 32 * u < nq && ch < p.dim ? *reinterpret_cast<const u4v *>(q + ch) ^ flip : u4v{0, 0, 0, 0};
-      }
+    for (int i = 0; i < NS; ++i) {
+      const int ch = 16 * i + 8 * hi;
+      qf[i] = row < nq && ch < p.dim ? *reinterpret_cast<const u4v *>(q + ch) ^ flip : u4v{0, 0, 0, 0};
     }
 
     // steps: `first` over the first tokens, the others from step `from` on
@@ -201,6 +190,10 @@ __global__ void __launch_bounds__(256, ragged_waves(DP, QT)) ragged_attn_kernel(
     const int total = end > 0 ? first + (end + kKeys - 1) / kKeys - from : 0;
     auto key_of = [&](int n) { return kKeys * (n < first ? n : from + n - first); };
 
+    constexpr std::integral_constant<int, 0> c0{};
+    constexpr std::integral_constant<int, 1> c1{};
+    constexpr std::integral_constant<int, 2> c2{};
+    constexpr std::integral_constant<int, 3> c3{};
     // keys of block g (32 of step g / 2) into slot sl of the ring; values of step n into stage st
     auto copy_keys = [&](int g, auto sl) __attribute__((always_inline)) {
       if (g >= 2 * total) return;
@@ -220,27 +213,26 @@ __global__ void __launch_bounds__(256, ragged_waves(DP, QT)) ragged_attn_kernel(
       for (int i = 0; i < VI; ++i)
         copy_to_lds(at, bytes, voff[i], (st ? V1 : V0) + 1024 * (wave + 4 * i));
     };
-    // what this lane's rows see, less the lane's first key of a 32-key block
-    int seen_lo[QT], seen_n[QT], seen_first[QT];
-#pragma unroll
-    for (int u = 0; u < QT; ++u) {
-      const int place = row + 32 * u < nq ? row + 32 * u + shift : -(1 << 27);
-      seen_lo[u] = see.lo(place) - 4 * hi;
-      seen_n[u] = see.hi(place) - see.lo(place);
-      seen_first[u] = min(see.sinks, see.causal ? place + 1 : see.nk) - 4 * hi;
-    }
-    auto none_of = [&](int n) { return wmax < wmin || see.none(wmin, wmax, key_of(n), key_of(n) + kKeys - 1); };
+    auto copy_step = [&](int n) __attribute__((always_inline)) {  // the whole of step n, alone
+      __syncthreads();
+      copy_keys(2 * n, c0);
+      copy_keys(2 * n + 1, c1);
+      copy_values(n, c0);
+      __builtin_amdgcn_s_waitcnt(vm_wait(0));
+      __syncthreads();
+    };
+    // what this lane's row sees, less the lane's first key of a 32-key block
+    const int place = row < nq ? row + shift : -(1 << 27);
+    const int seen_lo = see.lo(place) - 4 * hi, seen_n = see.hi(place) - see.lo(place);
+    const int seen_first = min(see.sinks, see.causal ? place + 1 : see.nk) - 4 * hi;
 
-    f16v o[QT][NB], s0[QT], s1[QT];
-    float M[QT], L[QT];
+    f16v o[NB], s0, s1;
+    float M, L;
     auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
-      for (int u = 0; u < QT; ++u) {
-#pragma unroll
-        for (int j = 0; j < NB; ++j) o[u][j] = f16v{};
-        M[u] = kLowest;
-        L[u] = 0.0f;
-      }
+      for (int j = 0; j < NB; ++j) o[j] = f16v{};
+      M = kLowest;
+      L = 0.0f;
     };
     // fragment of channels 16 i .. of the keys in ring slot sl; of the values of keys 16 q .. and channels
     // 32 j .. in stage st, two transposing loads of 4 keys each
@@ -253,73 +245,57 @@ __global__ void __launch_bounds__(256, ragged_waves(DP, QT)) ragged_attn_kernel(
       return u4v{x[0], x[1], y[0], y[1]};
     };
     // S^T of the 32 keys in slot sl
-    auto scores = [&](auto sl, f16v (&s)[QT]) __attribute__((always_inline)) {
+    auto scores = [&](auto sl, f16v & s) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        const u4v a = key_piece_of(sl, i);
-#pragma unroll
-        for (int u = 0; u < QT; ++u) s[u] = T::mma32(a, qf[u][i], i ? s[u] : f16v{});
-      }
+      for (int i = 0; i < NS; ++i) s = T::mma32(key_piece_of(sl, i), qf[i], i ? s : f16v{});
     };
     // scores of keys (from key0 on) that a row does not see become -inf; the reference exponent follows the
     // running maximum only when that is 2^8 above it: weights up to 2^8 lose nothing in either 16-bit type
-    auto settle = [&](int key0, bool inner, f16v (&s)[QT]) __attribute__((always_inline)) {
+    auto settle = [&](int key0, bool inner, f16v & s) __attribute__((always_inline)) {
       if (!inner) {
 #pragma unroll
-        for (int u = 0; u < QT; ++u)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) {
-            const int j = key0 + 8 * (v / 4) + v % 4;
-            const bool ok = (seen_n[u] >= 0 && (unsigned)j - (unsigned)seen_lo[u] <= (unsigned)seen_n[u]) || j < seen_first[u];
-            s[u][v] = ok ? s[u][v] : -__builtin_inff();
-          }
-      }
-      float top[QT];
-      bool grow = false;
-#pragma unroll
-      for (int u = 0; u < QT; ++u) {
-        float a = s[u][0], b = s[u][1];
-#pragma unroll
-        for (int v = 2; v < 16; v += 4) {
-          a = top_of(a, s[u][v], s[u][v + 1]);
-          if (v + 2 < 16) b = top_of(b, s[u][v + 2], s[u][v + 3]);
+        for (int v = 0; v < 16; ++v) {
+          const int j = key0 + 8 * (v / 4) + v % 4;
+          const bool ok = (seen_n >= 0 && (unsigned)j - (unsigned)seen_lo <= (unsigned)seen_n) || j < seen_first;
+          s[v] = ok ? s[v] : -__builtin_inff();
         }
-        top[u] = across32(top_of(a, b, b), MaxOp()) * scale;
-        grow = grow || top[u] > M[u] + 8.0f;
       }
-      if (__any(grow)) {
+      float a = s[0], b = s[1];
 #pragma unroll
-        for (int u = 0; u < QT; ++u) {
-          const float m = fmaxf(M[u], top[u]), a = __builtin_amdgcn_exp2f(M[u] - m);
-          M[u] = m;
-          L[u] *= a;
+      for (int v = 2; v < 16; v += 4) {
+        a = top_of(a, s[v], s[v + 1]);
+        if (v + 2 < 16) b = top_of(b, s[v + 2], s[v + 3]);
+      }
+      const float top = across32(top_of(a, b, b), MaxOp()) * scale;
+      if (__any(top > M + 8.0f)) {
+        const float m = fmaxf(M, top), e = __builtin_amdgcn_exp2f(M - m);
+        M = m;
+        L *= e;
 #pragma unroll
-          for (int j = 0; j < NB; ++j)
+        for (int j = 0; j < NB; ++j)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) o[u][j][v] *= a;
-        }
+          for (int v = 0; v < 16; ++v) o[j][v] *= e;
       }
     };
-    // weights of score pairs [from, to) of the tiles' 8 each, two 16-bit values a pair; their sum is of
-    // the rounded ones, which are what the values get
-    auto weights = [&](const f16v (&s)[QT], u4v (&pf)[QT][2], int from, int to) __attribute__((always_inline)) {
+    // weights of score pairs [from, to) of 8, two 16-bit values a pair; their sum is of the rounded
+    // ones, which are what the values get
+    auto weights = [&](const f16v & s, u4v (&pf)[2], int from, int to) __attribute__((always_inline)) {
 #pragma unroll
-      for (int k = from; k < to; ++k) {
-        const int u = k % QT, i = k / QT;
-        const float x = __builtin_amdgcn_exp2f(fmaf(s[u][2 * i], scale, -M[u]));
-        const float y = __builtin_amdgcn_exp2f(fmaf(s[u][2 * i + 1], scale, -M[u]));
+      for (int i = from; i < to; ++i) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[2 * i], scale, -M));
+        const float y = __builtin_amdgcn_exp2f(fmaf(s[2 * i + 1], scale, -M));
         const unsigned w = pack2<TYPE>(x, y);
-        L[u] = T::add2(w, L[u]);
-        pf[u][i / 4][i % 4] = w;
+        L = T::add2(w, L);
+        pf[i / 4][i % 4] = w;
       }
     };
     // 32 keys, half kb of the step in stage st.  The matrix cores form the scores of the next 32 (in
     // slot nsl) while the vector unit turns these into weights, then take the values.  The order is
     // pinned slot by slot, with fragments read ahead.
-    auto block = [&](auto st, auto kb, auto nsl, int key0, bool inner, f16v (&s)[QT], f16v (&next)[QT]) __attribute__((always_inline)) {
+    auto block = [&](auto st, auto kb, auto nsl, int key0, bool inner, f16v & s, f16v & next) __attribute__((always_inline)) {
       // slots: the next keys' products, then the values'; fragment i is read R - 1 slots before its slot
       constexpr int Q = NS, W = 2 * NB, R = 5;
-      u4v pf[QT][2], f[R];
+      u4v pf[2], f[R];
       auto read = [&](auto i) __attribute__((always_inline)) {
         if constexpr (i < Q) f[i % R] = key_piece_of(nsl, i);
         else if constexpr (i < Q + W) f[i % R] = value_piece_of(st, 2 * kb + (i - Q) / NB, (i - Q) % NB);
@@ -329,26 +305,16 @@ __global__ void __launch_bounds__(256, ragged_waves(DP, QT)) ragged_attn_kernel(
       __builtin_amdgcn_sched_barrier(0);
       static_for<0, Q>([&](auto i) __attribute__((always_inline)) {
         read(std::integral_constant<int, i + R - 1>{});
-        static_for<0, QT>([&](auto u) __attribute__((always_inline)) {
-          if constexpr (i == 0) next[u] = T::mma32(f[0], qf[u][0], f16v{});
-          else next[u] = T::mma32(f[i % R], qf[u][i], next[u]);
-          constexpr int at = i * QT + u;
-          weights(s, pf, at * 8 / Q, (at + 1) * 8 / Q);
-          __builtin_amdgcn_sched_barrier(0);
-        });
+        next = T::mma32(f[i % R], qf[i], i ? next : f16v{});
+        weights(s, pf, i * 8 / Q, (i + 1) * 8 / Q);
+        __builtin_amdgcn_sched_barrier(0);
       });
       static_for<0, W>([&](auto i) __attribute__((always_inline)) {
         read(std::integral_constant<int, Q + i + R - 1>{});
-        static_for<0, QT>([&](auto u) __attribute__((always_inline)) {
-          o[u][i % NB] = T::mma32(f[(Q + i) % R], pf[u][i / NB], o[u][i % NB]);
-        });
+        o[i % NB] = T::mma32(f[(Q + i) % R], pf[i / NB], o[i % NB]);
         __builtin_amdgcn_sched_barrier(0);
       });
     };
-    constexpr std::integral_constant<int, 0> c0{};
-    constexpr std::integral_constant<int, 1> c1{};
-    constexpr std::integral_constant<int, 2> c2{};
-    constexpr std::integral_constant<int, 3> c3{};
     // Step n in value stage st, whose first 32 scores are there; x, y: ring slots of the two key blocks
     // it multiplies, behind the ones it weighs; z, w: the slots that take the two after those.
     auto step = [&](int n, auto st, auto nst, auto x, auto y, auto z, auto w) __attribute__((always_inline)) {
@@ -363,8 +329,22 @@ __global__ void __launch_bounds__(256, ragged_waves(DP, QT)) ragged_attn_kernel(
       block(st, c1, y, key0 + 32, inner, s1, s0);  // after the last step s0 is of no use (whatever the slot holds)
     };
 
+    // a step of which this wave's rows see no key: its share of the copies
+    auto idle = [&](int n) __attribute__((always_inline)) {
+      __builtin_amdgcn_s_waitcnt(vm_wait(0));
+      __syncthreads();
+      if (n & 1) {
+        copy_keys(2 * n + 3, c1);
+        copy_keys(2 * n + 4, c2);
+        copy_values(n + 1, c0);
+      } else {
+        copy_keys(2 * n + 3, c3);
+        copy_keys(2 * n + 4, c0);
+        copy_values(n + 1, c1);
+      }
+    };
+
     __syncthreads();  // the last rows' stages are no longer read
-    clear();
     if (total > 0) {
       copy_keys(0, c0);
       __builtin_amdgcn_s_waitcnt(vm_wait(0));
@@ -372,11 +352,23 @@ __global__ void __launch_bounds__(256, ragged_waves(DP, QT)) ragged_attn_kernel(
       copy_keys(1, c1);
       copy_keys(2, c2);
       copy_values(0, c0);
+    }
+    if (wmax < wmin) {  // no rows: this wave's share of the copies, up to the same barriers as the others
+      for (int n = 0; n < total; ++n) idle(n);
+      if (__syncthreads_or(0))
+        for (int n = 0; n < total; ++n) copy_step(n);
+      continue;
+    }
+    clear();
+    if (total > 0) {
+      // the wave's last key may lie steps before the work-group's
+      const int wend = p.causal ? max(0, min(total, first + (wmax + kKeys) / kKeys - from)) : total;
       scores(c0, s0);
-      for (int n = 0; n < total; n += 2) {
+      for (int n = 0; n < wend; n += 2) {
         step(n, c0, c1, c1, c2, c3, c0);
-        if (n + 1 < total) step(n + 1, c1, c0, c3, c0, c1, c2);
+        if (n + 1 < wend) step(n + 1, c1, c0, c3, c0, c1, c2);
       }
+      for (int n = wend; n < total; ++n) idle(n);
     }
 
     // An infinity or NaN among the values reaches rows that do not see it, as 0 x inf, and stays
@@ -384,29 +376,21 @@ __global__ void __launch_bounds__(256, ragged_waves(DP, QT)) ragged_attn_kernel(
     // values left out of the product and added to the rows that do see them.
     bool odd = false;
 #pragma unroll
-    for (int u = 0; u < QT; ++u)
+    for (int j = 0; j < NB; ++j)
 #pragma unroll
-      for (int j = 0; j < NB; ++j)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) odd = odd || !(fabsf(o[u][j][v]) < __builtin_inff());
+      for (int v = 0; v < 16; ++v) odd = odd || !(fabsf(o[j][v]) < __builtin_inff());
     if (__syncthreads_or(odd)) {
       clear();
       for (int n = 0; n < total; ++n) {
-        __syncthreads();
-        copy_keys(2 * n, c0);
-        copy_keys(2 * n + 1, c1);
-        copy_values(n, c0);
-        __builtin_amdgcn_s_waitcnt(vm_wait(0));
-        __syncthreads();
-        if (none_of(n)) continue;
+        copy_step(n);
         const bool inner = see.all(wmin, wmax, key_of(n), key_of(n) + kKeys - 1);
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-          u4v pf[QT][2];
+          u4v pf[2];
           if (kb) scores(c1, s0);
           else scores(c0, s0);
           settle(key_of(n) + 32 * kb, inner, s0);
-          weights(s0, pf, 0, 8 * QT);
+          weights(s0, pf, 0, 8);
 #pragma unroll
           for (int sl = 0; sl < 2; ++sl)
 #pragma unroll
@@ -414,44 +398,35 @@ __global__ void __launch_bounds__(256, ragged_waves(DP, QT)) ragged_attn_kernel(
               u4v a = value_piece_of(c0, 2 * kb + sl, j);
 #pragma unroll
               for (int x = 0; x < 4; ++x) a[x] &= ~((T::odd_bits(a[x]) >> 15) * 0xffffu);
-#pragma unroll
-              for (int u = 0; u < QT; ++u) o[u][j] = T::mma32(a, pf[u][sl], o[u][j]);
+              o[j] = T::mma32(a, pf[sl], o[j]);
             }
         }
         const E * Vs = reinterpret_cast<const E *>(V0);
         for (int r = 0; r < kKeys; ++r) {
-          bool mine[QT];
-#pragma unroll
-          for (int u = 0; u < QT; ++u) mine[u] = row + 32 * u < nq && see(row + 32 * u + shift, key_of(n) + r);
+          const bool mine = row < nq && see(place, key_of(n) + r);
 #pragma unroll
           for (int j = 0; j < NB; ++j)
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
               const int ch = 32 * j + 8 * (v / 4) + 4 * hi + v % 4;
               const float x = (float)Vs[r * DP + value_piece<DP>(r, ch / 8) * 8 + ch % 8];
-              if (fabsf(x) < __builtin_inff()) continue;
-#pragma unroll
-              for (int u = 0; u < QT; ++u)
-                if (mine[u]) o[u][j][v] += x;
+              if (mine && !(fabsf(x) < __builtin_inff())) o[j][v] += x;
             }
         }
       }
     }
 
-#pragma unroll
-    for (int u = 0; u < QT; ++u) {
-      const float sum = across32(L[u], SumOp());
-      if (row + 32 * u >= nq) continue;
+    const float sum = across32(L, SumOp());
+    if (row < nq) {
       const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;  // a row that saw nothing is zero (NaN stays)
-      E * out = static_cast<E *>(p.o) + (long)(q0 + row + 32 * u) * p.o_token + (long)head * p.o_head;
+      E * out = static_cast<E *>(p.o) + (long)(q0 + row) * p.o_token + (long)head * p.o_head;
 #pragma unroll
       for (int j = 0; j < NB; ++j)
 #pragma unroll
         for (int v = 0; v < 16; v += 4) {
           const int ch = 32 * j + 2 * v + 4 * hi;
           if (ch >= p.dim) continue;
-          const f16v & x = o[u][j];
-          const u2v y = {pack2<TYPE>(x[v] * inv, x[v + 1] * inv), pack2<TYPE>(x[v + 2] * inv, x[v + 3] * inv)};
+          const u2v y = {pack2<TYPE>(o[j][v] * inv, o[j][v + 1] * inv), pack2<TYPE>(o[j][v + 2] * inv, o[j][v + 3] * inv)};
           *reinterpret_cast<u2v *>(out + ch) = y;
         }
     }
@@ -460,9 +435,8 @@ __global__ void __launch_bounds__(256, ragged_waves(DP, QT)) ragged_attn_kernel(
 
 namespace {
 
-template <int TYPE, int DP, int QT> void launch_ragged(const RaggedParams & p, hipStream_t s)
+template <int TYPE, int DP, int NS> void launch_ragged(const RaggedParams & p, hipStream_t s)
 {
-  constexpr int kRows = 128 * QT;
   // max_q only sizes the grid: a work-group takes every slots-th row block of its sequence.  A
   // launch holds 2^24 work-groups of 256 lanes.
   const long heads = (long)p.batch * p.heads;
@@ -470,18 +444,18 @@ template <int TYPE, int DP, int QT> void launch_ragged(const RaggedParams & p, h
   const long units = heads / p.group;
   const int round = units % kXcds == 0 || units >= 4 * kXcds;
   const long wgs = (round ? (units + kXcds - 1) / kXcds * kXcds : units) * p.group * slots;
-  hipLaunchKernelGGL((ragged_attn_kernel<TYPE, DP, QT>), dim3((unsigned)wgs), dim3(256), 0, s, p, slots, round);
+  hipLaunchKernelGGL((ragged_attn_kernel<TYPE, DP, NS>), dim3((unsigned)wgs), dim3(256), 0, s, p, slots, round);
 }
 
 template <int TYPE> void launch_ragged_dim(const RaggedParams & p, hipStream_t s)
 {
-  const bool wide = getenv("QT2") != nullptr;
-  if (p.dim <= 32) launch_ragged<TYPE, 32, 1>(p, s);
-  else if (p.dim <= 64) wide ? launch_ragged<TYPE, 64, 2>(p, s) : launch_ragged<TYPE, 64, 1>(p, s);
-  else if (p.dim <= 96) wide ? launch_ragged<TYPE, 96, 2>(p, s) : launch_ragged<TYPE, 96, 1>(p, s);
-  else if (p.dim <= 128) wide ? launch_ragged<TYPE, 128, 2>(p, s) : launch_ragged<TYPE, 128, 1>(p, s);
-  else if (p.dim <= 192) launch_ragged<TYPE, 192, 1>(p, s);
-  else launch_ragged<TYPE, 256, 1>(p, s);
+  if (p.dim <= 32) launch_ragged<TYPE, 32, 2>(p, s);
+  else if (p.dim <= 64) launch_ragged<TYPE, 64, 4>(p, s);
+  else if (p.dim <= 80) launch_ragged<TYPE, 96, 5>(p, s);
+  else if (p.dim <= 96) launch_ragged<TYPE, 96, 6>(p, s);
+  else if (p.dim <= 128) launch_ragged<TYPE, 128, 8>(p, s);
+  else if (p.dim <= 192) launch_ragged<TYPE, 192, 12>(p, s);
+  else launch_ragged<TYPE, 256, 16>(p, s);
 }
 
 }  // namespace
