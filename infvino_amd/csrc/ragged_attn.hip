@@ -347,11 +347,11 @@ __global__ void __launch_bounds__(256, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) ragged_
     __syncthreads();  // the last rows' stages are no longer read
     if (total > 0) {
       copy_keys(0, c0);
-      __builtin_amdgcn_s_waitcnt(vm_wait(0));
-      __syncthreads();
       copy_keys(1, c1);
       copy_keys(2, c2);
       copy_values(0, c0);
+      __builtin_amdgcn_s_waitcnt(vm_wait(0));
+      __syncthreads();
     }
     if (wmax < wmin) {  // no rows: this wave's share of the copies, up to the same barriers as the others
       for (int n = 0; n < total; ++n) idle(n);
@@ -417,17 +417,26 @@ __global__ void __launch_bounds__(256, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) ragged_
     }
 
     const float sum = across32(L, SumOp());
-    if (row < nq) {
+    {
       const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;  // a row that saw nothing is zero (NaN stays)
-      E * out = static_cast<E *>(p.o) + (long)(q0 + row) * p.o_token + (long)head * p.o_head;
+      E * const out = static_cast<E *>(p.o) + (long)(q0 + row) * p.o_token + (long)head * p.o_head;
 #pragma unroll
       for (int j = 0; j < NB; ++j)
 #pragma unroll
-        for (int v = 0; v < 16; v += 4) {
-          const int ch = 32 * j + 2 * v + 4 * hi;
-          if (ch >= p.dim) continue;
-          const u2v y = {pack2<TYPE>(o[j][v] * inv, o[j][v + 1] * inv), pack2<TYPE>(o[j][v + 2] * inv, o[j][v + 3] * inv)};
-          *reinterpret_cast<u2v *>(out + ch) = y;
+        for (int v = 0; v < 16; v += 8) {
+          // a lane has channels 4 hi .. of both 8-channel groups; the two halves of the wave exchange
+          // theirs, so that a lane writes all 8 of group v / 4 + hi
+          u4v y;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const unsigned g0 = pack2<TYPE>(o[j][v + 2 * x] * inv, o[j][v + 2 * x + 1] * inv);
+            const unsigned g1 = pack2<TYPE>(o[j][v + 4 + 2 * x] * inv, o[j][v + 5 + 2 * x] * inv);
+            const auto r = __builtin_amdgcn_permlane32_swap(g0, g1, false, false);
+            y[x] = r[0];
+            y[2 + x] = r[1];
+          }
+          const int ch = 32 * j + 2 * v + 8 * hi;
+          if (row < nq && ch < p.dim) *reinterpret_cast<u4v *>(out + ch) = y;
         }
     }
   }
