@@ -78,12 +78,6 @@ template <int DP> __device__ __forceinline__ unsigned value_at(unsigned base, in
   return (base ^ (64u * (j & ((1 << BITS) - 1)))) + (unsigned)(j >> BITS) * (64u << BITS);
 }
 
-// the largest of three, NaN if one is: one instruction
-__device__ __forceinline__ float top_of(float a, float b, float c)
-{
-  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
-}
-
 // What a query at place i sees: keys lo..hi and the first `sinks`.
 struct RaggedMask {
   int nk, causal, window, sinks;  // sinks 0 without a window

@@ -86,6 +86,12 @@ template <int TYPE> __device__ __forceinline__ f2v unpack2(unsigned x)
   return f2v{(float)v[0], (float)v[1]};
 }
 
+// the largest of three, NaN if one is: one instruction
+__device__ __forceinline__ float top_of(float a, float b, float c)
+{
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
+}
+
 // x of the lane 16 and 32 away, combined: swaps of lane rows on the vector unit
 template <class Op> __device__ __forceinline__ float across16(float x, Op op)
 {

@@ -76,6 +76,7 @@ struct PagedParams {
 // sequence (bounds that only steer the split); returns the workspace bytes.
 size_t paged_split(PagedParams & p, int max_new, int max_len);
 void launch_paged_attention(const PagedParams & p, hipStream_t s);
+void launch_paged_bf16(const PagedParams & p, hipStream_t s);  // its bf16 kernels, built by themselves
 
 struct RaggedParams {
   int type = 0, heads = 0, group = 1, dim = 0;
