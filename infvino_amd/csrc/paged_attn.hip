@@ -23,7 +23,8 @@ size_t paged_split(PagedParams & p, int max_new, int max_len)
   if (p.window) len = std::min<long>(len, (long)p.window + p.sinks + max_new + 128);
   const long steps = (len + 63) / 64, waves = 4 / p.row_waves;
   const long wgs = (long)c.batch * c.heads * p.row_slots;
-  const long want = std::max<long>((1024 + wgs - 1) / wgs, (steps + 32 * waves - 1) / (32 * waves));
+  const long SPW = getenv("SPW") ? atoi(getenv("SPW")) : 64, TW = getenv("TW") ? atoi(getenv("TW")) : 256;
+  const long want = std::max<long>((TW + wgs - 1) / wgs, (steps + SPW * waves - 1) / (SPW * waves));
   const long top = std::max<long>(1, (steps + waves - 1) / waves);
   // a launch holds 2^24 work-groups of 256 lanes
   p.parts = (int)std::min<long>({std::max<long>(want, 1), top, 256, std::max<long>(1, (1L << 23) / wgs)});

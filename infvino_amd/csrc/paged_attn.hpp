@@ -310,11 +310,13 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
     clear();
     int n = n0 + wk;
     if (n < n1) {
-      int idk = page_of(n, r >> 2), idv = page_of(n, g);
-      load_k(n, idk);
-      load_v(n, idv);
-      idk = page_of(min(n + WK, n1 - 1), r >> 2);
-      idv = page_of(min(n + WK, n1 - 1), g);
+      // page numbers of two steps before the first step's data, in the order of the loop: the
+      // compiler's counted waits then hold for the first pass through it as well
+      const int firstk = page_of(n, r >> 2), firstv = page_of(n, g);
+      int idk = page_of(min(n + WK, n1 - 1), r >> 2), idv = page_of(min(n + WK, n1 - 1), g);
+      __builtin_amdgcn_sched_barrier(0);
+      load_k(n, firstk);
+      load_v(n, firstv);
       for (; n + WK < n1; n += WK) {
         const int nk = idk, nv = idv;  // pages two steps ahead
         idk = page_of(min(n + 2 * WK, n1 - 1), r >> 2);
