@@ -71,14 +71,15 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
   const int wk = wave % WK, wr = wave / WK;
-  // A unit (sequence, key head, part of the keys) has row_slots work-groups, on one XCD; units go
-  // round the XCDs, so that each gets its share of long and short sequences.
+  // A unit (part of the keys, sequence, key head) has row_slots work-groups, on one XCD; units go
+  // round the XCDs, so that each gets its share of long and short sequences, and of their last parts,
+  // which only long ones have and which come last.
   int w = blockIdx.x / kXcds;
   const int slot = w % p.row_slots;
   w = w / p.row_slots * kXcds + blockIdx.x % kXcds;
   if (w >= units) return;
-  const int part = w % p.parts;
-  w /= p.parts;
+  const int seqs = c.batch * c.heads, part = w / seqs;
+  w -= part * seqs;
   const int h = w % c.heads, b = w / c.heads;
 
   const int c0 = min(max(c.cu[b], 0), c.tokens), c1 = min(max(c.cu[b + 1], c0), c.tokens);

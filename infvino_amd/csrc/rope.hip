@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeParams p, const Rop
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       const int f = VEC * piece + i;
-      const f2v cs = rot_cossin(p.r.pos[rot_axis(p.r, f) * p.r.pos_axis + token], p.r.freq[f]);
+      const f2v cs = rot_cossin(p.r.pos[rot_axis(p.r, f) * p.r.pos_axis + token], p.r.freq[f], rot_turns(p.r.freq[f]));
       c[i] = cs[0];
       s[i] = cs[1];
     }
@@ -116,9 +116,11 @@ template <int TYPE, int VEC> void launch_rope_vec(const RopeParams & p, hipStrea
   g.pieces = p.dim / (2 * VEC);
   g.rotating = p.r.rot / (2 * VEC);
   g.copy = !same;
-  // one head a thread until the chip is full (256 CUs x 2048 lanes), then up to 8 that share the angles
+  // a thread's heads share its angles: as many as leave two waves a SIMD, up to 8 (6400 tokens of 32
+  // heads of 80 channels: 16 us, with four waves a SIMD 18, with one head a thread 25)
   const long lanes = p.tokens * g.pieces * p.heads;
-  g.hg = lanes <= (1L << 20) ? p.heads : (p.heads + 7) / 8;
+  const int per_thread = (int)std::min<long>({8, std::max<long>(1, lanes >> 17), p.heads});
+  g.hg = (p.heads + per_thread - 1) / per_thread;
   g.dv_pieces = fastdiv_make(g.pieces);
   g.dv_hg = fastdiv_make(g.hg);
   // slices of tokens, so that a launch's lanes stay below 2^31
@@ -195,12 +197,6 @@ __device__ __forceinline__ bool page_work(const CacheParams & c, int w, PageWork
   return true;
 }
 
-__device__ __forceinline__ float finite_abs(float x)
-{
-  const float a = fabsf(x);
-  return a < __builtin_inff() ? a : 0.0f;  // infinities and NaN have no part in a scale
-}
-
 // the smallest power of two s with amax <= 448 s = 1.75 x 2^8 s, from the bits of amax
 __device__ __forceinline__ float page_scale(float amax)
 {
@@ -210,17 +206,10 @@ __device__ __forceinline__ float page_scale(float amax)
   return fmaxf(__builtin_bit_cast(float, (unsigned)max(e, 1) << 23), kLowestScale);
 }
 
-// e4m3 codes of four values of the page's scale: nearest, ties to even; infinities become the
-// largest value, NaN stays NaN
-__device__ __forceinline__ float clamp_code(float x)
-{
-  x = x > kMaxCode ? kMaxCode : x;
-  return x < -kMaxCode ? -kMaxCode : x;
-}
+// e4m3 codes of four values in units of the page's scale, nearest, ties to even; NaN stays NaN
 __device__ __forceinline__ unsigned codes4(float a, float b, float c, float d)
 {
-  unsigned r = __builtin_amdgcn_cvt_pk_fp8_f32(clamp_code(a), clamp_code(b), 0, false);
-  return __builtin_amdgcn_cvt_pk_fp8_f32(clamp_code(c), clamp_code(d), r, true);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
 }
 __device__ __forceinline__ unsigned rescale4(unsigned x, float ratio)
 {
@@ -228,249 +217,435 @@ __device__ __forceinline__ unsigned rescale4(unsigned x, float ratio)
   return codes4(a[0] * ratio, a[1] * ratio, b[0] * ratio, b[1] * ratio);
 }
 
-// maximum over the work-group, and the page's new scale
-__device__ __forceinline__ float group_scale(float amax, float old, float * red)
+// maximum over the work-group
+__device__ __forceinline__ float group_max(float amax, float * red)
 {
   for (int m = 1; m < 64; m *= 2) amax = fmaxf(amax, __shfl_xor(amax, m));
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = amax;
   __syncthreads();
-  amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  return fmaxf(page_scale(amax), old);
+  return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+// The page's new scale; amax: this thread's largest magnitude.  If there is an infinity among the
+// work-group's values (all of its threads see that), `finite` gives the thread's largest finite one, and
+// saturate is set: infinities are to become the largest code.  A NaN is passed over by the maximum.
+template <class Fn>
+__device__ __forceinline__ float group_scale(float amax, float before, float (*red)[4], bool & saturate, Fn && finite)
+{
+  amax = group_max(amax, red[0]);
+  saturate = !(amax < __builtin_inff());
+  if (saturate) amax = group_max(finite(), red[2]);
+  return fmaxf(page_scale(amax), before);
+}
+__device__ __forceinline__ float finite_abs(float x)
+{
+  const float a = fabsf(x);
+  return a < __builtin_inff() ? a : 0.0f;
+}
+__device__ __forceinline__ float saturated(float x)
+{
+  x = x > kMaxCode ? kMaxCode : x;
+  return x < -kMaxCode ? -kMaxCode : x;
 }
 
 }  // namespace
 
-// Keys.  A thread owns a token's 16 bytes of the stored page (EK channels), U of them: the
-// channels' partners come from a second read that hits the cache, and a granule's tokens times
-// frequencies of cosines and sines from LDS.
-template <int TYPE, int BITS, int U>
-__device__ __forceinline__ void append_keys(const AppendParams & p, const PageWork & w, int h, float * red, f2v * cs)
+// Cosines and sines of the page's new tokens in LDS, two planes [token][pitch] of 16-byte runs of 4
+// frequencies.  A thread reads Q runs that follow each other, its neighbour the Q after: runs are
+// stored with the neighbours' side by side and a pitch of 2 mod 8 runs, so that the lanes that are
+// served together lie in distinct banks.
+template <int Q> struct AngleTable {
+  int lots, pitch;
+  static __host__ __device__ int lots_of(int half) { return (half / 4 + Q - 1) / Q; }
+  static __host__ __device__ int pitch_of(int half) { return (Q * lots_of(half) + 5) / 8 * 8 + 2; }
+  __device__ __forceinline__ AngleTable(int half) : lots(lots_of(half)), pitch(pitch_of(half)) {}
+  __device__ __forceinline__ int at(int t, int f) const { return (t * pitch + f / 4 % Q * lots + f / 4 / Q) * 4 + f % 4; }
+};
+
+template <int Q>
+__device__ __forceinline__ void page_angles(const RotParams & r, const PageWork & w, float * cos, float * sin)
 {
-  typedef typename St<TYPE>::e E;
-  constexpr int EK = BITS == 8 ? 16 : 8, Q = EK / 4;
-  const CacheParams & c = p.c;
-  const RotParams & r = p.r;
-  const int tid = threadIdx.x, chunks = c.dim / EK, n = w.hi - w.lo;
-  const int rot = r.rot, half = r.half;
-  for (int i = tid; i < n * half; i += 256) {
-    const int t = i / half, f = i - t * half;
-    cs[i] = rot_cossin(r.pos[rot_axis(r, f) * r.pos_axis + w.row0 + t], r.freq[f]);
-  }
-  __syncthreads();
-  const E * src = static_cast<const E *>(p.k) + (long)h * p.k_head;
-  uint8_t * dst = static_cast<uint8_t *>(c.kc) + (w.base + h) * ((long)c.page * c.dim * (BITS / 8));
-  auto place = [&](int slot, int ch) { return ((slot / 4 * chunks + ch) * 4 + slot % 4) * 16; };
-  float v[U][EK];
-  float amax = 0.0f;
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int i = tid + 256 * u, t = i / chunks, ch = i - t * chunks;
-    if (i >= n * chunks) continue;
-    const E * row = src + (long)(w.row0 + t) * p.k_token;
-#pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      const int m = ch * EK + 4 * q;  // rot and half are multiples of 4: a run of 4 has one kind
-      const u2v own = *reinterpret_cast<const u2v *>(row + m);
-      const f2v a = unpack2<TYPE>(own[0]), b = unpack2<TYPE>(own[1]);
-      float * o = v[u] + 4 * q;
-      if (m >= rot) {
-        o[0] = a[0]; o[1] = a[1]; o[2] = b[0]; o[3] = b[1];
-      } else if (r.adjacent) {
-        const f2v c0 = cs[t * half + m / 2], c1 = cs[t * half + m / 2 + 1];
-        o[0] = a[0] * c0[0] - a[1] * c0[1]; o[1] = a[1] * c0[0] + a[0] * c0[1];
-        o[2] = b[0] * c1[0] - b[1] * c1[1]; o[3] = b[1] * c1[0] + b[0] * c1[1];
-      } else {
-        const bool first = m < half;
-        const u2v other = *reinterpret_cast<const u2v *>(row + (first ? m + half : m - half));
-        const f2v d = unpack2<TYPE>(other[0]), e = unpack2<TYPE>(other[1]);
-        const f2v * t4 = cs + t * half + (first ? m : m - half);
-        const float g = first ? -1.0f : 1.0f;
-        o[0] = a[0] * t4[0][0] + g * (d[0] * t4[0][1]); o[1] = a[1] * t4[1][0] + g * (d[1] * t4[1][1]);
-        o[2] = b[0] * t4[2][0] + g * (e[0] * t4[2][1]); o[3] = b[1] * t4[3][0] + g * (e[1] * t4[3][1]);
-      }
-    }
-    if (BITS == 8) {
-#pragma unroll
-      for (int k = 0; k < EK; ++k) amax = fmaxf(amax, finite_abs(v[u][k]));
-    } else {
-      const u4v y = {pack2<TYPE>(v[u][0], v[u][1]), pack2<TYPE>(v[u][2], v[u][3]), pack2<TYPE>(v[u][4], v[u][5]),
-                     pack2<TYPE>(v[u][6], v[u][7])};
-      *reinterpret_cast<u4v *>(dst + place(w.lo + t, ch)) = y;
-    }
-  }
-  if constexpr (BITS == 8) {
-    const float before = w.lo ? c.ks[w.base + h] : 0.0f;
-    const float s = group_scale(amax, before, red), inv = 1.0f / s;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = tid + 256 * u, t = i / chunks, ch = i - t * chunks;
-      if (i >= n * chunks) continue;
-      u4v y;
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        y[q] = codes4(v[u][4 * q] * inv, v[u][4 * q + 1] * inv, v[u][4 * q + 2] * inv, v[u][4 * q + 3] * inv);
-      *reinterpret_cast<u4v *>(dst + place(w.lo + t, ch)) = y;
-    }
-    if (w.lo && before != s) {
-      const float ratio = before * inv;
-      for (int i = tid; i < (c.page - n) * chunks; i += 256) {
-        const int t = i / chunks;
-        u4v * at = reinterpret_cast<u4v *>(dst + place(t < w.lo ? t : t + n, i - t * chunks));
-        u4v y = *at;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) y[q] = rescale4(y[q], ratio);
-        *at = y;
-      }
-    }
-    if (tid == 0) c.ks[w.base + h] = s;
+  const AngleTable<Q> table(r.half);
+  const int per = 256 / r.half, t0 = threadIdx.x / r.half, f = threadIdx.x - t0 * r.half, n = w.hi - w.lo;
+  if (t0 >= per) return;
+  const float freq = r.freq[f];
+  const f2v turns = rot_turns(freq);
+  const int32_t * pos = r.pos + rot_axis(r, f) * r.pos_axis + w.row0;
+  for (int t = t0; t < n; t += per) {
+    const f2v cs = rot_cossin(pos[t], freq, turns);
+    cos[table.at(t, f)] = cs[0];
+    sin[table.at(t, f)] = cs[1];
   }
 }
 
-// Values.  A thread owns two channels of EV tokens (a granule), 2 x 16 bytes side by side in the
-// stored page, U of them.
+// Keys of heads [h0, h1).  A thread owns two runs of R channels of a token whose pairs lie within the
+// two: channels f.. and rot / 2 + f.., or 2 R in a row (adjacent pairs, and what is not rotated); U such
+// units.  The next head's rows are asked for as soon as this one's are turned.
+template <int TYPE, int BITS, int R, int U>
+__device__ __forceinline__ void append_keys(const AppendParams & p, const PageWork & w, int h0, int h1, float (*red)[4], const float * cos,
+                                            const float * sin)
+{
+  typedef typename St<TYPE>::e E;
+  constexpr int EK = BITS == 8 ? 16 : 8, Q = R / 4;
+  const CacheParams & c = p.c;
+  const RotParams & r = p.r;
+  const int units = c.dim / (2 * R), chunks = c.dim / EK, n = w.hi - w.lo;
+  const int per = 256 / units, t0 = threadIdx.x / units, unit = threadIdx.x - t0 * units;  // tokens of a pass; this thread's
+  const bool on = t0 < per, turn = unit * 2 * R < r.rot;
+  const bool split = turn && !r.adjacent;
+  const int lo = split ? unit * R : unit * 2 * R, hi = split ? lo + r.half : lo + R, f0 = unit * R;
+  const AngleTable<Q> table(r.half);
+  // bytes of channel m of a slot in the stored page
+  auto place = [&](int slot, int m) { return ((slot / 4 * chunks + m / EK) * 4 + slot % 4) * 16 + m % EK * (BITS / 8); };
+  auto fetch = [&](int h, int t, u2v (&x)[2][Q]) __attribute__((always_inline)) {
+    const E * row = static_cast<const E *>(p.k) + (long)h * p.k_head + (long)(w.row0 + t) * p.k_token;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      x[0][q] = *reinterpret_cast<const u2v *>(row + lo + 4 * q);
+      x[1][q] = *reinterpret_cast<const u2v *>(row + hi + 4 * q);
+    }
+  };
+  auto turned = [&](int t, const u2v (&x)[2][Q], f4v (&v)[2][Q]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const f2v a = unpack2<TYPE>(x[i][q][0]), b = unpack2<TYPE>(x[i][q][1]);
+        v[i][q] = f4v{a[0], a[1], b[0], b[1]};
+      }
+    if (!turn) return;
+    if (r.adjacent) {  // pair j of the 2 R channels: v[j / (R / 2)], elements 2 (j % (R / 2)) and the next
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const int at = table.at(t, f0 + 4 * q);
+        const f4v c4 = *reinterpret_cast<const f4v *>(cos + at), s4 = *reinterpret_cast<const f4v *>(sin + at);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int j = 4 * q + k;
+          f4v & y = v[j / (2 * Q)][j % (2 * Q) / 2];
+          const float a = y[j % 2 * 2], b = y[j % 2 * 2 + 1];
+          y[j % 2 * 2] = a * c4[k] - b * s4[k];
+          y[j % 2 * 2 + 1] = b * c4[k] + a * s4[k];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const int at = table.at(t, f0 + 4 * q);
+        const f4v c4 = *reinterpret_cast<const f4v *>(cos + at), s4 = *reinterpret_cast<const f4v *>(sin + at);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float a = v[0][q][k], b = v[1][q][k];
+          v[0][q][k] = a * c4[k] - b * s4[k];
+          v[1][q][k] = b * c4[k] + a * s4[k];
+        }
+      }
+    }
+  };
+  if constexpr (BITS == 16) {
+    for (int h = h0; h < h1; ++h) {
+      uint8_t * dst = static_cast<uint8_t *>(c.kc) + (w.base + h) * ((long)c.page * c.dim * 2);
+#pragma unroll 2
+      for (int t = on ? t0 : n; t < n; t += per) {
+        u2v x[2][Q];
+        f4v v[2][Q];
+        fetch(h, t, x);
+        turned(t, x, v);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int q = 0; q < Q; q += 2) {
+            uint8_t * at = dst + place(w.lo + t, (i ? hi : lo) + 4 * q);
+            const u2v y = {pack2<TYPE>(v[i][q][0], v[i][q][1]), pack2<TYPE>(v[i][q][2], v[i][q][3])};
+            if constexpr (Q == 1) {
+              *reinterpret_cast<u2v *>(at) = y;
+            } else {
+              const f4v & z = v[i][q + 1];
+              *reinterpret_cast<u4v *>(at) = u4v{y[0], y[1], pack2<TYPE>(z[0], z[1]), pack2<TYPE>(z[2], z[3])};
+            }
+          }
+      }
+    }
+  } else {
+    u2v x[U][2][Q];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (on && t0 + per * u < n) fetch(h0, t0 + per * u, x[u]);
+    for (int h = h0; h < h1; ++h) {
+      uint8_t * dst = static_cast<uint8_t *>(c.kc) + (w.base + h) * ((long)c.page * c.dim);
+      f4v v[U][2][Q];
+      auto all = [&](auto && fn) __attribute__((always_inline)) {  // fn over the thread's values
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (on && t0 + per * u < n) {
+#pragma unroll
+            for (int i = 0; i < 2 * Q; ++i)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[u][i / Q][i % Q][k] = fn(v[u][i / Q][i % Q][k]);
+          }
+      };
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int t = t0 + per * u;
+        if (!on || t >= n) continue;
+        turned(t, x[u], v[u]);
+        if (h + 1 < h1) fetch(h + 1, t, x[u]);
+      }
+      float amax = 0.0f;
+      all([&](float y) {
+        amax = fmaxf(amax, fabsf(y));
+        return y;
+      });
+      const float before = w.lo ? c.ks[w.base + h] : 0.0f;
+      bool saturate;
+      const float s = group_scale(amax, before, red + (h & 1), saturate, [&]() {
+        float m = 0.0f;
+        all([&](float y) {
+          m = fmaxf(m, finite_abs(y));
+          return y;
+        });
+        return m;
+      });
+      const float inv = 1.0f / s;
+      all([&](float y) { return y * inv; });
+      if (saturate) all([&](float y) { return saturated(y); });
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int t = t0 + per * u;
+        if (!on || t >= n) continue;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          unsigned y[Q];
+#pragma unroll
+          for (int q = 0; q < Q; ++q) y[q] = codes4(v[u][i][q][0], v[u][i][q][1], v[u][i][q][2], v[u][i][q][3]);
+          uint8_t * at = dst + place(w.lo + t, i ? hi : lo);
+          if constexpr (Q == 4) *reinterpret_cast<u4v *>(at) = u4v{y[0], y[1], y[2], y[3]};
+          else if constexpr (Q == 2) *reinterpret_cast<u2v *>(at) = u2v{y[0], y[1]};
+          else *reinterpret_cast<unsigned *>(at) = y[0];
+        }
+      }
+      if (w.lo && before != s) {
+        const float ratio = before * inv;
+        for (int i = threadIdx.x; i < (c.page - n) * chunks; i += 256) {
+          const int t = i / chunks;
+          u4v * at = reinterpret_cast<u4v *>(dst + place(t < w.lo ? t : t + n, (i - t * chunks) * EK));
+          u4v y = *at;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) y[q] = rescale4(y[q], ratio);
+          *at = y;
+        }
+      }
+      if (threadIdx.x == 0) c.ks[w.base + h] = s;
+    }
+  }
+}
+
+// Values of heads [h0, h1).  A thread owns two channels of EV tokens (a granule), 2 x 16 bytes side by
+// side in the stored page, U of them.
 template <int TYPE, int BITS, int U>
-__device__ __forceinline__ void append_values(const AppendParams & p, const PageWork & w, int h, float * red)
+__device__ __forceinline__ void append_values(const AppendParams & p, const PageWork & w, int h0, int h1, float (*red)[4])
 {
   typedef typename St<TYPE>::e E;
   constexpr int EV = BITS == 8 ? 16 : 8;
   const CacheParams & c = p.c;
   const int tid = threadIdx.x, pairs = c.dim / 2;
-  const int g0 = w.lo / EV, work = ((w.hi + EV - 1) / EV - g0) * pairs;  // granules with new tokens
-  const E * src = static_cast<const E *>(p.v) + (long)h * p.v_head;
-  uint8_t * dst = static_cast<uint8_t *>(c.vc) + (w.base + h) * ((long)c.page * c.dim * (BITS / 8));
-  unsigned x[U][EV];
-  float amax = 0.0f;
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int i = tid + 256 * u, g = i / pairs, ch = 2 * (i - g * pairs), slot0 = (g0 + g) * EV;
-    if (i >= work) continue;
+  const int g0 = w.lo / EV, ng = (w.hi + EV - 1) / EV - g0;  // granules with new tokens
+  const int per = 256 / pairs, first = tid / pairs, ch = 2 * (tid - first * pairs);  // granules of a pass; this thread's
+  const bool on = first < per;
+  auto fetch = [&](int h, int slot0, unsigned * x) __attribute__((always_inline)) {
+    const E * src = static_cast<const E *>(p.v) + (long)h * p.v_head + ch;
 #pragma unroll
     for (int t = 0; t < EV; ++t) {
       const int slot = slot0 + t;
       const bool fresh = slot >= w.lo && slot < w.hi;
-      x[u][t] = fresh ? *reinterpret_cast<const unsigned *>(src + (long)(w.row0 + slot - w.lo) * p.v_token + ch) : 0u;
+      x[t] = fresh ? *reinterpret_cast<const unsigned *>(src + (long)(w.row0 + slot - w.lo) * p.v_token) : 0u;
     }
-    if (BITS == 8) {
+  };
+  if constexpr (BITS == 16) {
+    for (int h = h0; h < h1; ++h) {
+      uint8_t * dst = static_cast<uint8_t *>(c.vc) + (w.base + h) * ((long)c.page * c.dim * 2);
+      for (int g = on ? first : ng; g < ng; g += per) {
+        const int slot0 = (g0 + g) * EV;
+        unsigned x[EV];
+        fetch(h, slot0, x);
+        u4v * at = reinterpret_cast<u4v *>(dst + ((long)(g0 + g) * c.dim + ch) * 16);
+        u4v y0, y1;
 #pragma unroll
-      for (int t = 0; t < EV; ++t) {
-        const f2v a = unpack2<TYPE>(x[u][t]);
-        amax = fmaxf(amax, fmaxf(finite_abs(a[0]), finite_abs(a[1])));
-      }
-    } else {
-      u4v * at = reinterpret_cast<u4v *>(dst + ((long)(g0 + g) * c.dim + ch) * 16);
-      u4v y0, y1;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {  // two tokens of one channel, then of the next
-        y0[q] = (x[u][2 * q] & 0xffffu) | (x[u][2 * q + 1] << 16);
-        y1[q] = (x[u][2 * q] >> 16) | (x[u][2 * q + 1] & 0xffff0000u);
-      }
-      if (slot0 < w.lo || slot0 + EV > w.hi) {  // older tokens and slots behind the last one stay
-        const u4v z0 = at[0], z1 = at[1];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const unsigned m = (slot0 + 2 * q >= w.lo && slot0 + 2 * q < w.hi ? 0xffffu : 0u) |
-                             (slot0 + 2 * q + 1 >= w.lo && slot0 + 2 * q + 1 < w.hi ? 0xffff0000u : 0u);
-          y0[q] = (y0[q] & m) | (z0[q] & ~m);
-          y1[q] = (y1[q] & m) | (z1[q] & ~m);
+        for (int q = 0; q < 4; ++q) {  // two tokens of one channel, then of the next
+          y0[q] = (x[2 * q] & 0xffffu) | (x[2 * q + 1] << 16);
+          y1[q] = (x[2 * q] >> 16) | (x[2 * q + 1] & 0xffff0000u);
         }
-      }
-      at[0] = y0;
-      at[1] = y1;
-    }
-  }
-  if constexpr (BITS == 8) {
-    const float before = w.lo ? c.vs[w.base + h] : 0.0f;
-    const float s = group_scale(amax, before, red), inv = 1.0f / s;
-    const bool grown = w.lo && before != s;
-    const float ratio = before * inv;
+        if (slot0 < w.lo || slot0 + EV > w.hi) {  // older tokens and slots behind the last one stay
+          const u4v z0 = at[0], z1 = at[1];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = tid + 256 * u, g = i / pairs, ch = 2 * (i - g * pairs), slot0 = (g0 + g) * EV;
-      if (i >= work) continue;
-      u4v * at = reinterpret_cast<u4v *>(dst + ((long)(g0 + g) * c.dim + ch) * 16);
-      u4v y0, y1;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f2v a = unpack2<TYPE>(x[u][4 * q]), b = unpack2<TYPE>(x[u][4 * q + 1]);
-        const f2v d = unpack2<TYPE>(x[u][4 * q + 2]), e = unpack2<TYPE>(x[u][4 * q + 3]);
-        y0[q] = codes4(a[0] * inv, b[0] * inv, d[0] * inv, e[0] * inv);
-        y1[q] = codes4(a[1] * inv, b[1] * inv, d[1] * inv, e[1] * inv);
-      }
-      if (slot0 < w.lo || slot0 + EV > w.hi) {
-        const u4v z0 = at[0], z1 = at[1];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          unsigned fresh = 0;
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const int slot = slot0 + 4 * q + t;
-            if (slot >= w.lo && slot < w.hi) fresh |= 0xffu << (8 * t);
+          for (int q = 0; q < 4; ++q) {
+            const unsigned m = (slot0 + 2 * q >= w.lo && slot0 + 2 * q < w.hi ? 0xffffu : 0u) |
+                               (slot0 + 2 * q + 1 >= w.lo && slot0 + 2 * q + 1 < w.hi ? 0xffff0000u : 0u);
+            y0[q] = (y0[q] & m) | (z0[q] & ~m);
+            y1[q] = (y1[q] & m) | (z1[q] & ~m);
           }
-          const unsigned o0 = grown ? rescale4(z0[q], ratio) : z0[q], o1 = grown ? rescale4(z1[q], ratio) : z1[q];
-          y0[q] = (y0[q] & fresh) | (o0 & ~fresh);
-          y1[q] = (y1[q] & fresh) | (o1 & ~fresh);
+        }
+        at[0] = y0;
+        at[1] = y1;
+      }
+    }
+  } else {
+    unsigned x[U][EV];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (on && first + per * u < ng) fetch(h0, (g0 + first + per * u) * EV, x[u]);
+    for (int h = h0; h < h1; ++h) {
+      uint8_t * dst = static_cast<uint8_t *>(c.vc) + (w.base + h) * ((long)c.page * c.dim);
+      float amax = 0.0f;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (!on || first + per * u >= ng) continue;
+#pragma unroll
+        for (int t = 0; t < EV; ++t) {
+          const f2v a = unpack2<TYPE>(x[u][t]);
+          amax = fmaxf(fmaxf(amax, fabsf(a[0])), fabsf(a[1]));
         }
       }
-      at[0] = y0;
-      at[1] = y1;
-    }
-    if (grown) {  // the granules without new tokens
-      const int some = (w.hi + EV - 1) / EV - g0;
-      for (int i = tid; i < (c.page / EV - some) * c.dim; i += 256) {
-        u4v * at = reinterpret_cast<u4v *>(dst + (long)(i < g0 * c.dim ? i : i + some * c.dim) * 16);
-        u4v y = *at;
+      const float before = w.lo ? c.vs[w.base + h] : 0.0f;
+      bool saturate;
+      const float s = group_scale(amax, before, red + (h & 1), saturate, [&]() {
+        float m = 0.0f;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) y[q] = rescale4(y[q], ratio);
-        *at = y;
+        for (int u = 0; u < U; ++u) {
+          if (!on || first + per * u >= ng) continue;
+#pragma unroll
+          for (int t = 0; t < EV; ++t) {
+            const f2v a = unpack2<TYPE>(x[u][t]);
+            m = fmaxf(fmaxf(m, finite_abs(a[0])), finite_abs(a[1]));
+          }
+        }
+        return m;
+      });
+      const float inv = 1.0f / s;
+      const bool grown = w.lo && before != s;
+      const float ratio = before * inv;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int g = first + per * u, slot0 = (g0 + g) * EV;
+        if (!on || g >= ng) continue;
+        u4v * at = reinterpret_cast<u4v *>(dst + ((long)(g0 + g) * c.dim + ch) * 16);
+        u4v y0, y1;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          f2v a[4];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) a[t] = unpack2<TYPE>(x[u][4 * q + t]) * inv;
+          if (saturate) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) a[t] = f2v{saturated(a[t][0]), saturated(a[t][1])};
+          }
+          y0[q] = codes4(a[0][0], a[1][0], a[2][0], a[3][0]);
+          y1[q] = codes4(a[0][1], a[1][1], a[2][1], a[3][1]);
+        }
+        if (h + 1 < h1) fetch(h + 1, slot0, x[u]);
+        if (slot0 < w.lo || slot0 + EV > w.hi) {
+          const u4v z0 = at[0], z1 = at[1];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            unsigned fresh = 0;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              const int slot = slot0 + 4 * q + t;
+              if (slot >= w.lo && slot < w.hi) fresh |= 0xffu << (8 * t);
+            }
+            const unsigned o0 = grown ? rescale4(z0[q], ratio) : z0[q], o1 = grown ? rescale4(z1[q], ratio) : z1[q];
+            y0[q] = (y0[q] & fresh) | (o0 & ~fresh);
+            y1[q] = (y1[q] & fresh) | (o1 & ~fresh);
+          }
+        }
+        at[0] = y0;
+        at[1] = y1;
       }
+      if (grown) {  // the granules without new tokens
+        for (int i = tid; i < (c.page / EV - ng) * c.dim; i += 256) {
+          u4v * at = reinterpret_cast<u4v *>(dst + (long)(i < g0 * c.dim ? i : i + ng * c.dim) * 16);
+          u4v y = *at;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) y[q] = rescale4(y[q], ratio);
+          *at = y;
+        }
+      }
+      if (tid == 0) c.vs[w.base + h] = s;
     }
-    if (tid == 0) c.vs[w.base + h] = s;
   }
 }
 
-// UK, UV: 16-byte pieces of keys and 32-byte pieces of values a thread holds of a whole page.
-template <int TYPE, int BITS, int UK, int UV>
-__global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p)
+// R: channels of a run of keys; UK, UV: units of keys and 32-byte pieces of values a thread holds of a
+// whole page.  A work-group takes `span` heads, for the keys' of which it forms the angles once.
+template <int TYPE, int BITS, int R, int UK, int UV>
+__global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p, int span)
 {
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-  __shared__ float red[4];
+  __shared__ float red[4][4];  // of even and uneven heads, in each case a second for pages with infinities
   PageWork w;
   if (!page_work(p.c, blockIdx.x, w)) return;
-  if (blockIdx.z == 0) append_keys<TYPE, BITS, UK>(p, w, blockIdx.y, red, reinterpret_cast<f2v *>(lds));
-  else append_values<TYPE, BITS, UV>(p, w, blockIdx.y, red);
+  const int h0 = blockIdx.y * span, h1 = min(h0 + span, p.c.heads);
+  if (blockIdx.z == 0) {
+    float * cos = reinterpret_cast<float *>(lds), * sin = cos + p.c.page * AngleTable<R / 4>::pitch_of(p.r.half) * 4;
+    if (p.r.half) page_angles<R / 4>(p.r, w, cos, sin);
+    __syncthreads();
+    append_keys<TYPE, BITS, R, UK>(p, w, h0, h1, red, cos, sin);
+  } else {
+    append_values<TYPE, BITS, UV>(p, w, h0, h1, red);
+  }
 }
 
 namespace {
 
-template <int TYPE, int BITS> void launch_append(const AppendParams & p, hipStream_t s)
+template <int TYPE, int BITS, int R, int UK, int UV> void launch_append_kernel(const AppendParams & p, hipStream_t s)
 {
   const CacheParams & c = p.c;
-  const dim3 grid((unsigned)((long)c.tokens / c.page + 2L * c.batch), c.heads, 2), blk(256);
-  const size_t lds = (size_t)c.page * p.r.half * sizeof(f2v);
-  const int E = BITS == 8 ? 16 : 8;
-  const int need = (int)std::max<long>(1, ((long)c.page * c.dim / E + 255) / 256);  // pieces a thread
-  auto go = [&](auto kern) {
-    if (lds > 65536) {
-      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-      if (e != hipSuccess) throw std::runtime_error(std::string("HIP error: ") + hipGetErrorString(e));
-    }
-    hipLaunchKernelGGL(kern, grid, blk, lds, s, p);
-  };
-  // a value piece is two channels of a granule: half as many as key pieces
-  if (need <= 1) go(kv_append_kernel<TYPE, BITS, 1, 1>);
-  else if (need <= 2) go(kv_append_kernel<TYPE, BITS, 2, 1>);
-  else if (need <= 4) go(kv_append_kernel<TYPE, BITS, 4, 2>);
-  else if (need <= 8) go(kv_append_kernel<TYPE, BITS, 8, 4>);
-  else go(kv_append_kernel<TYPE, BITS, 16, 8>);
+  auto kern = kv_append_kernel<TYPE, BITS, R, UK, UV>;
+  // heads of a work-group: as many as leave four work-groups a CU (20033 tokens of 8 heads: 37 us with
+  // 4, 43 with 2, 58 with one each); in 16 bits, where no page's maximum is waited for, one
+  const long pages = (long)c.tokens / c.page, wgs = std::max<long>(pages, c.batch) * c.heads * 2;
+  const int span = BITS == 16 ? 1 : (int)std::min<long>(c.heads, std::max<long>(1, wgs / 1024));
+  const dim3 grid((unsigned)(pages + 2L * c.batch), (c.heads + span - 1) / span, 2);
+  const size_t lds = p.r.half ? (size_t)c.page * AngleTable<R / 4>::pitch_of(p.r.half) * 32 : 0;
+  if (lds > 65536) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) throw std::runtime_error(std::string("HIP error: ") + hipGetErrorString(e));
+  }
+  hipLaunchKernelGGL(kern, grid, dim3(256), lds, s, p, span);
+}
+
+template <int TYPE> void launch_append(const AppendParams & p, hipStream_t s)
+{
+  const CacheParams & c = p.c;
+  // runs of 16, 8 or 4 channels, as the rotated channels and the others divide
+  const int R = p.r.rot % 32 == 0 && c.dim % 32 == 0 ? 16 : p.r.rot % 16 == 0 ? 8 : 4;
+  if (c.bits == 16) {  // nothing waits in registers
+    if (R >= 8) launch_append_kernel<TYPE, 16, 8, 1, 1>(p, s);
+    else launch_append_kernel<TYPE, 16, 4, 1, 1>(p, s);
+    return;
+  }
+  // passes over a page: of the keys, 256 / (dim / 2 R) tokens at once; of the values, 512 / dim
+  // granules of 16
+  const int tokens = 256 / (c.dim / (2 * R)), uk = (c.page + tokens - 1) / tokens;
+  const int gran = 256 / (c.dim / 2), uv = (c.page / 16 + gran - 1) / gran;
+  if (R == 16) {
+    if (uk <= 1 && uv <= 1) launch_append_kernel<TYPE, 8, 16, 1, 1>(p, s);
+    else if (uk <= 2 && uv <= 2) launch_append_kernel<TYPE, 8, 16, 2, 2>(p, s);
+    else launch_append_kernel<TYPE, 8, 16, 4, 4>(p, s);
+  } else if (R == 8) {
+    if (uk <= 2 && uv <= 1) launch_append_kernel<TYPE, 8, 8, 2, 1>(p, s);
+    else launch_append_kernel<TYPE, 8, 8, 8, 4>(p, s);
+  } else {
+    launch_append_kernel<TYPE, 8, 4, 16, 4>(p, s);
+  }
 }
 
 }  // namespace
 
 void launch_kv_append(const AppendParams & p, hipStream_t s)
 {
-  const bool f16 = p.c.type == kSeqF16;
-  if (p.c.bits == 8) f16 ? launch_append<kSeqF16, 8>(p, s) : launch_append<kSeqBF16, 8>(p, s);
-  else f16 ? launch_append<kSeqF16, 16>(p, s) : launch_append<kSeqBF16, 16>(p, s);
+  if (p.c.type == kSeqF16) launch_append<kSeqF16>(p, s);
+  else launch_append<kSeqBF16>(p, s);
 }
 
 }  // namespace ivh

@@ -125,18 +125,40 @@ __device__ __forceinline__ int rot_axis(const RotParams & r, int f)
   return (f >= e0) + (f >= e1) + (f >= e2);
 }
 
-// cos and sin of pos * freq.  The angle is formed in turns in 64 bits and only its fraction is
-// rounded to 32: at position 10^6 a 32-bit angle would be off by 0.03 radians.
-__device__ __forceinline__ f2v rot_cossin(int pos, float freq)
+// A frequency in turns (radians / 2 pi) as the sum of two fp32 values.
+__device__ __forceinline__ f2v rot_turns(float freq)
 {
-  const double t = (double)pos * (double)freq * 0.15915494309189535;
-  const float u = (float)(2.0 * (t - rint(t)));
-  f2v cs;
-  float s, c;
-  sincospif(u, &s, &c);
-  cs[0] = c;
-  cs[1] = s;
-  return cs;
+  const double t = (double)freq * 0.15915494309189535;
+  const float h = (float)t;
+  return f2v{h, (float)(t - (double)h)};
+}
+
+// cos and sin of pos * freq; turns: rot_turns(freq).  At position 10^6 an angle of 32 bits would be off by
+// 0.03 radians: the product is formed in two parts, off by 2^-48 of it, of which the whole turns and then
+// the quadrant are dropped before the parts are added; positions from 2^22 on take 64 bits.  Taylor's polynomials up
+// to a quarter of pi are off by 2^-28 before rounding.
+__device__ __forceinline__ f2v rot_cossin(int pos, float freq, f2v turns)
+{
+#pragma clang fp contract(off)  // the product and its remainder are two values
+  const float x = (float)pos, a = x * turns[0];
+  float e = fmaf(x, turns[1], fmaf(x, turns[0], -a)), t = a - rintf(a);
+  if (pos >= 1 << 22 || pos <= -(1 << 22)) {
+    const double d = (double)pos * (double)freq * 0.15915494309189535, f = d - rint(d);
+    t = (float)f;
+    e = (float)(f - (double)t);
+  }
+  const float q = rintf(4.0f * (t + e)), r = 2.0f * (fmaf(q, -0.25f, t) + e), r2 = r * r;  // half turns, in [-1/4, 1/4]
+  constexpr double pi = 3.14159265358979323846, pi2 = pi * pi;
+  constexpr float s1 = (float)pi, s1l = (float)(pi - (double)(float)pi), s3 = (float)(-pi * pi2 / 6), s5 = (float)(pi * pi2 * pi2 / 120),
+                  s7 = (float)(-pi * pi2 * pi2 * pi2 / 5040), s9 = (float)(pi * pi2 * pi2 * pi2 * pi2 / 362880);
+  constexpr float c2 = (float)(-pi2 / 2), c4 = (float)(pi2 * pi2 / 24), c6 = (float)(-pi2 * pi2 * pi2 / 720),
+                  c8 = (float)(pi2 * pi2 * pi2 * pi2 / 40320), c10 = (float)(-pi2 * pi2 * pi2 * pi2 * pi2 / 3628800);
+  const float sp = fmaf(r2, fmaf(r2, fmaf(r2, fmaf(r2, s9, s7), s5), s3), s1l);
+  const float s = fmaf(r, s1, r * sp);
+  const float c = fmaf(r2, fmaf(r2, fmaf(r2, fmaf(r2, fmaf(r2, c10, c8), c6), c4), c2), 1.0f);
+  const unsigned n = (unsigned)(int)q;
+  const unsigned us = __builtin_bit_cast(unsigned, n & 1 ? c : s), uc = __builtin_bit_cast(unsigned, n & 1 ? s : c);
+  return f2v{__builtin_bit_cast(float, uc ^ ((n + 1) << 30 & 0x80000000u)), __builtin_bit_cast(float, us ^ (n << 30 & 0x80000000u))};
 }
 
 // The sequence whose start start(b) is the largest not above w, by a 64-wide search of one wave:
