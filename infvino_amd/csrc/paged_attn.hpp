@@ -448,48 +448,56 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
   }
 }
 
-// Joins the parts of a row: 4 channels a lane, and of every 8th part; the eight lots meet in LDS.  A part that
-// had no keys for the row left a sum of zero, and its values are not read.
+// Joins the parts of a row.  dim / 4 lanes have 4 channels each of every lots-th part, with a running
+// maximum; the lots of a row meet in LDS.  A part that had no keys for the row left a sum of zero, and its
+// values are not read.
 template <int TYPE>
-__global__ void __launch_bounds__(512) paged_join_kernel(const PagedParams p)
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p, int lots)
 {
   typedef typename St<TYPE>::e E;
-  __shared__ __attribute__((aligned(16))) float lds[8][64 * 4];
-  __shared__ float sums[8];
+  __shared__ __attribute__((aligned(16))) float sum[256 * 4];
+  __shared__ float top[256], den[256];
   const CacheParams & c = p.c;
-  const long n = (long)c.tokens * p.heads, row = blockIdx.x;
+  const int lanes = c.dim / 4, tid = threadIdx.x, at = tid / lanes, ch = 4 * (tid - at * lanes);
+  const int per = 256 / (lanes * lots), lot = at / per, sub = at - lot * per;  // rows of a work-group
+  const long n = (long)c.tokens * p.heads, row = (long)blockIdx.x * per + sub;
   const int token = (int)(row / p.heads), head = (int)(row - (long)token * p.heads);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ch = 4 * lane;
-  if (token < c.cu[0] || token >= c.cu[c.batch]) return;  // rows of no sequence stay as they are
+  // rows of no sequence stay as they are
+  const bool on = lot < lots && row < n && token >= c.cu[0] && token < c.cu[c.batch];
   const f2v * ml = reinterpret_cast<const f2v *>(p.ws + (long)p.parts * n * c.dim);
-  // parts are at most 256: a lane has the maxima and sums of four
-  float M = kLowest;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < p.parts) M = fmaxf(M, ml[(long)(lane + 64 * i) * n + row][0]);
-  for (int m = 1; m < 64; m *= 2) M = fmaxf(M, __shfl_xor(M, m));
-  float L = 0.0f;
+  float M = kLowest, L = 0.0f;
   f4v o = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (on) {
 #pragma unroll 4
-  for (int i = wave; i < p.parts; i += 8) {
-    const long at = (long)i * n + row;
-    const f2v t = ml[at];
-    const float e = t[1] != 0.0f ? __builtin_amdgcn_exp2f(t[0] - M) : 0.0f;
-    L = fmaf(t[1], e, L);
-    if (ch < c.dim && t[1] != 0.0f) {
-      const f4v x = *reinterpret_cast<const f4v *>(p.ws + at * c.dim + ch);
+    for (int i = lot; i < p.parts; i += lots) {
+      const long x = (long)i * n + row;
+      const f2v t = ml[x];
+      if (t[1] == 0.0f) continue;
+      const f4v v = *reinterpret_cast<const f4v *>(p.ws + x * c.dim + ch);
+      const float m = fmaxf(M, t[0]), a = __builtin_amdgcn_exp2f(M - m), e = __builtin_amdgcn_exp2f(t[0] - m);
+      M = m;
+      L = L * a + t[1] * e;
 #pragma unroll
-      for (int v = 0; v < 4; ++v) o[v] = fmaf(x[v], e, o[v]);
+      for (int k = 0; k < 4; ++k) o[k] = o[k] * a + v[k] * e;
     }
   }
-  *reinterpret_cast<f4v *>(&lds[wave][ch]) = o;
-  if (lane == 0) sums[wave] = L;
-  __syncthreads();
-  if (wave || ch >= c.dim) return;
+  if (lots > 1) {
+    *reinterpret_cast<f4v *>(sum + 4 * tid) = o;
+    top[tid] = M;
+    den[tid] = L;
+    __syncthreads();
+    if (!on || lot) return;
+    for (int i = 1; i < lots; ++i) {
+      const int other = tid + i * per * lanes;
+      const f4v v = *reinterpret_cast<const f4v *>(sum + 4 * other);
+      const float m = fmaxf(M, top[other]), a = __builtin_amdgcn_exp2f(M - m), e = __builtin_amdgcn_exp2f(top[other] - m);
+      M = m;
+      L = L * a + den[other] * e;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    L += sums[i];
-    o += *reinterpret_cast<const f4v *>(&lds[i][ch]);
+      for (int k = 0; k < 4; ++k) o[k] = o[k] * a + v[k] * e;
+    }
+  } else if (!on) {
+    return;
   }
   const float inv = L != 0.0f ? 1.0f / L : 0.0f;
   const u2v y = {pack2<TYPE>(o[0] * inv, o[1] * inv), pack2<TYPE>(o[2] * inv, o[3] * inv)};
@@ -534,7 +542,12 @@ template <int TYPE> void launch_paged_type(const PagedParams & p, hipStream_t s)
 {
   if (p.c.bits == 8) launch_paged_dim<TYPE, 8>(p, s);
   else launch_paged_dim<TYPE, 16>(p, s);
-  if (p.parts > 1) hipLaunchKernelGGL((paged_join_kernel<TYPE>), dim3((unsigned)((long)p.c.tokens * p.heads)), dim3(512), 0, s, p);
+  if (p.parts > 1) {
+    // a lot for every two parts where lanes allow it
+    const int lanes = p.c.dim / 4, lots = std::max(1, std::min(p.parts / 2, 256 / lanes)), per = 256 / (lanes * lots);
+    const dim3 grid((unsigned)(((long)p.c.tokens * p.heads + per - 1) / per));
+    hipLaunchKernelGGL((paged_join_kernel<TYPE>), grid, dim3(256), 0, s, p, lots);
+  }
 }
 
 }  // namespace
