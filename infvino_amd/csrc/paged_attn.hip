@@ -17,14 +17,16 @@ size_t paged_split(PagedParams & p, int max_new, int max_len)
   const int per_wg = per_wave * p.row_waves;
   p.row_slots = (int)std::min<long>({(rows + per_wg - 1) / per_wg, 1024, (1L << 23) / ((long)c.batch * c.heads)});
   // Keys: a work-group for each CU where there are keys enough (more parts cost more in joining
-  // than they bring: 32 rows over 60000 keys 28 us with 256 work-groups, 34 with 1024), and none longer
-  // than 24 steps a wave, so that a ragged batch's long sequences do not outlast the others (64 of 900 to
-  // 16001 keys 213 us, 220 unsplit; 64 of 8192 each 195 us, 185 unsplit).
+  // than they bring: 32 rows over 60000 keys 28 us with 256 work-groups, 36 with 1024).  With few rows none is
+  // longer than 24 steps a wave, so that a ragged batch's long sequences do not outlast the others (64 of
+  // 900 to 16001 keys 211 us, 220 unsplit; 64 of 8192 each 195 us, 185 unsplit); with many the partial sums would
+  // be too large for that.
   long len = std::min<long>(max_len, (long)c.width * c.page);
   if (p.window) len = std::min<long>(len, (long)p.window + p.sinks + max_new + 128);
   const long steps = (len + 63) / 64, waves = 4 / p.row_waves;
   const long wgs = (long)c.batch * c.heads * p.row_slots;
-  const long want = std::max<long>((256 + wgs - 1) / wgs, (steps + 24 * waves - 1) / (24 * waves));
+  const long balance = p.row_waves < 4 ? (steps + 24 * waves - 1) / (24 * waves) : 1;
+  const long want = std::max<long>((256 + wgs - 1) / wgs, balance);
   const long top = std::max<long>(1, (steps + waves - 1) / waves);
   // a launch holds 2^24 work-groups of 256 lanes
   p.parts = (int)std::min<long>({std::max<long>(want, 1), top, 256, std::max<long>(1, (1L << 23) / wgs)});
