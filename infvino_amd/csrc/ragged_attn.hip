@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(256, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) ragged_
       __syncthreads();
     };
     // what this lane's row sees, less the lane's first key of a 32-key block
-    const int place = row < nq ? row + shift : -(1 << 27);
+    const int place = row < nq ? row + shift : -(1 << 26);  // a row that is not there: as low as one can be
     const int seen_lo = see.lo(place) - 4 * hi, seen_n = see.hi(place) - see.lo(place);
     const int seen_first = min(see.sinks, see.causal ? place + 1 : see.nk) - 4 * hi;
 

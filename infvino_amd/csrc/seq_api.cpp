@@ -96,7 +96,7 @@ ivh::RotParams rotation(const ivh_rotation & r, int dim, const int32_t * pos, in
   return o;
 }
 
-constexpr int kMaxTokens = 1 << 26, kMaxBatch = 1 << 20;
+constexpr int kMaxTokens = 1 << 26, kMaxBatch = 1 << 20, kMaxHeads = 1 << 22;  // the last: sequences times heads
 // a larger window hides nothing either; with it a place less the window stays within 32 bits
 constexpr int kMaxWindow = INT32_MAX - 2 * kMaxTokens;
 
@@ -152,8 +152,8 @@ ivh::PagedParams paged(const ivh_paged_attn_desc * d, int batch, int tokens, siz
   p.c = cache(d->cache);
   check_counts(batch, tokens);
   need(d->heads >= 1 && d->heads % d->cache.heads == 0, "heads must be a multiple of the cache's heads");
-  need((int64_t)tokens * d->heads <= kMaxTokens && (int64_t)batch * d->cache.heads <= (1 << 24), "too many rows for a call");
-  need(std::isfinite(d->scale), "scale must be finite");
+  need((int64_t)tokens * d->heads <= kMaxTokens && (int64_t)batch * d->cache.heads <= kMaxHeads, "too many rows for a call");
+  need(std::isfinite(d->scale * kLog2E), "scale must be finite");
   need(d->window >= 0 && d->sinks >= 0, "window and sinks must not be negative");
   need(d->max_new >= 0 && d->max_len >= 0, "max_new and max_len must not be negative");
   p.c.batch = batch;
@@ -284,9 +284,9 @@ int ivh_attention(const ivh_attn_desc * d, const void * q, const void * k, const
     check_counts(batch, tokens_k);
     need(d->heads >= 1 && d->heads <= 4096 && d->kv_heads >= 1 && d->heads % d->kv_heads == 0,
          "heads must be a multiple of the key heads, at most 4096");
-    need((int64_t)batch * d->heads <= (1 << 24), "too many rows for a call");
+    need((int64_t)batch * d->heads <= kMaxHeads, "too many rows for a call");
     need(d->dim >= 8 && d->dim <= 256 && d->dim % 8 == 0, "dim must be a multiple of 8, at most 256");
-    need(std::isfinite(d->scale), "scale must be finite");
+    need(std::isfinite(d->scale * kLog2E), "scale must be finite");
     need(d->window >= 0 && d->sinks >= 0 && d->max_q >= 0, "window, sinks and max_q must not be negative");
     if (batch == 0 || tokens_q == 0) return;
     check_rows(q, d->q_token, d->q_head, 8, "queries");

@@ -116,6 +116,21 @@ def test_rope(t, tokens, heads, dim, sections, adjacent, dealt):
     assert torch.equal(z.view(torch.int16), y.view(torch.int16))
 
 
+@pytest.mark.parametrize("lo,hi", [((1 << 22) - 40, (1 << 22) + 40), (-(1 << 22) - 40, 40 - (1 << 22)), (1 << 24, (1 << 24) + 80),
+                                   ((1 << 31) - 80, (1 << 31) - 1), (-(1 << 31), 80 - (1 << 31))])
+def test_rope_far_positions(lo, hi):
+    """Angles of positions up to 32 bits: fp32 inputs of 1 and 0 through bf16's own rounding would hide an error, so values
+    that f16 has exactly; 64 bits carry 2 pi x 2^31 turns to 2^-19, which bounds the last two."""
+    code, dt, u = TYPES["f16"]
+    pos = torch.arange(lo, hi, dtype=torch.int64, device="cuda").to(torch.int32).reshape(1, -1)
+    n = pos.shape[1]
+    x = torch.ones((n, 1, 128), dtype=dt, device="cuda")
+    y, freq = torch.empty_like(x), _freq(64)
+    ops.rope(ops.rope_desc(code, 1, 128, (64,)), _p(x), _p(pos), _p(freq), _p(y), n, _stream())
+    ref, mag = _rotated(x, pos, freq, (64,), False, False)
+    assert ((y.double() - ref).abs() <= u * ref.abs() + 2.0 ** -18 * mag + 2.0 ** -25).all()
+
+
 def test_rope_strided_rows():
     """q and k of packed q, k, v rows, written head by head; 8-byte row starts."""
     code, dt, u = TYPES["bf16"]
@@ -214,6 +229,12 @@ APPENDS = [  # bits, heads, dim, page, sections, adjacent, dealt, chunks of each
     (16, 3, 80, 32, (20, 20), True, False, [(70, 1, 5), (0, 0, 1), (31, 33, 64)]),
     (16, 2, 256, 128, (64, 64), False, True, [(130, 1, 300), (1, 127, 1)]),
     (16, 1, 112, 64, (), False, False, [(65, 64, 1)]),
+    # runs of 4 and 8 channels, whole pages of many channels
+    (8, 2, 240, 128, (12,), False, False, [(128, 1, 200), (3, 0, 125)]),
+    (8, 2, 240, 64, (8, 8, 8), True, True, [(70, 30)]),
+    (8, 1, 256, 128, (24, 16), False, True, [(300, 1)]),
+    (8, 1, 192, 128, (64,), True, False, [(129, 129)]),
+    (16, 2, 144, 16, (4, 8), False, False, [(20, 13)]),
 ]
 
 
@@ -728,6 +749,69 @@ def test_graph_and_streams():
         assert torch.equal(o, want) and (o[batch:] == 5.0).all()
         assert torch.equal(cache.kc, plain.kc) and torch.equal(cache.vc, plain.vc)
         _check_paged(cache, qr[:batch], o[:batch], [1] * batch, [m + n for m in start], table, 0, 0, 0.09)
+
+
+def test_offsets_past_32_bits():
+    """Pages whose bytes lie past 2^32: the same codes and results as from pages at the start."""
+    g = _gen(40)
+    kv, dim, page, pages = 8, 128, 128, 36000  # 128 KB a page of keys: 4.7 GB, and as much of values
+    desc = ops.cache_desc(ops.BF16, 8, kv, dim, page, pages, 4)
+    nb, ns = ops.cache_bytes(desc)
+    assert nb > 1 << 32
+    kc, vc = (torch.empty(nb, dtype=torch.uint8, device="cuda") for _ in range(2))
+    ks, vs = (torch.ones(ns // 4, device="cuda") for _ in range(2))
+    n = 300
+    k, v, q = (_randn(g, torch.bfloat16, n, h, dim) for h in (kv, kv, 16))
+    cu, lens = _ends([n]), _i32([n])
+    got = []
+    for ids in ([0, 1, 2, -1], [pages - 1, pages - 3, pages - 2, -1]):
+        table = _i32([ids])
+        ops.kv_append(ops.append_desc(desc), _p(k), _p(v), None, None, _p(cu), _p(lens), _p(table), _p(kc), _p(vc), _p(ks), _p(vs), 1, n, _stream())
+        d = ops.paged_attention_desc(desc, 16, 0.1, max_new=n, max_len=n)
+        ws = torch.empty(max(16, ops.paged_attention_workspace(d, 1, n)), dtype=torch.uint8, device="cuda")
+        o = torch.empty_like(q)
+        ops.paged_attention(d, _p(q), _p(kc), _p(vc), _p(ks), _p(vs), _p(cu), _p(lens), _p(table), _p(o), 1, n, _p(ws), ws.numel(), _stream())
+        at = torch.tensor(ids[:3], device="cuda")
+        got.append([o, ks.reshape(pages, kv)[at], vs.reshape(pages, kv)[at]] + [torch.stack([c.reshape(pages, -1)[i] for i in ids[:3]]) for c in (kc, vc)])
+    for a, b in zip(*got):
+        # the last page's empty slots are whatever the memory held
+        if a.dtype == torch.uint8:
+            assert torch.equal(a[:2], b[:2])
+        else:
+            assert torch.equal(a, b)
+
+
+def test_two_graphs_at_once():
+    """Two captured calls with a workspace each, replayed on two streams at once, with a strided output."""
+    g = _gen(41)
+    heads, kv, dim, page = 16, 2, 128, 32
+    lens, new = [5000, 3000], [1, 1]
+    cache = Cache("bf16", 8, kv, dim, page, 300, 160)
+    table = _tables(g, [-(-n // page) for n in lens], 160, 300)
+    _fill(cache, g, table, lens)
+    cu, dl, tb = _ends(new), _i32(lens), _i32(table)
+    # output head by head
+    d = ops.paged_attention_desc(cache.desc, heads, 0.09, o=(dim, 2 * dim), max_new=1, max_len=5000)
+    need = ops.paged_attention_workspace(d, 2, 2)
+    assert need > 0
+    runs = []
+    for _ in range(2):
+        q, o = _randn(g, cache.dt, 2, heads, dim), torch.empty((heads, 2, dim), dtype=cache.dt, device="cuda")
+        ws, s, graph = torch.empty(need, dtype=torch.uint8, device="cuda"), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=s):
+            ops.paged_attention(d, _p(q), _p(cache.kc), _p(cache.vc), _p(cache.ks), _p(cache.vs), _p(cu), _p(dl), _p(tb), _p(o), 2, 2, _p(ws), need, _stream())
+        runs.append((q, o, ws, s, graph))
+    for _ in range(5):
+        for q, o, ws, s, graph in runs:
+            o.fill_(7.0)
+        torch.cuda.synchronize()
+        for q, o, ws, s, graph in runs:
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for q, o, ws, s, graph in runs:
+            _check_paged(cache, q, o.transpose(0, 1), new, lens, table, 0, 0, 0.09)
 
 
 def test_operands_that_are_not_on_the_device():

@@ -124,6 +124,12 @@ def test_paged_attention_refuses_operands_and_workspace():
         _paged(many, ws=A + 8, ws_bytes=need)
     with pytest.raises(RuntimeError, match="too many rows"):
         _paged(one, tokens=1 << 25)
+    with pytest.raises(RuntimeError, match="too many rows"):
+        ops.paged_attention_workspace(ops.paged_attention_desc(_cache(heads=64), 64, 0.1), 1 << 17, 1)
+    with pytest.raises(RuntimeError, match="too many rows"):
+        ops.attention(ops.attention_desc(ops.F16, 64, 2, 64, 0.1), *[A] * 6, 1 << 17, 4, 4)
+    with pytest.raises(RuntimeError, match="finite"):
+        ops.paged_attention_workspace(ops.paged_attention_desc(_cache(), 4, 3e38), 1, 1)
 
 
 @pytest.mark.parametrize("kw,msg", [({"type": -1}, "type"), ({"kv_heads": 3}, "multiple"), ({"kv_heads": 0}, "multiple"),
