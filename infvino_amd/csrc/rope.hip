@@ -179,14 +179,28 @@ __device__ __forceinline__ bool page_work(const CacheParams & c, int w, PageWork
 {
   const int * cu = c.cu;
   const int tokens = c.tokens, page = c.page;
-  auto start = [&](int b) { return (long)(min(max(cu[b], 0), tokens) / page) + 2L * b; };
-  const int b = __builtin_amdgcn_readfirstlane(find_seq(c.batch, w, start));
-  const int c0 = min(max(cu[b], 0), tokens), c1 = min(max(cu[b + 1], c0), tokens);
-  const long old = (long)c.lens[b] - (c1 - c0);  // place of the first new token; below 0: not stored
+  auto start = [&](int b, int first) { return (long)(min(max(first, 0), tokens) / page) + 2L * b; };
+  int b, c0, c1, len;
+  if (c.batch < 64) {  // all sequences at once, a lane each: one trip to memory instead of two
+    const int lane = threadIdx.x & 63, x = cu[min(lane, c.batch)], y = c.lens[min(lane, c.batch - 1)];
+    const unsigned long long below = __ballot(lane < c.batch && start(lane, x) <= w);
+    b = below ? 63 - __clzll(below) : 0;
+    c0 = __builtin_amdgcn_readlane(x, b);
+    c1 = __builtin_amdgcn_readlane(x, b + 1);
+    len = __builtin_amdgcn_readlane(y, b);
+  } else {
+    b = __builtin_amdgcn_readfirstlane(find_seq(c.batch, w, [&](int i) { return start(i, cu[i]); }));
+    c0 = cu[b];
+    c1 = cu[b + 1];
+    len = c.lens[b];
+  }
+  c0 = min(max(c0, 0), tokens);
+  c1 = min(max(c1, c0), tokens);
+  const long old = (long)len - (c1 - c0);  // place of the first new token; below 0: not stored
   const long first = (old > 0 ? old : 0) / page;
-  const long at = first + (w - start(b));
+  const long at = first + (w - start(b, c0));
   if (at < first || at >= c.width) return false;
-  const long lo = max(old, at * page), hi = min((long)c.lens[b], (at + 1) * page);
+  const long lo = max(old, at * page), hi = min((long)len, (at + 1) * page);
   if (lo >= hi) return false;
   const int id = c.table[(long)b * c.width + at];
   if ((unsigned)id >= (unsigned)c.pages) return false;
@@ -282,8 +296,8 @@ __device__ __forceinline__ void page_angles(const RotParams & r, const PageWork 
 // two: channels f.. and rot / 2 + f.., or 2 R in a row (adjacent pairs, and what is not rotated); U such
 // units.  The next head's rows are asked for as soon as this one's are turned.
 template <int TYPE, int BITS, int R, int U>
-__device__ __forceinline__ void append_keys(const AppendParams & p, const PageWork & w, int h0, int h1, float (*red)[4], const float * cos,
-                                            const float * sin)
+__device__ __forceinline__ void append_keys(const AppendParams & p, const PageWork & w, int h0, int h1, float (*red)[4], float * cos,
+                                            float * sin)
 {
   typedef typename St<TYPE>::e E;
   constexpr int EK = BITS == 8 ? 16 : 8, Q = R / 4;
@@ -343,6 +357,8 @@ __device__ __forceinline__ void append_keys(const AppendParams & p, const PageWo
     }
   };
   if constexpr (BITS == 16) {
+    if (r.half) page_angles<Q>(r, w, cos, sin);
+    __syncthreads();
     for (int h = h0; h < h1; ++h) {
       uint8_t * dst = static_cast<uint8_t *>(c.kc) + (w.base + h) * ((long)c.page * c.dim * 2);
 #pragma unroll 2
@@ -371,8 +387,11 @@ __device__ __forceinline__ void append_keys(const AppendParams & p, const PageWo
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (on && t0 + per * u < n) fetch(h0, t0 + per * u, x[u]);
+    if (r.half) page_angles<Q>(r, w, cos, sin);
+    __syncthreads();
     for (int h = h0; h < h1; ++h) {
       uint8_t * dst = static_cast<uint8_t *>(c.kc) + (w.base + h) * ((long)c.page * c.dim);
+      const float before = w.lo ? c.ks[w.base + h] : 0.0f;
       f4v v[U][2][Q];
       auto all = [&](auto && fn) __attribute__((always_inline)) {  // fn over the thread's values
 #pragma unroll
@@ -396,7 +415,6 @@ __device__ __forceinline__ void append_keys(const AppendParams & p, const PageWo
         amax = fmaxf(amax, fabsf(y));
         return y;
       });
-      const float before = w.lo ? c.ks[w.base + h] : 0.0f;
       bool saturate;
       const float s = group_scale(amax, before, red + (h & 1), saturate, [&]() {
         float m = 0.0f;
@@ -496,6 +514,7 @@ __device__ __forceinline__ void append_values(const AppendParams & p, const Page
       if (on && first + per * u < ng) fetch(h0, (g0 + first + per * u) * EV, x[u]);
     for (int h = h0; h < h1; ++h) {
       uint8_t * dst = static_cast<uint8_t *>(c.vc) + (w.base + h) * ((long)c.page * c.dim);
+      const float before = w.lo ? c.vs[w.base + h] : 0.0f;
       float amax = 0.0f;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -506,7 +525,6 @@ __device__ __forceinline__ void append_values(const AppendParams & p, const Page
           amax = fmaxf(fmaxf(amax, fabsf(a[0])), fabsf(a[1]));
         }
       }
-      const float before = w.lo ? c.vs[w.base + h] : 0.0f;
       bool saturate;
       const float s = group_scale(amax, before, red + (h & 1), saturate, [&]() {
         float m = 0.0f;
@@ -587,8 +605,6 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p, in
   const int h0 = blockIdx.y * span, h1 = min(h0 + span, p.c.heads);
   if (blockIdx.z == 0) {
     float * cos = reinterpret_cast<float *>(lds), * sin = cos + p.c.page * AngleTable<R / 4>::pitch_of(p.r.half) * 4;
-    if (p.r.half) page_angles<R / 4>(p.r, w, cos, sin);
-    __syncthreads();
     append_keys<TYPE, BITS, R, UK>(p, w, h0, h1, red, cos, sin);
   } else {
     append_values<TYPE, BITS, UV>(p, w, h0, h1, red);
