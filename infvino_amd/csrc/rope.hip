@@ -232,9 +232,10 @@ __device__ __forceinline__ unsigned rescale4(unsigned x, float ratio)
 }
 
 // maximum over the work-group
-__device__ __forceinline__ float group_max(float amax, float * red)
+template <int NT> __device__ __forceinline__ float group_max(float amax, float * red)
 {
   for (int m = 1; m < 64; m *= 2) amax = fmaxf(amax, __shfl_xor(amax, m));
+  if (NT == 64) return amax;
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = amax;
   __syncthreads();
   return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
@@ -243,12 +244,12 @@ __device__ __forceinline__ float group_max(float amax, float * red)
 // The page's new scale; amax: this thread's largest magnitude.  If there is an infinity among the
 // work-group's values (all of its threads see that), `finite` gives the thread's largest finite one, and
 // saturate is set: infinities are to become the largest code.  A NaN is passed over by the maximum.
-template <class Fn>
+template <int NT, class Fn>
 __device__ __forceinline__ float group_scale(float amax, float before, float (*red)[4], bool & saturate, Fn && finite)
 {
-  amax = group_max(amax, red[0]);
+  amax = group_max<NT>(amax, red[0]);
   saturate = !(amax < __builtin_inff());
-  if (saturate) amax = group_max(finite(), red[2]);
+  if (saturate) amax = group_max<NT>(finite(), red[2]);
   return fmaxf(page_scale(amax), before);
 }
 __device__ __forceinline__ float finite_abs(float x)
@@ -276,11 +277,11 @@ template <int Q> struct AngleTable {
   __device__ __forceinline__ int at(int t, int f) const { return (t * pitch + f / 4 % Q * lots + f / 4 / Q) * 4 + f % 4; }
 };
 
-template <int Q>
+template <int NT, int Q>
 __device__ __forceinline__ void page_angles(const RotParams & r, const PageWork & w, float * cos, float * sin)
 {
   const AngleTable<Q> table(r.half);
-  const int per = 256 / r.half, t0 = threadIdx.x / r.half, f = threadIdx.x - t0 * r.half, n = w.hi - w.lo;
+  const int per = NT / r.half, t0 = threadIdx.x / r.half, f = threadIdx.x - t0 * r.half, n = w.hi - w.lo;
   if (t0 >= per) return;
   const float freq = r.freq[f];
   const f2v turns = rot_turns(freq);
@@ -295,7 +296,7 @@ __device__ __forceinline__ void page_angles(const RotParams & r, const PageWork 
 // Keys of heads [h0, h1).  A thread owns two runs of R channels of a token whose pairs lie within the
 // two: channels f.. and rot / 2 + f.., or 2 R in a row (adjacent pairs, and what is not rotated); U such
 // units.  The next head's rows are asked for as soon as this one's are turned.
-template <int TYPE, int BITS, int R, int U>
+template <int TYPE, int BITS, int NT, int R, int U>
 __device__ __forceinline__ void append_keys(const AppendParams & p, const PageWork & w, int h0, int h1, float (*red)[4], float * cos,
                                             float * sin)
 {
@@ -304,7 +305,7 @@ __device__ __forceinline__ void append_keys(const AppendParams & p, const PageWo
   const CacheParams & c = p.c;
   const RotParams & r = p.r;
   const int units = c.dim / (2 * R), chunks = c.dim / EK, n = w.hi - w.lo;
-  const int per = 256 / units, t0 = threadIdx.x / units, unit = threadIdx.x - t0 * units;  // tokens of a pass; this thread's
+  const int per = NT / units, t0 = threadIdx.x / units, unit = threadIdx.x - t0 * units;  // tokens of a pass; this thread's
   const bool on = t0 < per, turn = unit * 2 * R < r.rot;
   const bool split = turn && !r.adjacent;
   const int lo = split ? unit * R : unit * 2 * R, hi = split ? lo + r.half : lo + R, f0 = unit * R;
@@ -357,7 +358,7 @@ __device__ __forceinline__ void append_keys(const AppendParams & p, const PageWo
     }
   };
   if constexpr (BITS == 16) {
-    if (r.half) page_angles<Q>(r, w, cos, sin);
+    if (r.half) page_angles<NT, Q>(r, w, cos, sin);
     __syncthreads();
     for (int h = h0; h < h1; ++h) {
       uint8_t * dst = static_cast<uint8_t *>(c.kc) + (w.base + h) * ((long)c.page * c.dim * 2);
@@ -387,7 +388,7 @@ __device__ __forceinline__ void append_keys(const AppendParams & p, const PageWo
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (on && t0 + per * u < n) fetch(h0, t0 + per * u, x[u]);
-    if (r.half) page_angles<Q>(r, w, cos, sin);
+    if (r.half) page_angles<NT, Q>(r, w, cos, sin);
     __syncthreads();
     for (int h = h0; h < h1; ++h) {
       uint8_t * dst = static_cast<uint8_t *>(c.kc) + (w.base + h) * ((long)c.page * c.dim);
@@ -416,7 +417,7 @@ __device__ __forceinline__ void append_keys(const AppendParams & p, const PageWo
         return y;
       });
       bool saturate;
-      const float s = group_scale(amax, before, red + (h & 1), saturate, [&]() {
+      const float s = group_scale<NT>(amax, before, red + (h & 1), saturate, [&]() {
         float m = 0.0f;
         all([&](float y) {
           m = fmaxf(m, finite_abs(y));
@@ -444,7 +445,7 @@ __device__ __forceinline__ void append_keys(const AppendParams & p, const PageWo
       }
       if (w.lo && before != s) {
         const float ratio = before * inv;
-        for (int i = threadIdx.x; i < (c.page - n) * chunks; i += 256) {
+        for (int i = threadIdx.x; i < (c.page - n) * chunks; i += NT) {
           const int t = i / chunks;
           u4v * at = reinterpret_cast<u4v *>(dst + place(t < w.lo ? t : t + n, (i - t * chunks) * EK));
           u4v y = *at;
@@ -460,7 +461,7 @@ __device__ __forceinline__ void append_keys(const AppendParams & p, const PageWo
 
 // Values of heads [h0, h1).  A thread owns two channels of EV tokens (a granule), 2 x 16 bytes side by
 // side in the stored page, U of them.
-template <int TYPE, int BITS, int U>
+template <int TYPE, int BITS, int NT, int U>
 __device__ __forceinline__ void append_values(const AppendParams & p, const PageWork & w, int h0, int h1, float (*red)[4])
 {
   typedef typename St<TYPE>::e E;
@@ -468,7 +469,7 @@ __device__ __forceinline__ void append_values(const AppendParams & p, const Page
   const CacheParams & c = p.c;
   const int tid = threadIdx.x, pairs = c.dim / 2;
   const int g0 = w.lo / EV, ng = (w.hi + EV - 1) / EV - g0;  // granules with new tokens
-  const int per = 256 / pairs, first = tid / pairs, ch = 2 * (tid - first * pairs);  // granules of a pass; this thread's
+  const int per = NT / pairs, first = tid / pairs, ch = 2 * (tid - first * pairs);  // granules of a pass; this thread's
   const bool on = first < per;
   auto fetch = [&](int h, int slot0, unsigned * x) __attribute__((always_inline)) {
     const E * src = static_cast<const E *>(p.v) + (long)h * p.v_head + ch;
@@ -526,7 +527,7 @@ __device__ __forceinline__ void append_values(const AppendParams & p, const Page
         }
       }
       bool saturate;
-      const float s = group_scale(amax, before, red + (h & 1), saturate, [&]() {
+      const float s = group_scale<NT>(amax, before, red + (h & 1), saturate, [&]() {
         float m = 0.0f;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -580,7 +581,7 @@ __device__ __forceinline__ void append_values(const AppendParams & p, const Page
         at[1] = y1;
       }
       if (grown) {  // the granules without new tokens
-        for (int i = tid; i < (c.page / EV - ng) * c.dim; i += 256) {
+        for (int i = tid; i < (c.page / EV - ng) * c.dim; i += NT) {
           u4v * at = reinterpret_cast<u4v *>(dst + (long)(i < g0 * c.dim ? i : i + ng * c.dim) * 16);
           u4v y = *at;
 #pragma unroll
@@ -593,10 +594,10 @@ __device__ __forceinline__ void append_values(const AppendParams & p, const Page
   }
 }
 
-// R: channels of a run of keys; UK, UV: units of keys and 32-byte pieces of values a thread holds of a
+// NT: lanes; R: channels of a run of keys; UK, UV: units of keys and 32-byte pieces of values a thread holds of a
 // whole page.  A work-group takes `span` heads, for the keys' of which it forms the angles once.
-template <int TYPE, int BITS, int R, int UK, int UV>
-__global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p, int span)
+template <int TYPE, int BITS, int NT, int R, int UK, int UV>
+__global__ void __launch_bounds__(NT) kv_append_kernel(const AppendParams p, int span)
 {
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   __shared__ float red[4][4];  // of even and uneven heads, in each case a second for pages with infinities
@@ -605,18 +606,18 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p, in
   const int h0 = blockIdx.y * span, h1 = min(h0 + span, p.c.heads);
   if (blockIdx.z == 0) {
     float * cos = reinterpret_cast<float *>(lds), * sin = cos + p.c.page * AngleTable<R / 4>::pitch_of(p.r.half) * 4;
-    append_keys<TYPE, BITS, R, UK>(p, w, h0, h1, red, cos, sin);
+    append_keys<TYPE, BITS, NT, R, UK>(p, w, h0, h1, red, cos, sin);
   } else {
-    append_values<TYPE, BITS, UV>(p, w, h0, h1, red);
+    append_values<TYPE, BITS, NT, UV>(p, w, h0, h1, red);
   }
 }
 
 namespace {
 
-template <int TYPE, int BITS, int R, int UK, int UV> void launch_append_kernel(const AppendParams & p, hipStream_t s)
+template <int TYPE, int BITS, int NT, int R, int UK, int UV> void launch_append_kernel(const AppendParams & p, hipStream_t s)
 {
   const CacheParams & c = p.c;
-  auto kern = kv_append_kernel<TYPE, BITS, R, UK, UV>;
+  auto kern = kv_append_kernel<TYPE, BITS, NT, R, UK, UV>;
   // heads of a work-group: as many as leave four work-groups a CU (20033 tokens of 8 heads: 37 us with
   // 4, 43 with 2, 58 with one each); in 16 bits, where no page's maximum is waited for, one
   const long pages = (long)c.tokens / c.page, wgs = std::max<long>(pages, c.batch) * c.heads * 2;
@@ -627,7 +628,7 @@ template <int TYPE, int BITS, int R, int UK, int UV> void launch_append_kernel(c
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) throw std::runtime_error(std::string("HIP error: ") + hipGetErrorString(e));
   }
-  hipLaunchKernelGGL(kern, grid, dim3(256), lds, s, p, span);
+  hipLaunchKernelGGL(kern, grid, dim3(NT), lds, s, p, span);
 }
 
 template <int TYPE> void launch_append(const AppendParams & p, hipStream_t s)
@@ -636,23 +637,39 @@ template <int TYPE> void launch_append(const AppendParams & p, hipStream_t s)
   // runs of 16, 8 or 4 channels, as the rotated channels and the others divide
   const int R = p.r.rot % 32 == 0 && c.dim % 32 == 0 ? 16 : p.r.rot % 16 == 0 ? 8 : 4;
   if (c.bits == 16) {  // nothing waits in registers
-    if (R >= 8) launch_append_kernel<TYPE, 16, 8, 1, 1>(p, s);
-    else launch_append_kernel<TYPE, 16, 4, 1, 1>(p, s);
+    if (R >= 8) launch_append_kernel<TYPE, 16, 256, 8, 1, 1>(p, s);
+    else launch_append_kernel<TYPE, 16, 256, 4, 1, 1>(p, s);
     return;
   }
   // passes over a page: of the keys, 256 / (dim / 2 R) tokens at once; of the values, 512 / dim
   // granules of 16
   const int tokens = 256 / (c.dim / (2 * R)), uk = (c.page + tokens - 1) / tokens;
   const int gran = 256 / (c.dim / 2), uv = (c.page / 16 + gran - 1) / gran;
+  // One wave does a page where the other three would have little to do: pages of 16, or a token or two for
+  // each sequence. Registers for four passes cost more than they save while the chip is not full. One
+  // wave / four, 8 heads of 128 channels, in us: 60 sequences of a token each, pages of 16, 5.6 / 9.2;
+  // 512 of them, pages of 64, 23.0 / 30.5; 8 prompts of 200, pages of 16, 7.5 / 12.1; one token, pages of
+  // 64, 6.0 / 4.5 (so not there).
+  const bool few = (long)c.tokens <= 4L * c.batch, small = c.page * c.dim <= 64 * 32;
+  if (R == 16 && uk <= 1 && uv <= 1 && p.r.half <= 64 && c.dim <= 128 && (few || c.page == 16)) {
+    if (small) {
+      launch_append_kernel<TYPE, 8, 64, 16, 1, 1>(p, s);
+      return;
+    }
+    if ((long)c.batch * c.heads >= 256) {
+      launch_append_kernel<TYPE, 8, 64, 16, 4, 4>(p, s);
+      return;
+    }
+  }
   if (R == 16) {
-    if (uk <= 1 && uv <= 1) launch_append_kernel<TYPE, 8, 16, 1, 1>(p, s);
-    else if (uk <= 2 && uv <= 2) launch_append_kernel<TYPE, 8, 16, 2, 2>(p, s);
-    else launch_append_kernel<TYPE, 8, 16, 4, 4>(p, s);
+    if (uk <= 1 && uv <= 1) launch_append_kernel<TYPE, 8, 256, 16, 1, 1>(p, s);
+    else if (uk <= 2 && uv <= 2) launch_append_kernel<TYPE, 8, 256, 16, 2, 2>(p, s);
+    else launch_append_kernel<TYPE, 8, 256, 16, 4, 4>(p, s);
   } else if (R == 8) {
-    if (uk <= 2 && uv <= 1) launch_append_kernel<TYPE, 8, 8, 2, 1>(p, s);
-    else launch_append_kernel<TYPE, 8, 8, 8, 4>(p, s);
+    if (uk <= 2 && uv <= 1) launch_append_kernel<TYPE, 8, 256, 8, 2, 1>(p, s);
+    else launch_append_kernel<TYPE, 8, 256, 8, 8, 4>(p, s);
   } else {
-    launch_append_kernel<TYPE, 8, 4, 16, 4>(p, s);
+    launch_append_kernel<TYPE, 8, 256, 4, 16, 4>(p, s);
   }
 }
 

@@ -235,6 +235,14 @@ APPENDS = [  # bits, heads, dim, page, sections, adjacent, dealt, chunks of each
     (8, 1, 256, 128, (24, 16), False, True, [(300, 1)]),
     (8, 1, 192, 128, (64,), True, False, [(129, 129)]),
     (16, 2, 144, 16, (4, 8), False, False, [(20, 13)]),
+    # many sequences, some of them without new tokens
+    (8, 2, 64, 16, (32,), False, False, [(i % 5, i % 3 == 0, 1) for i in range(63)]),
+    (8, 1, 128, 32, (24, 20, 20), False, True, [(i % 41, i % 3, 1) for i in range(70)]),
+    (8, 3, 32, 64, (), False, False, [(0 if i % 7 else 70, 1, 2) for i in range(130)]),
+    (16, 2, 64, 16, (32,), True, False, [(i % 19, i % 2, 1) for i in range(200)]),
+    (8, 4, 128, 64, (32,), False, False, [(i % 7 and 3 + i % 90, i % 3, 3, 60 * (i == 5)) for i in range(70)]),
+    (8, 4, 96, 64, (16, 32), False, True, [(i % 7 and 3 + i % 64, i % 3, 3) for i in range(66)]),
+    (8, 8, 64, 128, (), False, False, [(i % 5 and 3 + i % 150, i % 3, 3) for i in range(40)]),
 ]
 
 
