@@ -472,6 +472,21 @@ PAGED = [  # bits, heads, kv heads, dim, page, new, lens, window, sinks
     (16, 8, 1, 64, 16, [300], [700], 0, 0),
     (16, 8, 4, 256, 32, [40, 3], [500, 70], 33, 10),
     (16, 4, 1, 112, 16, [1, 9], [500, 300], 17, 1),
+    # batches that fill the chip, whose waves take rows: four row ranges, then two
+    (8, 8, 8, 128, 16, [70, 65] + [1, 0, 17] * 4, [300, 65] + [1, 40, 190] * 4, 0, 0),
+    (8, 8, 8, 128, 64, [70] + [2] * 13, [500] + [290] * 13, 50, 3),
+    (8, 8, 8, 80, 32, [80, 3] * 7, [80, 400] * 7, 0, 0),
+    (8, 8, 8, 64, 32, [100] + [5] * 23, [400] + [131] * 23, 0, 0),
+    (8, 8, 8, 256, 16, [70] + [1] * 13, [270] + [33] * 13, 0, 0),
+    (16, 8, 8, 128, 16, [70, 65] + [1, 0, 17] * 4, [300, 65] + [1, 40, 190] * 4, 0, 0),
+    (16, 8, 8, 64, 32, [100] + [5] * 23, [400] + [131] * 23, 70, 0),
+    (16, 8, 8, 256, 16, [70] + [1] * 13, [270] + [33] * 13, 0, 0),
+    (8, 32, 8, 128, 16, [5, 1, 0, 8] * 9, [40, 17, 3, 200] * 9, 0, 0),
+    (8, 32, 8, 64, 16, [9, 1, 0, 16] * 9, [40, 17, 3, 200] * 9, 20, 2),
+    (8, 32, 8, 240, 16, [5, 1, 0, 8] * 9, [40, 17, 3, 200] * 9, 0, 0),
+    (16, 32, 8, 128, 16, [5, 1, 0, 8] * 9, [40, 17, 3, 200] * 9, 0, 0),
+    (16, 32, 8, 64, 16, [9, 1, 0, 16] * 9, [40, 17, 3, 200] * 9, 0, 0),
+    (16, 32, 8, 256, 16, [5, 1, 0, 8] * 9, [40, 17, 3, 200] * 9, 33, 0),
 ]
 
 
