@@ -231,7 +231,7 @@ int ivh_bmm_f16(const void * a, const void * b, void * y, int bb, int m, int k, 
 
 /* Rotary positions: frequency f < rot / 2 turns a pair of a head's first rot channels by
    pos[axis(f)][token] * freq[f] radians: (a, b) -> (a cos - b sin, b cos + a sin).  Channels from rot on
-   stay.  Angles are formed in 64 bits, the rotation in fp32, rounded once. */
+   stay.  Angles are formed in 47 bits or more, the rotation in fp32, rounded once. */
 typedef struct ivh_rotation {
   int rot;                  /* rotated channels of a head, a multiple of 8 */
   int adjacent;             /* pairs: 0 channels (f, f + rot / 2), 1 channels (2 f, 2 f + 1) */
@@ -286,8 +286,9 @@ typedef struct ivh_append_desc {
    lens[b] - (cu[b + 1] - cu[b]) + i.  An 8-bit page's scale is the smallest power of two s with
    max |x| <= 448 s over the page's new values of a head, at least 2^-32 and at least the scale of
    older tokens in the page; when it grows, the page's other codes of that head are rounded to it
-   (nearest, ties to even).  Infinities are stored as +-448 s, NaN as NaN; neither counts for s.  A page that gets tokens must belong to one
-   sequence alone; ks and vs of a page without tokens need no value. */
+   (nearest, ties to even).  Infinities are stored as +-448 s, NaN as NaN; neither counts for s.
+   A page that gets tokens must stand in the tables once, in one sequence's; a full page may be
+   shared.  ks and vs of a page without tokens need no value.  The rows must not overlap the cache. */
 int ivh_kv_append(const ivh_append_desc * d, const void * k, const void * v, const int32_t * pos, const float * freq,
                   const int32_t * cu, const int32_t * lens, const int32_t * table, void * kc, void * vc, float * ks,
                   float * vs, int batch, int tokens, void * stream);
@@ -307,7 +308,8 @@ typedef struct ivh_paged_attn_desc {
    same time need one each; its contents before a call do not matter */
 int ivh_paged_attention_workspace(const ivh_paged_attn_desc * d, int batch, int tokens, size_t * bytes);
 /* o = softmax(scale q k^T) v over the cached tokens of each row's sequence; lens, cu as for the append
-   that stored the rows' own tokens.  A row that sees no key is zero. */
+   that stored the rows' own tokens.  A row that sees no key is zero; infinities and NaN reach only
+   rows that see them.  o must not overlap an operand. */
 int ivh_paged_attention(const ivh_paged_attn_desc * d, const void * q, const void * kc, const void * vc, const float * ks,
                         const float * vs, const int32_t * cu, const int32_t * lens, const int32_t * table, void * o,
                         int batch, int tokens, void * workspace, size_t workspace_bytes, void * stream);
@@ -323,7 +325,7 @@ typedef struct ivh_attn_desc {
 } ivh_attn_desc;
 
 /* The same over contiguous rows: sequence b's queries are rows cu_q[b] .., its keys and values rows
-   cu_k[b] .. (cu_q and cu_k may be one array). */
+   cu_k[b] .. (cu_q and cu_k may be one array).  o must not overlap an operand. */
 int ivh_attention(const ivh_attn_desc * d, const void * q, const void * k, const void * v, const int32_t * cu_q,
                   const int32_t * cu_k, void * o, int batch, int tokens_q, int tokens_k, void * stream);
 

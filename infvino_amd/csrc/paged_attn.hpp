@@ -13,14 +13,20 @@
 //   * O^T = V^T P^T wants of group g the values and probabilities of 8 tokens of one granule: the
 //     probabilities are in place, with no lane exchange, and 16 bytes of the stored values are
 //     16 (8-bit) or 8 tokens of one channel.
-// e4m3 codes become f16 or bf16 exactly; the key scale multiplies the scores, one factor a lane.  The
-// value scale goes into the exponent: with w = exp2(t + log2 vs - M), M the running maximum of t + log2 vs, the output is
-// sum w V / sum (w / vs), so no product of a code and its scale can leave the 16-bit range.
-// Probabilities are rounded to 16 bits for the second product (half a step relative, as the
-// output's own rounding); their sum is taken before that.
+// e4m3 codes become f16 or bf16 exactly; the key scale multiplies the scores, one factor a lane.
+// The value scale goes into the exponent: with w = exp2(t + log2 vs - M), M the running maximum of
+// t + log2 vs, the output is sum w V / sum (w / vs), so no product of a code and its scale can leave
+// the 16-bit range.  Weights are rounded to 16 bits for the second product (half a step relative, as
+// the output's own rounding); their sum is that of the rounded ones.
 //
-// Few rows: a work-group's four waves take every fourth step, and further work-groups further keys; the partial
-// sums are joined through LDS and by a second kernel.  Many rows: each wave takes rows of its own.
+// Few rows: a work-group's four waves take every fourth step, and further work-groups further keys;
+// the partial sums are joined through LDS and by a second kernel.  Many rows: each wave takes rows
+// of its own.
+//
+// Measured, 32 query heads on 8 key heads of 128 channels, 8-bit pages: 64 sequences of 8192 tokens
+// 191 us, 5.6 TB/s of cache (16-bit pages 6.1); 64 of 900 to 16001 210 us, 5.3 TB/s: HBM.  One of 5000
+// 12 us, of which the join is 4: the chain offsets, table, keys, values and a second launch.  5 new
+// tokens of 24 sequences in a window of 1024 16.6 us: the same chain and 5 steps a wave.
 #pragma once
 
 #include <algorithm>

@@ -5,8 +5,18 @@
 // (2f, 2f + 1) by the angle t = pos[axis(f)][token] * freq[f]:
 //   a' = a cos t - b sin t,   b' = b cos t + a sin t
 // in fp32, rounded once.  Both kernels move every channel once and do three multiply-adds on it,
-// so the memory bounds them; the angles (a 64-bit product and a sine each) are the one thing that
-// can cost more and are shared by a token's heads.
+// so the memory bounds them; the angles (a two-part product and some 30 operations each) are the one
+// thing that can cost more and are shared by a token's heads.
+//
+// Measured (a 1 GiB copy reaches 5.2 TB/s here): 32768 tokens of 40 heads of 128 channels, bf16,
+// three axes: 135 us, 5.0 TB/s.  6400 tokens of 32 heads of 80 channels cut from packed rows 14.9 us,
+// 4.4 TB/s.  One token: 4 us, launch and two trips to memory.
+//
+// The append gives a work-group a page (or the part of it that is new) of a run of heads, keys
+// and values apart: a page's scale needs the page's maximum, so the rows wait in registers while it
+// is found.  20033 tokens of 8 heads of 128 channels into an 8-bit cache: 37 us, 3.3 TB/s, held by the
+// chain of rows, maximum, codes with three work-groups a CU; the same in 16 bits, 7000 tokens of 4 heads
+// of 256 channels, 13 us.  A token each of 60 sequences: 5.6 us, the chain of offsets, table, rows.
 #include <algorithm>
 #include <stdexcept>
 
