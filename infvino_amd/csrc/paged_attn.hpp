@@ -114,21 +114,29 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
     int seen_lo[QT], seen_n[QT], seen_first[QT];
     // Q^T fragments in the order of the key pieces: 8-bit pieces hold 16 channels, two slices
     u4v qf[QT][NS];
+    auto query_ch = [&](int s) { return BITS == 8 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g; };
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-      const int row = row0 + 16 * t + r, tok = row / p.group, head = h * p.group + row - tok * p.group;
+      const int row = row0 + 16 * t + r, tok = row / p.group;
       const bool live = row < rows;
       const int place = place0 + tok, hi = live ? min(place, full - 1) : -1;
       seen_lo[t] = p.window ? place - p.window + 1 : 0;
       seen_n[t] = hi - seen_lo[t];
       seen_first[t] = p.window ? min(p.sinks, hi + 1) : 0;
-      const E * q = static_cast<const E *>(p.q) + (long)(c0 + tok) * p.q_token + (long)head * p.q_head;
+      // rows and channels that are not there read some that are: a branch would make each load wait
+      // for the one before
+      const int there = live ? row : 0, from = there / p.group;
+      const E * q = static_cast<const E *>(p.q) + (long)(c0 + from) * p.q_token + (long)(h * p.group + there - from * p.group) * p.q_head;
 #pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const int ch = BITS == 8 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g;
-        qf[t][s] = live && (FULL || ch < c.dim) ? *reinterpret_cast<const u4v *>(q + ch) ^ flip : u4v{0, 0, 0, 0};
-      }
+      for (int s = 0; s < NS; ++s) qf[t][s] = *reinterpret_cast<const u4v *>(q + (FULL || query_ch(s) < c.dim ? query_ch(s) : 0));
     }
+    auto settle_queries = [&]() __attribute__((always_inline)) {  // when they are there
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+          qf[t][s] = row0 + 16 * t + r < rows && (FULL || query_ch(s) < c.dim) ? qf[t][s] ^ flip : u4v{0, 0, 0, 0};
+    };
 
     f4v o[QT][NB];
     float M[QT], L[QT];
@@ -324,6 +332,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
       __builtin_amdgcn_sched_barrier(0);
       load_k(n, firstk);
       load_v(n, firstv);
+      settle_queries();
       for (; n + WK < n1; n += WK) {
         const int nk = idk, nv = idv;  // pages two steps ahead
         idk = page_of(min(n + 2 * WK, n1 - 1), r >> 2);

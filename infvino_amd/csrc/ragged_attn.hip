@@ -183,12 +183,14 @@ __global__ void __launch_bounds__(256, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) ragged_
     const int imin = qb * kRows + shift, imax = min(nq - 1, qb * kRows + kRows - 1) + shift;
     const int wmin = imin + 32 * wave, wmax = min(imax, wmin + 31);  // this wave's rows (none where wmax < wmin)
     const int row = qb * kRows + 32 * wave + col;
-    const E * q = static_cast<const E *>(p.q) + (long)(q0 + row) * p.q_token + (long)head * p.q_head;
+    // rows and channels that are not there read some that are, without a branch that would make each
+    // load wait for the one before
+    const E * q = static_cast<const E *>(p.q) + (long)(q0 + min(row, nq - 1)) * p.q_token + (long)head * p.q_head;
     u4v qf[NS];
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       const int ch = 16 * i + 8 * hi;
-      qf[i] = row < nq && ch < p.dim ? *reinterpret_cast<const u4v *>(q + ch) ^ flip : u4v{0, 0, 0, 0};
+      qf[i] = *reinterpret_cast<const u4v *>(q + (ch < p.dim ? ch : 0));
     }
 
     // steps: `first` over the first tokens, the others from step `from` on
@@ -363,6 +365,8 @@ __global__ void __launch_bounds__(256, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) ragged_
       __builtin_amdgcn_s_waitcnt(vm_wait(0));
       __syncthreads();
     }
+#pragma unroll
+    for (int i = 0; i < NS; ++i) qf[i] = row < nq && 16 * i + 8 * hi < p.dim ? qf[i] ^ flip : u4v{0, 0, 0, 0};
     if (wmax < wmin) {  // no rows: this wave's share of the copies, up to the same barriers as the others
       for (int n = 0; n < total; ++n) idle(n);
       if (__syncthreads_or(0))
