@@ -24,9 +24,9 @@
 // of its own.
 //
 // Measured, 32 query heads on 8 key heads of 128 channels, 8-bit pages: 64 sequences of 8192 tokens
-// 191 us, 5.6 TB/s of cache (16-bit pages 6.1); 64 of 900 to 16001 210 us, 5.3 TB/s: HBM.  One of 5000
+// 191 us, 5.6 TB/s of cache (16-bit pages 6.1); 64 of 900 to 16001 208 us, 5.3 TB/s: HBM.  One of 5000
 // 12 us, of which the join is 4: the chain offsets, table, keys, values and a second launch.  5 new
-// tokens of 24 sequences in a window of 1024 16.6 us: the same chain and 5 steps a wave.
+// tokens of 24 sequences in a window of 1024 16.1 us: the same chain and 5 steps a wave.
 #pragma once
 
 #include <algorithm>

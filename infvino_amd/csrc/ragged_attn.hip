@@ -28,10 +28,12 @@
 // ones, so a row's weights add up to 1.
 //
 // Measured (a bf16 product of 8192^3 reaches 1.23 PFLOP/s here): a prompt of 16384 tokens, 16 heads
-// of 128 channels on 4, causal: 1053 us, 1.07 PFLOP/s, bound by power (matrix cores half busy at 1.8
-// GHz).  Five prompts of up to 6007 in a window of 1024: 194 us, 0.72 PFLOP/s, the last of 4.2 rounds of work-groups
-// and masked steps at both ends of the window.  64 x 16 images of up to 400 tokens, 72 channels: 102
-// us, 0.47 PFLOP/s: channels padded to 80 and 96, 7 steps a work-group, the softmax's VALU work.
+// of 128 channels on 4, causal: 1000 us, 1.12 PFLOP/s.  The matrix cores are busy half the cycles and
+// the vector unit most of the others: work of one wave hides little of another's, with or without
+// copies, exponentials or LDS reads (each taken out alone changes 3 to 10 %), and zeros for data run
+// a fifth faster, which is power.  Five prompts of up to 6007 in a window of 1024: 189 us, 0.74 PFLOP/s, the
+// same and the last of 4.2 rounds of work-groups.  64 x 16 images of up to 400 tokens, 72 channels:
+// 100 us, 0.48 PFLOP/s: products on 80 and 96 channels, 7 steps a work-group behind 3 us of its start.
 #include <algorithm>
 #include <stdexcept>
 
@@ -115,7 +117,7 @@ struct RaggedMask {
 
 // NS: 16-channel slices of the head size, DP: that rounded up to a build's rows.
 template <int TYPE, int DP, int NS>
-__global__ void __launch_bounds__(256, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) ragged_attn_kernel(const RaggedParams p, int slots, int round)
+__global__ void __launch_bounds__(256, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) ragged_attn_kernel(const RaggedParams p, int slots, int side)
 {
   using T = St<TYPE>;
   typedef typename T::e E;
@@ -131,22 +133,33 @@ __global__ void __launch_bounds__(256, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) ragged_
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, hi = lane >> 5;
-  // The work-groups of a unit (sequence and key head) run on one XCD, whose L2 they share keys and values in.
-  // Units go round the XCDs where that is even, so that each gets its share of long and short
-  // sequences; a few units are cut into equal runs of work-groups instead.
+  // The work-groups of a unit (sequence and key head) run on one XCD, whose L2 they share keys and
+  // values in: a row block of each of its heads, then the next block of each, since those want the
+  // same keys at the same time (16384 tokens, 32 heads on 8, window 4096: 934 us, 968 head by head; 8 of 4096
+  // without a window 1130, 1162).  Units go round the XCDs where that is even, so that each gets its
+  // share of long and short sequences; few units are cut into `side` heads for each XCD, or else
+  // into equal runs of work-groups, head by head (block by block the first run would be the long ones).
   const int unit_wgs = p.group * slots, units = p.batch * (p.heads / p.group);
-  int w = blockIdx.x, unit;
-  if (round) {
+  int w = blockIdx.x, unit, slot, g;
+  if (side < 0) {
     unit = w / kXcds / unit_wgs * kXcds + w % kXcds;
     w = w / kXcds % unit_wgs;
     if (unit >= units) return;
+    slot = w / p.group;
+    g = w - slot * p.group;
+  } else if (side > 0) {
+    slot = w / kXcds / side;
+    g = w % kXcds * side + w / kXcds % side;
+    unit = g / p.group;
+    g -= unit * p.group;
   } else {
     w = xcd_tile(w, gridDim.x);
     unit = w / unit_wgs;
     w -= unit * unit_wgs;
+    g = w / slots;
+    slot = w - g * slots;
   }
-  const int kv_heads = p.heads / p.group, b = unit / kv_heads, kvh = unit - b * kv_heads;
-  const int slot = w % slots, head = kvh * p.group + w / slots;
+  const int kv_heads = p.heads / p.group, b = unit / kv_heads, kvh = unit - b * kv_heads, head = kvh * p.group + g;
 
   const int q0 = min(max(p.cu_q[b], 0), p.tokens_q), q1 = min(max(p.cu_q[b + 1], q0), p.tokens_q);
   const int k0 = min(max(p.cu_k[b], 0), p.tokens_k), k1 = min(max(p.cu_k[b + 1], k0), p.tokens_k);
@@ -465,9 +478,11 @@ template <int TYPE, int DP, int NS> void launch_ragged(const RaggedParams & p, h
   const long heads = (long)p.batch * p.heads;
   const int slots = (int)std::min<long>((std::max(1, std::min(p.max_q, p.tokens_q)) + kRows - 1) / kRows, (1L << 24) / (heads + kXcds * p.group));
   const long units = heads / p.group;
-  const int round = units % kXcds == 0 || units >= 4 * kXcds;
+  const bool round = units % kXcds == 0 || units >= 4 * kXcds;
+  const long share = heads / kXcds;  // heads of an XCD
+  const int side = round ? -1 : heads % kXcds == 0 && p.group % share == 0 ? (int)share : 0;
   const long wgs = (round ? (units + kXcds - 1) / kXcds * kXcds : units) * p.group * slots;
-  hipLaunchKernelGGL((ragged_attn_kernel<TYPE, DP, NS>), dim3((unsigned)wgs), dim3(256), 0, s, p, slots, round);
+  hipLaunchKernelGGL((ragged_attn_kernel<TYPE, DP, NS>), dim3((unsigned)wgs), dim3(256), 0, s, p, slots, side);
 }
 
 template <int TYPE> void launch_ragged_dim(const RaggedParams & p, hipStream_t s)

@@ -587,6 +587,11 @@ RAGGED = [  # heads, kv heads, dim, causal, window, sinks, lengths of queries, o
     (2, 1, 128, True, 200, 1, [700], None), (2, 1, 256, True, 33, 2, [257], None),
     (4, 2, 64, True, 0, 0, [5, 300, 64, 3, 0], [200, 64, 64, 0, 40]), (4, 2, 128, False, 0, 0, [5, 300, 7], [200, 64, 0]),
     (4, 2, 64, True, 40, 3, [5, 300, 64], [200, 64, 300]), (4, 2, 64, False, 40, 3, [5, 300, 64], [200, 64, 300]),
+    # heads dealt to the XCDs in each way: one, two and seven for each, units in turn, and runs of work-groups
+    (8, 1, 64, True, 0, 0, [300], None), (16, 4, 64, True, 0, 0, [700], None), (16, 2, 128, True, 90, 3, [300], [500]),
+    (28, 2, 64, True, 0, 0, [200, 0, 129, 31], None), (16, 4, 64, True, 0, 0, [300, 7, 0, 129], None),
+    (28, 4, 64, True, 0, 0, [300], None), (16, 4, 64, True, 0, 0, [300, 130, 5], None), (7, 1, 64, False, 0, 0, [129, 260], None),
+    (6, 3, 64, True, 0, 0, [140] * 13, None),
 ]
 
 
