@@ -851,3 +851,31 @@ def test_operands_that_are_not_on_the_device():
         ops.rope(d, _p(x), _p(pos), _p(freq), _p(y), 2, _stream())
     ops.rope(d, _p(y), _p(pos), _p(freq), _p(y), 2, _stream())
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (20, 3)])
+def test_paged_attention_lengths_that_do_not_fit(bits, window, sinks):
+    """Lengths below the number of new rows, of nothing, below 0 and behind the table's end; first rows
+    that lie behind the rows there are: rows whose place is before the first key are zero."""
+    g = _gen(8)
+    page, width = 16, 4
+    cache = Cache("bf16", bits, 2, 64, page, 20, width)
+    new, lens = [4, 3, 2, 0, 1, 5], [2, 0, -5, 7, 1000, 64]
+    stored = [min(max(n, 0), page * width) for n in lens]
+    table = _tables(g, [-(-n // page) for n in stored], width, 20)
+    _fill(cache, g, table, stored)
+    rows = sum(new)
+    q = _randn(g, cache.dt, rows, 8, 64)
+    cu = _ends(new)
+    cu[-1] += 1000
+    for hints in ({}, {"max_new": 5, "max_len": 64}):
+        o, _ = _run_paged(cache, q, cu, _i32(lens), _i32(table), 8, len(new), window, sinks, **hints)
+        row = 0
+        for b, (n, m, kept) in enumerate(zip(new, lens, stored)):
+            k, v = cache.rows(table[b], kept)
+            place = torch.arange(n, device="cuda") + max(m, 0) - n
+            r, av, err = _attend(q[row:row + n], k, v, place, True, window, sinks, 0.125)
+            _close(o[row:row + n], r, av, err, cache.u, kept, v.abs().max() if kept else 0)
+            row += n
+        assert (o[:2] == 0).all() and (o[4:9] == 0).all()
