@@ -28,7 +28,7 @@
 // ones, so a row's weights add up to 1.
 //
 // Measured (a bf16 product of 8192^3 reaches 1.23 PFLOP/s here): a prompt of 16384 tokens, 16 heads
-// of 128 channels on 4, causal: 1000 us, 1.12 PFLOP/s.  The matrix cores are busy half the cycles and
+// of 128 channels on 4, causal: 1000 to 1080 us by card, 1.12 to 1.04 PFLOP/s.  The matrix cores are busy half the cycles and
 // the vector unit most of the others: work of one wave hides little of another's, with or without
 // copies, exponentials or LDS reads (each taken out alone changes 3 to 10 %), and zeros for data run
 // a fifth faster, which is power.  Five prompts of up to 6007 in a window of 1024: 189 us, 0.74 PFLOP/s, the
