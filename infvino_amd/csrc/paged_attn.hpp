@@ -16,8 +16,10 @@
 // e4m3 codes become f16 or bf16 exactly; the key scale multiplies the scores, one factor a lane.
 // The value scale goes into the exponent: with w = exp2(t + log2 vs - M), M the running maximum of
 // t + log2 vs, the output is sum w V / sum (w / vs), so no product of a code and its scale can leave
-// the 16-bit range.  Weights are rounded to 16 bits for the second product (half a step relative, as
-// the output's own rounding); their sum is that of the rounded ones.
+// the 16-bit range.  Weights are rounded to 16 bits for the second product.  A page's keys count in the
+// sum however small its values are (zeros have the scale 2^-32): the sum is of the weights before
+// their rounding where fp16 would lose them, and where the scales are so far apart that fp32 would, of
+// exp2(t - M).  Elsewhere (bf16, 16-bit pages) it is that of the rounded ones.
 //
 // Few rows: a work-group's four waves take every fourth step, and further work-groups further keys;
 // the partial sums are joined through LDS and by a second kernel.  Many rows: each wave takes rows
@@ -214,7 +216,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
       if (!inner && !(ok && key0 + 16 * g < full)) ks = vs = 1.0f;  // a granule without tokens: its scales may be anything
       const float mul = scale * ks, ev = BITS == 8 ? __builtin_amdgcn_logf(vs) : 0.0f;
       const float unv = BITS == 8 ? __builtin_amdgcn_rcpf(vs) : 1.0f;
-      float top[QT];
+      float top[QT], most[QT];  // largest exponents of the rows, and of this lane's granule
       bool grow = false;
 #pragma unroll
       for (int u = 0; u < QT; ++u) {
@@ -234,7 +236,8 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
           if (x + 2 < 16) d = top_of(d, s[u][(x + 2) / 4][(x + 2) % 4], s[u][(x + 2) / 4][(x + 2) % 4 + 1]);
         }
         // the page's scales are the lane group's: they enter before the groups are compared
-        top[u] = across16(across32(fmaf(top_of(a, d, d), mul, ev), MaxOp()), MaxOp());
+        most[u] = fmaf(top_of(a, d, d), mul, ev);
+        top[u] = across16(across32(most[u], MaxOp()), MaxOp());
         grow = grow || top[u] > M[u] + 8.0f;
       }
       // the reference exponent follows the maximum only when that is 2^8 above it: weights up to
@@ -254,15 +257,28 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
 #pragma unroll
       for (int u = 0; u < QT; ++u) {
         const float shift = ev - M[u];
-        float sum = 0.0f;
+        float sum = 0.0f, sum2 = 0.0f;
 #pragma unroll
         for (int x = 0; x < 16; x += 2) {
           const f4v & y = s[u][x / 4];
-          const unsigned e = pack2<TYPE>(__builtin_amdgcn_exp2f(fmaf(y[x % 4], mul, shift)), __builtin_amdgcn_exp2f(fmaf(y[x % 4 + 1], mul, shift)));
-          sum = T::add2(e, sum);  // of the rounded weights, which are what the values get
+          const float e0 = __builtin_amdgcn_exp2f(fmaf(y[x % 4], mul, shift)), e1 = __builtin_amdgcn_exp2f(fmaf(y[x % 4 + 1], mul, shift));
+          const unsigned e = pack2<TYPE>(e0, e1);
           pf[u][x / 8][x % 8 / 2] = e;
+          if (BITS == 8 && TYPE == kSeqF16) {  // rounded to fp16, those of a page of small values are gone
+            sum += e0;
+            sum2 += e1;
+          } else {
+            sum = T::add2(e, sum);
+          }
         }
-        L[u] = fmaf(sum, unv, L[u]);
+        sum = (sum + sum2) * unv;
+        // so far below M that even the fp32 weights may be gone: summed without the value scale
+        if (BITS == 8 && __any(most[u] < M[u] - 100.0f && most[u] > -__builtin_inff())) {
+          sum = 0.0f;
+#pragma unroll
+          for (int x = 0; x < 16; ++x) sum += __builtin_amdgcn_exp2f(fmaf(s[u][x / 4][x % 4], mul, -M[u]));
+        }
+        L[u] += sum;
       }
     };
     // values that no row sees (behind the last key, outside every window, in no page) may be

@@ -879,3 +879,65 @@ def test_paged_attention_lengths_that_do_not_fit(bits, window, sinks):
             _close(o[row:row + n], r, av, err, cache.u, kept, v.abs().max() if kept else 0)
             row += n
         assert (o[:2] == 0).all() and (o[4:9] == 0).all()
+
+
+# ------------------------------------------------------------------ value scales far apart
+def _fill_apart(cache, gen, table, lens, apart):
+    """Pages whose value scales differ: page i of a sequence has values of zero (None), or 2^-apart[i] of
+    ordinary ones; `apart` is repeated."""
+    rows = sum(lens)
+    k, v = (_randn(gen, cache.dt, rows, cache.heads, cache.dim) for _ in range(2))
+    place = torch.cat([torch.arange(n, device="cuda") for n in lens])
+    zero = torch.tensor([a is None for a in apart], device="cuda")[place // cache.page % len(apart)]
+    v[zero] = 0
+    cache.append(k, v, None, None, _ends(lens), _i32(lens), _i32(table), len(lens))
+    vs = cache.vs.view(cache.pages, cache.heads)
+    for ids in table:
+        for i, at in enumerate(ids):
+            if at >= 0 and apart[i % len(apart)]:
+                vs[at] *= 2.0 ** -apart[i % len(apart)]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("heads,kv,dim,page", [(8, 2, 128, 16), (4, 1, 64, 32), (3, 3, 80, 16), (4, 2, 256, 64)])
+@pytest.mark.parametrize("apart", [[0, None], [None] * 7 + [0], [0] + [None] * 7, [0, 12], [16, 0], [0, 20, 0, 24, None], [25, 0, 10]])
+def test_paged_attention_value_scales_apart(t, heads, kv, dim, page, apart):
+    """Keys of a page count with their weight however small the page's values are: pages of zeros before, between
+    and behind ordinary ones, in a step, across steps and across parts; one new token and several.
+
+    A small weight of fp16 is off by 2^-25 of the largest, in units of its page's codes: 448 times the scale
+    at most, which is twice the page's largest value."""
+    g = _gen(50 + dim)
+    new, lens = [1, 3, 1, 1], [5 * page - 3, 130, 2, 300 * page - 7]
+    used = [-(-n // page) for n in lens]
+    table = _tables(g, used, max(used), sum(used))
+    cache = Cache(t, 8, kv, dim, page, sum(used), max(used))
+    _fill_apart(cache, g, table, lens, apart)
+    q = _randn(g, cache.dt, sum(new), heads, dim, scale=0.5)
+    q[0] = 0  # every key has the same weight
+    for hints in ({"max_new": 3, "max_len": max(lens)}, {"max_new": 3, "max_len": 1}, {}):
+        o, _ = _run_paged(cache, q, _ends(new), _i32(lens), _i32(table), heads, 4, **hints)
+        row = 0
+        for b, (n, m) in enumerate(zip(new, lens)):
+            k, v = cache.rows(table[b], m)
+            r, av, err = _attend(q[row:row + n], k, v, torch.arange(m - n, m, device="cuda"), True, 0, 0, 1 / math.sqrt(dim))
+            _close(o[row:row + n], r, av, err, cache.u, m, 2 * v.abs().max())
+            row += n
+
+
+def test_paged_attention_value_scales_past_fp32():
+    """bf16 values of 2^100 and more beside zeros: the pages' scales are further apart than the exponents
+    of fp32 reach, and the zeros' keys count all the same."""
+    g = _gen(60)
+    lens, page = [133, 4000], 16
+    used = [-(-n // page) for n in lens]
+    table = _tables(g, used, max(used), sum(used))
+    cache = Cache("bf16", 8, 2, 64, page, sum(used), max(used))
+    _fill_apart(cache, g, table, lens, [-118, None, None, 0])
+    q = _randn(g, cache.dt, 4, 4, 64, scale=0.5)
+    for hints in ({"max_new": 2, "max_len": 4000}, {"max_new": 2, "max_len": 1}):
+        o, _ = _run_paged(cache, q, _ends([2, 2]), _i32(lens), _i32(table), 4, 2, **hints)
+        for b, m in enumerate(lens):
+            k, v = cache.rows(table[b], m)
+            r, av, err = _attend(q[2 * b:2 * b + 2], k, v, torch.arange(m - 2, m, device="cuda"), True, 0, 0, 0.125)
+            _close(o[2 * b:2 * b + 2], r, av, err, cache.u, m, 2 * v.abs().max())
