@@ -214,7 +214,8 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
     // masks, running maximum, weights in 16 bits
     auto weights = [&](int key0, bool inner, bool ok, float ks, float vs, f4v (&s)[QT][4], u4v (&pf)[QT][2]) __attribute__((always_inline)) {
       if (!inner && !(ok && key0 + 16 * g < full)) ks = vs = 1.0f;  // a granule without tokens: its scales may be anything
-      const float mul = scale * ks, ev = BITS == 8 ? __builtin_amdgcn_logf(vs) : 0.0f;
+      // a product of small scales is not 0 either
+      const float mul = BITS == 8 ? fmaxf(scale * ks, 1.2e-38f) : scale, ev = BITS == 8 ? __builtin_amdgcn_logf(vs) : 0.0f;
       const float unv = BITS == 8 ? __builtin_amdgcn_rcpf(vs) : 1.0f;
       float top[QT], most[QT];  // largest exponents of the rows, and of this lane's granule
       bool grow = false;

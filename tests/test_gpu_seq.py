@@ -941,3 +941,24 @@ def test_paged_attention_value_scales_past_fp32():
             k, v = cache.rows(table[b], m)
             r, av, err = _attend(q[2 * b:2 * b + 2], k, v, torch.arange(m - 2, m, device="cuda"), True, 0, 0, 0.125)
             _close(o[2 * b:2 * b + 2], r, av, err, cache.u, m, 2 * v.abs().max())
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("scale", [0.0, 1e-35, -1e-30, -0.25])
+def test_paged_attention_small_and_negative_scales(t, bits, scale):
+    """A softmax scale of zero or nearly: the plain average of the values, over keys of zero too (whose pages
+    have a scale of 2^-32), with a last page that is not full and a window that ends inside pages."""
+    g = _gen(61)
+    lens, new, page = [37, 150, 16], [1, 4, 2], 16
+    used = [-(-n // page) for n in lens]
+    table = _tables(g, used, 10, sum(used))
+    cache = Cache(t, bits, 2, 64, page, sum(used), 10)
+    rows = sum(lens)
+    k, v = _randn(g, cache.dt, rows, 2, 64), _randn(g, cache.dt, rows, 2, 64)
+    k[30:37], k[37 + 144:] = 0, 0
+    cache.append(k, v, None, None, _ends(lens), _i32(lens), _i32(table), 3)
+    q = _randn(g, cache.dt, sum(new) + 1, 4, 64)
+    for window, sinks in ((0, 0), (21, 3)):
+        o, _ = _run_paged(cache, q, _ends(new), _i32(lens), _i32(table), 4, 3, window, sinks, scale=scale)
+        _check_paged(cache, q, o, new, lens, table, window, sinks, scale)
