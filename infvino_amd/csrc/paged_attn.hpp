@@ -18,8 +18,7 @@
 // t + log2 vs, the output is sum w V / sum (w / vs), so no product of a code and its scale can leave
 // the 16-bit range.  Weights are rounded to 16 bits for the second product.  A page's keys count in the
 // sum however small its values are (zeros have the scale 2^-32): the sum is of the weights before
-// their rounding where fp16 would lose them, and where the scales are so far apart that fp32 would, of
-// exp2(t - M).  Elsewhere (bf16, 16-bit pages) it is that of the rounded ones.
+// their rounding where fp16 would lose them, else of the rounded ones.
 //
 // Few rows: a work-group's four waves take every fourth step, and further work-groups further keys;
 // the partial sums are joined through LDS and by a second kernel.  Many rows: each wave takes rows
@@ -73,6 +72,9 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
   constexpr int NB = DP / 16;                   // channel blocks
   constexpr int NS = DP / 32;                   // 32-channel slices
   constexpr int ROWS = 16 * QT * (4 / WK);      // rows of a work-group
+  // weights and the sums of values hold a power of two more, so that small ones stay above fp32's lowest
+  // exponent where pages' scales are 2^120 for bf16's largest values and 2^-32 for zeros
+  constexpr int UP = TYPE == kSeqBF16 && BITS == 8 ? 64 : 0;
   extern __shared__ __attribute__((aligned(16))) float lds[];
 
   const CacheParams & c = p.c;
@@ -216,8 +218,10 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
       if (!inner && !(ok && key0 + 16 * g < full)) ks = vs = 1.0f;  // a granule without tokens: its scales may be anything
       // a product of small scales is not 0 either
       const float mul = BITS == 8 ? fmaxf(scale * ks, 1.2e-38f) : scale, ev = BITS == 8 ? __builtin_amdgcn_logf(vs) : 0.0f;
-      const float unv = BITS == 8 ? __builtin_amdgcn_rcpf(vs) : 1.0f;
-      float top[QT], most[QT];  // largest exponents of the rows, and of this lane's granule
+      // 2^-UP / vs, whose exponent may not fit
+      const float unv = __builtin_amdgcn_rcpf(__builtin_amdgcn_frexp_mantf(vs));
+      const int unv_exp = -UP - __builtin_amdgcn_frexp_expf(vs);
+      float top[QT];
       bool grow = false;
 #pragma unroll
       for (int u = 0; u < QT; ++u) {
@@ -237,8 +241,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
           if (x + 2 < 16) d = top_of(d, s[u][(x + 2) / 4][(x + 2) % 4], s[u][(x + 2) / 4][(x + 2) % 4 + 1]);
         }
         // the page's scales are the lane group's: they enter before the groups are compared
-        most[u] = fmaf(top_of(a, d, d), mul, ev);
-        top[u] = across16(across32(most[u], MaxOp()), MaxOp());
+        top[u] = across16(across32(fmaf(top_of(a, d, d), mul, ev), MaxOp()), MaxOp());
         grow = grow || top[u] > M[u] + 8.0f;
       }
       // the reference exponent follows the maximum only when that is 2^8 above it: weights up to
@@ -257,7 +260,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
       }
 #pragma unroll
       for (int u = 0; u < QT; ++u) {
-        const float shift = ev - M[u];
+        const float shift = ev + UP - M[u];
         float sum = 0.0f, sum2 = 0.0f;
 #pragma unroll
         for (int x = 0; x < 16; x += 2) {
@@ -265,21 +268,16 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
           const float e0 = __builtin_amdgcn_exp2f(fmaf(y[x % 4], mul, shift)), e1 = __builtin_amdgcn_exp2f(fmaf(y[x % 4 + 1], mul, shift));
           const unsigned e = pack2<TYPE>(e0, e1);
           pf[u][x / 8][x % 8 / 2] = e;
-          if (BITS == 8 && TYPE == kSeqF16) {  // rounded to fp16, those of a page of small values are gone
+          if (TYPE == kSeqF16 && BITS == 8) {  // rounded to fp16, those of a page of small values are gone
             sum += e0;
             sum2 += e1;
           } else {
             sum = T::add2(e, sum);
           }
         }
-        sum = (sum + sum2) * unv;
-        // so far below M that even the fp32 weights may be gone: summed without the value scale
-        if (BITS == 8 && __any(most[u] < M[u] - 100.0f && most[u] > -__builtin_inff())) {
-          sum = 0.0f;
-#pragma unroll
-          for (int x = 0; x < 16; ++x) sum += __builtin_amdgcn_exp2f(fmaf(s[u][x / 4][x % 4], mul, -M[u]));
-        }
-        L[u] += sum;
+        if (TYPE == kSeqF16 && BITS == 8) sum += sum2;
+        if (BITS == 8) L[u] += __builtin_ldexpf(sum * unv, unv_exp);
+        else L[u] += sum;
       }
     };
     // values that no row sees (behind the last key, outside every window, in no page) may be
@@ -455,6 +453,9 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
       for (int u = 0; u < QT; ++u) {
         const int at_row = row0 + 16 * u + r, tok = at_row / p.group, head = h * p.group + at_row - tok * p.group;
         if (at_row >= rows) continue;
+        if (UP)
+#pragma unroll
+          for (int j = 0; j < NB; ++j) o[u][j] *= __builtin_ldexpf(1.0f, -UP);
         const long row = (long)(c0 + tok) * p.heads + head;
         if (p.parts == 1) {
           const float inv = L[u] != 0.0f ? 1.0f / L[u] : 0.0f;  // a row that saw nothing is zero (NaN stays)
