@@ -72,9 +72,10 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
   constexpr int NB = DP / 16;                   // channel blocks
   constexpr int NS = DP / 32;                   // 32-channel slices
   constexpr int ROWS = 16 * QT * (4 / WK);      // rows of a work-group
-  // weights and the sums of values hold a power of two more, so that small ones stay above fp32's lowest
-  // exponent where pages' scales are 2^120 for bf16's largest values and 2^-32 for zeros
-  constexpr int UP = TYPE == kSeqBF16 && BITS == 8 ? 64 : 0;
+  // weights and the sums of values hold a power of two more: in fp16 those of 2^-21 of the largest are normal
+  // numbers then and the largest is below 2^15; in bf16 small ones stay above fp32's lowest exponent
+  // where pages' scales are 2^120 for the type's largest values and 2^-32 for zeros
+  constexpr int UP = TYPE == kSeqF16 ? 7 : BITS == 8 ? 64 : 0;
   extern __shared__ __attribute__((aligned(16))) float lds[];
 
   const CacheParams & c = p.c;
@@ -244,8 +245,8 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
         top[u] = across16(across32(fmaf(top_of(a, d, d), mul, ev), MaxOp()), MaxOp());
         grow = grow || top[u] > M[u] + 8.0f;
       }
-      // the reference exponent follows the maximum only when that is 2^8 above it: weights up to
-      // 2^8 lose nothing in either 16-bit type
+      // the reference exponent follows the maximum only when that is 2^8 above it: weights that are
+      // larger by that lose nothing in either 16-bit type
       if (__any(grow)) {
 #pragma unroll
         for (int u = 0; u < QT; ++u) {
@@ -277,7 +278,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
         }
         if (TYPE == kSeqF16 && BITS == 8) sum += sum2;
         if (BITS == 8) L[u] += __builtin_ldexpf(sum * unv, unv_exp);
-        else L[u] += sum;
+        else L[u] = fmaf(sum, __builtin_ldexpf(1.0f, -UP), L[u]);
       }
     };
     // values that no row sees (behind the last key, outside every window, in no page) may be

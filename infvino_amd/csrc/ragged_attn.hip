@@ -19,7 +19,8 @@
 //     this one's second product, the exponentials beside the former; fragments are read from LDS
 //     four slots before their use, so that the matrix cores do not wait for them;
 //   * the running maximum moves only when a score exceeds it by 8 (in powers of two): until then
-//     exp2(score - M) stays below 2^8, and the accumulators need no rescaling;
+//     the accumulators need no rescaling.  fp16 weights hold 2^7 more, so that thousands of small ones
+//     are not lost: those below 2^-21 of the largest are off by 2^-32 of it at most;
 //   * a second, careful pass over the keys runs for rows whose result is not finite: there 0 times an
 //     infinity or NaN of a key that the row does not see may be the reason.
 // LDS rows are not padded (DMA writes 64 x 16 bytes in a row); 16-byte pieces are permuted within
@@ -126,6 +127,7 @@ __global__ void __launch_bounds__(256, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) ragged_
   constexpr int VI = kKeys * PR / 256; // copies of a wave: values of a step,
   constexpr int KC = 32 * PR / 64, KI = (KC + 3) / 4;  // keys of a block (KC in all)
   constexpr int STAGE = kKeys * DP, BLOCK = 32 * DP;
+  constexpr int UP = TYPE == kSeqF16 ? 7 : 0;  // weights of 2^-21 of the largest are normal fp16 numbers, the largest is below 2^15
   // keys: a ring of four 32-key blocks; values: two stages of 64.  Arrays of their own, so that the
   // compiler sees that a copy into one does not touch the others and leaves it in flight.
   __shared__ __attribute__((aligned(16))) unsigned char K0[BLOCK * 2], K1[BLOCK * 2], K2[BLOCK * 2], K3[BLOCK * 2];
@@ -274,8 +276,9 @@ __global__ void __launch_bounds__(256, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) ragged_
 #pragma unroll
       for (int i = 0; i < NS; ++i) s = T::mma32(key_piece_of(sl, i), qf[i], i ? s : f16v{});
     };
-    // scores of keys (from key0 on) that a row does not see become -inf; the reference exponent follows the
-    // running maximum only when that is 2^8 above it: weights up to 2^8 lose nothing in either 16-bit type
+    // scores of keys (from key0 on) that a row does not see become -inf; the reference exponent lies UP
+    // below a maximum and follows it only when that is 2^8 above: weights that are larger by that lose nothing
+    // in either 16-bit type
     auto settle = [&](int key0, bool inner, f16v & s) __attribute__((always_inline)) {
       if (!inner) {
 #pragma unroll
@@ -292,8 +295,8 @@ __global__ void __launch_bounds__(256, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) ragged_
         if (v + 2 < 16) b = top_of(b, s[v + 2], s[v + 3]);
       }
       const float top = across32(top_of(a, b, b), MaxOp()) * scale;
-      if (__any(top > M + 8.0f)) {
-        const float m = fmaxf(M, top), e = __builtin_amdgcn_exp2f(M - m);
+      if (__any(top > M + (8.0f + UP))) {
+        const float m = fmaxf(M, top - UP), e = __builtin_amdgcn_exp2f(M - m);
         M = m;
         L *= e;
 #pragma unroll

@@ -962,3 +962,52 @@ def test_paged_attention_small_and_negative_scales(t, bits, scale):
     for window, sinks in ((0, 0), (21, 3)):
         o, _ = _run_paged(cache, q, _ends(new), _i32(lens), _i32(table), 4, 3, window, sinks, scale=scale)
         _check_paged(cache, q, o, new, lens, table, window, sinks, scale)
+
+
+# ------------------------------------------------------------------ many small weights
+def _few_and_many(gen, dt, n, kv, dim, low):
+    """Queries, keys and values of which one key per head has a weight 2^low times the others', which vary by
+    2^0.5 and less, and values of zero."""
+    q = torch.zeros((1, kv, dim), device="cuda")
+    q[..., 0], q[..., 1] = 1, 1
+    k, v = torch.zeros((n, kv, dim), device="cuda"), _randn(gen, dt, n, kv, dim).abs() + 1
+    k[:, :, 1] = torch.rand((n, kv), generator=gen, device="cuda") * 0.5
+    k[n // 3, :, 0], k[n // 3, :, 1], v[n // 3] = low, 0, 0
+    return q.to(dt), k.to(dt), v.to(dt)
+
+
+def _small_weights_close(o, q, k, v, n, u):
+    """fp16 weights from 2^-21 of the largest on are rounded by u of themselves, those below by 2^-32 of
+    the largest; over 8-bit pages in units of the codes, 448 times the scale at most, which is twice the
+    page's largest value."""
+    r, av, err = _attend(q, k, v, torch.tensor([n - 1], device="cuda"), True, 0, 0, math.log(2))
+    tol = u * r.abs() + u * av + 2 * (err + 2.0 ** -15) * av + n * 2.0 ** -31 * v.double().abs().max() + 2.0 ** -25
+    assert ((o.double() - r).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("low", [14, 20, 25])
+@pytest.mark.parametrize("n", [60, 16000])
+def test_attention_many_small_weights(t, low, n):
+    """Thousands of keys whose weights lie at and below fp16's lowest normal value, relative to one other's: what
+    they add up to reaches the row."""
+    code, dt, u = TYPES[t]
+    q, k, v = _few_and_many(_gen(70), dt, n, 2, 64, low)
+    o = torch.empty_like(q)
+    cq, ck = _ends([1]), _ends([n])
+    ops.attention(ops.attention_desc(code, 2, 2, 64, math.log(2)), _p(q), _p(k), _p(v), _p(cq), _p(ck), _p(o), 1, 1, n, _stream())
+    _small_weights_close(o, q, k, v, n, u)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("low", [14, 20, 25])
+@pytest.mark.parametrize("n", [60, 16000])
+def test_paged_attention_many_small_weights(t, bits, low, n):
+    cache = Cache(t, bits, 2, 64, 32, -(-n // 32), -(-n // 32))
+    q, k, v = _few_and_many(_gen(71), cache.dt, n, 2, 64, low)
+    table = [list(range(-(-n // 32)))]
+    cache.append(k, v, None, None, _ends([n]), _i32([n]), _i32(table), 1)
+    for hints in ({"max_new": 1, "max_len": n}, {"max_new": 1, "max_len": 1}):
+        o, _ = _run_paged(cache, q, _ends([1]), _i32([n]), _i32(table), 2, 1, scale=math.log(2), **hints)
+        _small_weights_close(o, q, *cache.rows(table[0], n), n, cache.u)
