@@ -38,8 +38,10 @@ size_t paged_split(PagedParams & p, int max_new, int max_len)
     want = steps <= 24 * waves * one ? one : (512 + wgs - 1) / wgs;
   }
   const long top = std::max<long>(1, (steps + waves - 1) / waves);
-  // a launch holds 2^24 work-groups of 256 lanes
+  // a launch holds fewer than 2^24 work-groups of 256 lanes
   p.parts = (int)std::min<long>({std::max<long>(want, 1), top, 256, std::max<long>(1, (1L << 23) / wgs)});
+  // the join has up to a work-group for each row, of which a launch holds as many: more rows fill the chip
+  if ((long)c.tokens * p.heads >= 1L << 24) p.parts = 1;
   p.part_steps = (int)((((steps + p.parts - 1) / p.parts) + waves - 1) / waves * waves);
   p.parts = (int)std::max<long>(1, (steps + p.part_steps - 1) / p.part_steps);
   if (p.parts == 1) return 0;

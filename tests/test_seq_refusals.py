@@ -174,3 +174,18 @@ def test_workspace_follows_the_split():
     assert ops.paged_attention_workspace(ops.paged_attention_desc(c, 4, 0.1, max_new=1, max_len=2000), 2000, 2000) == 0
     # a window bounds what a row reads
     assert ops.paged_attention_workspace(ops.paged_attention_desc(c, 4, 0.1, window=64, max_new=1, max_len=60000), 1, 1) == 0
+
+
+def test_workspace_of_more_rows_than_a_join_holds():
+    """The join of partial sums has a work-group for each row at most, of which a launch holds fewer than
+    2^24: calls of more rows are not split."""
+    def need(rows, heads, dim):
+        c = _cache(heads=1, dim=dim, page=128, table_width=512, pages=1)
+        d = ops.paged_attention_desc(c, heads, 0.1, max_new=1, max_len=60000)
+        return ops.paged_attention_workspace(d, 1 << 10, rows // heads)
+
+    for dim in (16, 176, 256):
+        for heads in (1, 8):
+            assert need((1 << 24) - 8, heads, dim) > 0
+            assert need(1 << 24, heads, dim) == 0
+            assert need(1 << 26, heads, dim) == 0
