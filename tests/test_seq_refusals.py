@@ -2,6 +2,10 @@
 before anything is enqueued, and what an empty call does.  No device is needed: every check here comes
 before the first HIP call."""
 import ctypes as C
+import os
+import re
+import shutil
+import subprocess
 
 import pytest
 
@@ -189,3 +193,37 @@ def test_workspace_of_more_rows_than_a_join_holds():
             assert need((1 << 24) - 8, heads, dim) > 0
             assert need(1 << 24, heads, dim) == 0
             assert need(1 << 26, heads, dim) == 0
+
+
+@pytest.mark.skipif(shutil.which("gcc") is None, reason="no C compiler")
+def test_structs_have_the_layout_of_the_header(tmp_path):
+    """Size of each descriptor, and place and size of each of its fields, as a C compiler has them from
+    include/ivh.h."""
+    mirrors = {"ivh_conv_desc": ia.ConvDesc, "ivh_rotation": ia.Rotation, "ivh_rope_desc": ia.RopeDesc, "ivh_cache_desc": ia.CacheDesc,
+               "ivh_append_desc": ia.AppendDesc, "ivh_paged_attn_desc": ia.PagedAttentionDesc, "ivh_attn_desc": ia.AttentionDesc}
+    lines, want = [], []
+    for name, mirror in mirrors.items():
+        lines.append(f'printf("%zu\\n", sizeof({name}));')
+        want.append([C.sizeof(mirror)])
+        for field in mirror._fields_:
+            at, kind = getattr(mirror, field[0]), field[1]
+            # a float or an integer: halves of 1 differ in whether anything is left
+            lines.append(f'{{ {name} d; printf("%zu %zu", offsetof({name}, {field[0]}), sizeof d.{field[0]});')
+            want.append([at.offset, at.size])
+            if kind in (C.c_int, C.c_int64, C.c_float):
+                lines.append(f'd.{field[0]} = 1; d.{field[0]} /= 2; printf(" %d", d.{field[0]} != 0);')
+                want[-1].append(int(kind is C.c_float))
+            lines.append('printf("\\n"); }')
+    source = tmp_path / "layout.c"
+    source.write_text("#include <stddef.h>\n#include <stdio.h>\n#include <ivh.h>\nint main(void)\n{\n" + "\n".join(lines) + "\nreturn 0;\n}\n")
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    subprocess.run(["gcc", "-std=c11", "-Wall", "-I", include, str(source), "-o", str(tmp_path / "layout")], check=True)
+    out = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout
+    got = [[int(x) for x in line.split()] for line in out.splitlines()]
+    assert got == want
+    # and no field that is not in the mirror
+    text = re.sub(r"/\*.*?\*/", "", open(os.path.join(include, "ivh.h")).read(), flags=re.S)
+    for name, mirror in mirrors.items():
+        body = text[text.index(f"typedef struct {name} {{"):text.index(f"}} {name};")]
+        fields = [re.search(r"(\w+)(\[\d+\])?$", x.strip()).group(1) for line in body.split("{")[1].split(";")[:-1] for x in line.split(",")]
+        assert fields == [x[0] for x in mirror._fields_]
