@@ -48,9 +48,9 @@ struct Steps {
 __device__ __forceinline__ Steps key_steps(int full, int imin, int imax, int window, int sinks)
 {
   const int end = imax >= full ? full : imax + 1;
-  const int lo = window ? max(0, imin - window + 1) : 0;
+  const int lo = window ? (int)min(max((long)imin - window + 1, 0L), (long)max(end, 0)) : 0;
   Steps s;
-  s.from = min(lo, end) / 64;
+  s.from = lo / 64;
   s.first = min((min(sinks, lo) + 63) / 64, s.from);
   s.total = end > 0 ? s.first + (end + 63) / 64 - s.from : 0;
   return s;
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
       const int row = row0 + 16 * t + r, tok = row / p.group;
       const bool live = row < rows;
       const int place = place0 + tok, hi = live ? min(place, full - 1) : -1;
-      seen_lo[t] = p.window ? place - p.window + 1 : 0;
+      seen_lo[t] = p.window ? (int)max((long)place - p.window + 1, 0L) : 0;
       seen_n[t] = hi - seen_lo[t];
       seen_first[t] = p.window ? min(p.sinks, hi + 1) : 0;
       // rows and channels that are not there read some that are: a branch would make each load wait

@@ -97,7 +97,7 @@ ivh::RotParams rotation(const ivh_rotation & r, int dim, const int32_t * pos, in
 }
 
 constexpr int kMaxTokens = 1 << 26, kMaxBatch = 1 << 20, kMaxHeads = 1 << 22;  // the last: sequences times heads
-// a larger window hides nothing either; with it a place less the window stays within 32 bits
+// of contiguous rows: a larger window hides nothing either; with it a place less the window stays within 32 bits
 constexpr int kMaxWindow = INT32_MAX - 2 * kMaxTokens;
 
 void check_counts(int batch, int tokens)
@@ -161,7 +161,7 @@ ivh::PagedParams paged(const ivh_paged_attn_desc * d, int batch, int tokens, siz
   p.heads = d->heads;
   p.group = d->heads / d->cache.heads;
   p.scale_log2 = d->scale * kLog2E;
-  p.window = std::min(d->window, kMaxWindow);
+  p.window = d->window;
   p.sinks = d->sinks;
   const int max_new = d->max_new ? d->max_new : tokens;
   const int max_len = d->max_len ? d->max_len : d->cache.table_width * d->cache.page;

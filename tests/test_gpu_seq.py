@@ -1011,3 +1011,20 @@ def test_paged_attention_many_small_weights(t, bits, low, n):
     for hints in ({"max_new": 1, "max_len": n}, {"max_new": 1, "max_len": 1}):
         o, _ = _run_paged(cache, q, _ends([1]), _i32([n]), _i32(table), 2, 1, scale=math.log(2), **hints)
         _small_weights_close(o, q, *cache.rows(table[0], n), n, cache.u)
+
+
+def test_paged_attention_lengths_near_the_largest():
+    """Lengths of up to 2^31 - 1 over a table of a few pages: rows stand far behind the last key and see the
+    first tokens alone, or with no window all there are."""
+    g = _gen(9)
+    cache = Cache("f16", 8, 2, 64, 16, 8, 8)
+    table = [list(range(8))]
+    _fill(cache, g, table, [128])
+    q = _randn(g, cache.dt, 3, 4, 64)
+    for n in ((1 << 31) - 1, (1 << 31) - 60, 1 << 30):
+        for window, sinks in ((1, (1 << 31) - 1), (1 << 20, 70), ((1 << 31) - 1, 1), (5, 0), (0, 0)):
+            o, _ = _run_paged(cache, q, _ends([3]), _i32([n]), _i32(table), 4, 1, window, sinks)
+            k, v = cache.rows(table[0], 128)
+            place = torch.arange(n - 3, n, device="cuda")
+            r, av, err = _attend(q, k, v, place, True, window, sinks, 0.125)
+            _close(o, r, av, err, cache.u, 128, v.abs().max())
