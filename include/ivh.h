@@ -308,8 +308,9 @@ typedef struct ivh_paged_attn_desc {
    same time need one each; its contents before a call do not matter */
 int ivh_paged_attention_workspace(const ivh_paged_attn_desc * d, int batch, int tokens, size_t * bytes);
 /* o = softmax(scale q k^T) v over the cached tokens of each row's sequence; lens, cu as for the append
-   that stored the rows' own tokens.  A row that sees no key is zero; infinities and NaN reach only
-   rows that see them.  o must not overlap an operand. */
+   that stored the rows' own tokens.  A row that sees no key, or none with a score above -infinity, is zero;
+   infinities and NaN reach only rows that see them.  Value scales below 1e-30 count as 1e-30.  o must
+   not overlap an operand. */
 int ivh_paged_attention(const ivh_paged_attn_desc * d, const void * q, const void * kc, const void * vc, const float * ks,
                         const float * vs, const int32_t * cu, const int32_t * lens, const int32_t * table, void * o,
                         int batch, int tokens, void * workspace, size_t workspace_bytes, void * stream);

@@ -23,7 +23,7 @@ size_t paged_split(PagedParams & p, int max_new, int max_len)
   // Keys: a work-group for each CU where there are keys enough (more parts cost more in joining
   // than they bring: 32 rows over 60000 keys 28 us with 256 work-groups, 36 with 1024).  With few rows none is
   // longer than 24 steps a wave, so that a ragged batch's long sequences do not outlast the others (64 of
-  // 900 to 16001 keys 208 us, 220 unsplit; 64 of 8192 each 195 us, 185 unsplit); with many the partial sums would
+  // 900 to 16001 keys 209 us, 218 unsplit; 64 of 8192 each pay for it, 191 us, 182 unsplit); with many the partial sums would
   // be too large for that.
   long len = std::min<long>(max_len, (long)c.width * c.page);
   if (p.window) len = std::min<long>(len, (long)p.window + p.sinks + max_new + 128);

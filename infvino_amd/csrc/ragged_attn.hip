@@ -29,12 +29,13 @@
 // ones, so a row's weights add up to 1.
 //
 // Measured (a bf16 product of 8192^3 reaches 1.23 PFLOP/s here): a prompt of 16384 tokens, 16 heads
-// of 128 channels on 4, causal: 1000 to 1080 us by card, 1.12 to 1.04 PFLOP/s.  The matrix cores are busy half the cycles and
+// of 128 channels on 4, causal: 1000 to 1080 us by card, 1.10 to 1.02 PFLOP/s.  The matrix cores are busy half the cycles and
 // the vector unit most of the others: work of one wave hides little of another's, with or without
 // copies, exponentials or LDS reads (each taken out alone changes 3 to 10 %), and zeros for data run
-// a fifth faster, which is power.  Five prompts of up to 6007 in a window of 1024: 189 us, 0.74 PFLOP/s, the
-// same and the last of 4.2 rounds of work-groups.  64 x 16 images of up to 400 tokens, 72 channels:
-// 100 us, 0.48 PFLOP/s: products on 80 and 96 channels, 7 steps a work-group behind 3 us of its start.
+// a fifth faster, which is power.  Five prompts of up to 6007 in a window of 1024: 186 to 194 us, 0.73 to
+// 0.70 PFLOP/s, the same and the last of 4.6 rounds of work-groups.  64 x 16 images of up to 400 tokens, 72
+// channels: 100 us, 0.35 PFLOP/s (0.43 with the products on 80 and 96 channels that it runs), 5 to 7
+// steps a work-group behind 3 us of its start.  Operations are those of the pairs that are seen.
 #include <algorithm>
 #include <stdexcept>
 
