@@ -228,6 +228,7 @@ int ivh_bmm_f16(const void * a, const void * b, void * y, int bb, int m, int k, 
  */
 #define IVH_F16 0
 #define IVH_BF16 1
+#define IVH_F32 2           /* logits of ivh_sample alone */
 
 /* Rotary positions: frequency f < rot / 2 turns a pair of a head's first rot channels by
    pos[axis(f)][token] * freq[f] radians: (a, b) -> (a cos - b sin, b cos + a sin).  Channels from rot on
@@ -329,6 +330,79 @@ typedef struct ivh_attn_desc {
    cu_k[b] .. (cu_q and cu_k may be one array).  o must not overlap an operand. */
 int ivh_attention(const ivh_attn_desc * d, const void * q, const void * k, const void * v, const int32_t * cu_q,
                   const int32_t * cu_k, void * o, int batch, int tokens_q, int tokens_k, void * stream);
+
+typedef struct ivh_prefix_attn_desc {
+  ivh_cache_desc cache;
+  int heads;                /* query heads; heads / cache.heads share a key head */
+  float scale;              /* of q . k */
+  int64_t q_token, q_head, o_token, o_head;
+  int max_new, max_len;     /* new and cached tokens of a sequence at most, 0: unknown, */
+  int max_shared;           /* and shared tokens of a group.  They steer how the call is split;
+                               results hold for any lengths */
+} ivh_prefix_attn_desc;
+
+/* workspace of a call: partial sums.  Calls that may run at the same time need one each; its contents
+   before a call do not matter */
+int ivh_prefix_attention_workspace(const ivh_prefix_attn_desc * d, int batch, int groups, int tokens, size_t * bytes);
+/* ivh_paged_attention without a window, for sequences that share their first pages (answers to one prompt, a common
+   instruction): a group's shared keys and values are read once for all rows of its sequences.  Group g is sequences
+   group[g] .. group[g + 1] - 1 (group [groups + 1] never decreases; sequences of no group share nothing) and
+   its sequences' tables hold the same pages for the first shared[g] tokens, counted in whole pages.  Only
+   tokens that every new row of the group may see are taken together, in whole steps of 64; what is left of them is
+   read with each sequence's own, so any shared[g] whose pages are the same is right. */
+int ivh_prefix_attention(const ivh_prefix_attn_desc * d, const void * q, const void * kc, const void * vc, const float * ks,
+                         const float * vs, const int32_t * cu, const int32_t * lens, const int32_t * table,
+                         const int32_t * group, const int32_t * shared, void * o, int batch, int groups, int tokens,
+                         void * workspace, size_t workspace_bytes, void * stream);
+
+typedef struct ivh_linear_attn_desc {
+  int type;                 /* IVH_F16 or IVH_BF16 */
+  int heads, key_heads;     /* heads of values, states and outputs; heads / key_heads share queries and keys */
+  int key_dim, dim;         /* channels of queries and keys, of values: multiples of 16, at most 256 */
+  float scale;              /* of q . k */
+  int slots;                /* states in the buffer */
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head;
+  int64_t g_token, g_head;  /* of the decays; g_token 0: one for each head, whatever the token */
+  int max_new;              /* rows of a sequence at most, 0: unknown.  Steers how the call is split;
+                               results hold for any lengths */
+} ivh_linear_attn_desc;
+
+/* workspace of a call: states between the parts of long sequences; as above */
+int ivh_linear_attention_workspace(const ivh_linear_attn_desc * d, int batch, int tokens, size_t * bytes);
+/* Linear attention with a decay: for a sequence's rows t in order and each head
+     S <- exp(g[t]) S + k[t]^T v[t],   o[t] = scale q[t] S
+   with the state S [key_dim][dim] in fp32.  state [slots][heads][key_dim][dim]; sequence b begins with
+   slot from[b] (null, or a number outside [0, slots): zeros) and leaves its state in slot to[b] (null, or
+   outside: nowhere).  A slot that a sequence writes is no other sequence's of the same call, but any
+   number may begin with one that none writes, and to[b] may be from[b]: the answers to one prompt begin with its
+   state.  A sequence without rows hands its state on.  g: natural logarithms of the decays, fp32; -infinity
+   forgets what was before (but no infinity or NaN in it).  q, k, v rows start at multiples of 16 bytes, o's
+   too.  Infinities and NaN reach only the rows from theirs on.  o and state must not overlap an operand. */
+int ivh_linear_attention(const ivh_linear_attn_desc * d, const void * q, const void * k, const void * v, const float * g,
+                         const int32_t * cu, const int32_t * from, const int32_t * to, float * state, void * o, int batch,
+                         int tokens, void * workspace, size_t workspace_bytes, void * stream);
+
+typedef struct ivh_sample_desc {
+  int type;                 /* of the logits: IVH_F16, IVH_BF16 or IVH_F32 */
+  int vocab;                /* at most 2^19 */
+  int64_t row;              /* elements between rows of logits */
+} ivh_sample_desc;
+
+int ivh_sample_workspace(const ivh_sample_desc * d, int rows, size_t * bytes);
+/* The next token of each row of logits [rows][vocab], drawn with the random number u[row] in [0, 1).
+   With T = temperature[row], weights are w = exp((x - max x) / T), held as whole multiples of 2^-44, so that sums
+   do not depend on an order.  Tokens in descending order, equal ones by index, are kept up to the shortest of
+     top_k[row] tokens (<= 0: all),
+     the fewest of those whose weights reach top_p[row] times the sum of those (>= 1: all),
+     the tokens with w >= min_p[row] (<= 0: all),
+   but one at least.  The token is the first by index whose weight and those of the kept tokens before it
+   sum to more than u times the sum of all kept.  T <= 0: the first of the largest.  Null arrays: T = 1, no
+   filter.  NaN logits count as -infinity, and so does nothing else: a row without a larger one gives -1.  NaN
+   in temperature: as 0; in top_p, min_p: no filter; u: as 0, and u >= 1 takes the last kept token that has a weight.
+   Logits of any alignment of their type. */
+int ivh_sample(const ivh_sample_desc * d, const void * logits, const float * temperature, const int32_t * top_k,
+               const float * top_p, const float * min_p, const float * u, int32_t * token, int rows, void * workspace,
+               size_t workspace_bytes, void * stream);
 
 #ifdef __cplusplus
 }

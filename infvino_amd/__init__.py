@@ -90,6 +90,26 @@ class AttentionDesc(C.Structure):
         [("max_q", C.c_int)]
 
 
+class PrefixAttentionDesc(C.Structure):
+    """ivh_prefix_attn_desc."""
+    _fields_ = [("cache", CacheDesc), ("heads", C.c_int), ("scale", C.c_float)] + \
+        [(n, C.c_int64) for n in ("q_token", "q_head", "o_token", "o_head")] + \
+        [(n, C.c_int) for n in ("max_new", "max_len", "max_shared")]
+
+
+class LinearAttentionDesc(C.Structure):
+    """ivh_linear_attn_desc."""
+    _fields_ = [(n, C.c_int) for n in ("type", "heads", "key_heads", "key_dim", "dim")] + \
+        [("scale", C.c_float), ("slots", C.c_int)] + \
+        [(n, C.c_int64) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "o_token", "o_head",
+                                  "g_token", "g_head")] + [("max_new", C.c_int)]
+
+
+class SampleDesc(C.Structure):
+    """ivh_sample_desc."""
+    _fields_ = [("type", C.c_int), ("vocab", C.c_int), ("row", C.c_int64)]
+
+
 _cdp = C.POINTER(ConvDesc)
 
 SIGNATURES = {
@@ -141,6 +161,12 @@ SIGNATURES = {
     "ivh_paged_attention_workspace": (_i, [C.POINTER(PagedAttentionDesc), _i, _i, _szp]),
     "ivh_paged_attention": (_i, [C.POINTER(PagedAttentionDesc)] + [_vp] * 9 + [_i, _i, _vp, _sz, _vp]),
     "ivh_attention": (_i, [C.POINTER(AttentionDesc)] + [_vp] * 6 + [_i, _i, _i, _vp]),
+    "ivh_prefix_attention_workspace": (_i, [C.POINTER(PrefixAttentionDesc), _i, _i, _i, _szp]),
+    "ivh_prefix_attention": (_i, [C.POINTER(PrefixAttentionDesc)] + [_vp] * 11 + [_i, _i, _i, _vp, _sz, _vp]),
+    "ivh_linear_attention_workspace": (_i, [C.POINTER(LinearAttentionDesc), _i, _i, _szp]),
+    "ivh_linear_attention": (_i, [C.POINTER(LinearAttentionDesc)] + [_vp] * 9 + [_i, _i, _vp, _sz, _vp]),
+    "ivh_sample_workspace": (_i, [C.POINTER(SampleDesc), _i, _szp]),
+    "ivh_sample": (_i, [C.POINTER(SampleDesc)] + [_vp] * 7 + [_i, _vp, _sz, _vp]),
 }
 
 _lib = None

@@ -46,10 +46,10 @@ namespace {
 struct Steps {
   int total, first, from;
 };
-__device__ __forceinline__ Steps key_steps(int full, int imin, int imax, int window, int sinks)
+__device__ __forceinline__ Steps key_steps(int full, int imin, int imax, int window, int sinks, int skip)
 {
   const int end = imax >= full ? full : imax + 1;
-  const int lo = window ? (int)min(max((long)imin - window + 1, 0L), (long)max(end, 0)) : 0;
+  const int lo = window ? (int)min(max((long)imin - window + 1, 0L), (long)max(end, 0)) : min(skip, max(end, 0));
   Steps s;
   s.from = lo / 64;
   s.first = min((min(sinks, lo) + 63) / 64, s.from);
@@ -58,11 +58,43 @@ __device__ __forceinline__ Steps key_steps(int full, int imin, int imax, int win
 }
 __device__ __forceinline__ int step_key(const Steps & s, int n) { return 64 * (n < s.first ? n : s.from + n - s.first); }
 
+// Which keys a build takes: all of a sequence; those behind what its group shares; a group's shared ones,
+// for the rows of all its sequences.
+enum KeysOf : int { kAllKeys, kOwnKeys, kSharedKeys };
+
+// Group g's first sequence and rows, and the leading keys that are taken once for all of them: whole
+// pages and steps, of which the first new row of every sequence sees each, so that nothing is masked.
+struct SharedPart {
+  int first, c0, c1, keys;
+};
+__device__ __forceinline__ SharedPart shared_part(const PagedParams & p, int g)
+{
+  const CacheParams & c = p.c;
+  const int b0 = min(max(p.member[g], 0), c.batch), b1 = min(max(p.member[g + 1], b0), c.batch);
+  int keys = min(max(p.shared[g], 0), c.width * c.page);
+  for (int b = b0 + (threadIdx.x & 63); b < b1; b += 64) {
+    const int c0 = min(max(c.cu[b], 0), c.tokens), c1 = min(max(c.cu[b + 1], c0), c.tokens);
+    if (c1 > c0) keys = min(keys, max(max(c.lens[b], 0) - (c1 - c0) + 1, 0));
+  }
+#pragma unroll
+  for (int i = 32; i >= 1; i /= 2) keys = min(keys, __shfl_xor(keys, i));
+  const int unit = max(c.page, 64);
+  const int c0 = min(max(c.cu[b0], 0), c.tokens), c1 = min(max(c.cu[b1], c0), c.tokens);
+  return SharedPart{b0, c0, c1, __builtin_amdgcn_readfirstlane(keys / unit * unit)};
+}
+// keys that sequence b leaves to its group
+__device__ __forceinline__ int keys_shared(const PagedParams & p, int b)
+{
+  if (p.groups == 0) return 0;
+  const int g = find_seq(p.groups, b, [&](int i) { return (long)p.member[i]; });
+  return p.member[g] <= b && b < p.member[g + 1] ? shared_part(p, g).keys : 0;
+}
+
 }  // namespace
 
 // QT: 16-row tiles of a wave; WK: waves that share rows and split the keys, 4 / WK row ranges.
 // DP: head size rounded up to 64, 128 or 256; FULL: it is that size.
-template <int TYPE, int BITS, int DP, bool FULL, int QT, int WK>
+template <int TYPE, int BITS, int DP, bool FULL, int QT, int WK, int KEYS>
 __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(const PagedParams p, int units)
 {
   using T = St<TYPE>;
@@ -90,16 +122,29 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
   const int slot = w % p.row_slots;
   w = w / p.row_slots * kXcds + blockIdx.x % kXcds;
   if (w >= units) return;
-  const int seqs = c.batch * c.heads, part = w / seqs;
+  const int seqs = (KEYS == kSharedKeys ? p.groups : c.batch) * c.heads, part = w / seqs;
   w -= part * seqs;
   const int h = w % c.heads, b = w / c.heads;
 
-  const int c0 = min(max(c.cu[b], 0), c.tokens), c1 = min(max(c.cu[b + 1], c0), c.tokens);
+  int c0, c1, full, place0, skip = 0;  // place0: of the first new token
+  const int32_t * table = c.table;
+  if constexpr (KEYS == kSharedKeys) {
+    const SharedPart part_of = shared_part(p, b);
+    if (part_of.keys == 0) return;
+    c0 = part_of.c0;
+    c1 = part_of.c1;
+    full = place0 = part_of.keys;  // every row sees all of them
+    table += (long)part_of.first * c.width;
+  } else {
+    c0 = min(max(c.cu[b], 0), c.tokens);
+    c1 = min(max(c.cu[b + 1], c0), c.tokens);
+    const long len = c.lens[b];
+    full = (int)min(max(len, 0L), (long)c.width * c.page);
+    place0 = (int)max(len, 0L) - (c1 - c0);
+    table += (long)b * c.width;
+    if constexpr (KEYS == kOwnKeys) skip = keys_shared(p, b);
+  }
   const int nnew = c1 - c0, rows = nnew * p.group;
-  const long len = c.lens[b];
-  const int full = (int)min(max(len, 0L), (long)c.width * c.page);
-  const int place0 = (int)max(len, 0L) - nnew;  // place of the first new token
-  const int32_t * table = c.table + (long)b * c.width;
   const int lp = 31 - __clz(c.page);  // page is a power of two
   const long page_bytes = (long)c.page * c.dim * (BITS / 8);
   const int nblk = c.dim / 16;
@@ -111,7 +156,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
     const int row0 = tile * ROWS + wr * 16 * QT, rend = min(rows, row0 + 16 * QT);  // this wave's rows
     const int wg_last = min(rows, tile * ROWS + ROWS) - 1;
     // the steps are the work-group's, the masks this wave's (which may have no rows)
-    const Steps steps = key_steps(full, place0 + tile * ROWS / p.group, place0 + wg_last / p.group, p.window, p.sinks);
+    const Steps steps = key_steps(full, place0 + tile * ROWS / p.group, place0 + wg_last / p.group, p.window, p.sinks, skip);
     const int imin = place0 + row0 / p.group, imax = place0 + (max(rend, row0 + 1) - 1) / p.group;
     const int per = max(p.part_steps, (steps.total + p.parts - 1) / p.parts);
     const int n0 = part * per, n1 = rend > row0 ? min(steps.total, n0 + per) : 0;
@@ -126,7 +171,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
       const int row = row0 + 16 * t + r, tok = row / p.group;
       const bool live = row < rows;
       const int place = place0 + tok, hi = live ? min(place, full - 1) : -1;
-      seen_lo[t] = p.window ? (int)max((long)place - p.window + 1, 0L) : 0;
+      seen_lo[t] = p.window ? (int)max((long)place - p.window + 1, 0L) : skip;
       seen_n[t] = hi - seen_lo[t];
       seen_first[t] = p.window ? min(p.sinks, hi + 1) : 0;
       // rows and channels that are not there read some that are: a branch would make each load wait
@@ -459,7 +504,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
 #pragma unroll
           for (int j = 0; j < NB; ++j) o[u][j] *= __builtin_ldexpf(1.0f, -UP);
         const long row = (long)(c0 + tok) * p.heads + head;
-        if (p.parts == 1) {
+        if (KEYS == kAllKeys && p.parts == 1) {
           const float inv = L[u] != 0.0f ? 1.0f / L[u] : 0.0f;  // a row that saw nothing is zero (NaN stays)
           E * out = static_cast<E *>(p.o) + (long)(c0 + tok) * p.o_token + (long)head * p.o_head;
 #pragma unroll
@@ -469,14 +514,19 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
             *reinterpret_cast<u2v *>(out + 16 * j + 4 * g) = y;
           }
         } else {
-          const long total = (long)c.tokens * p.heads, at = (long)part * total + row;
+          const long total = (long)c.tokens * p.heads, at = (long)(part + (KEYS == kOwnKeys ? p.lead : 0)) * total + row;
+          const long all = KEYS == kAllKeys ? p.parts : p.all_parts;
           if (n0 < n1) {
             float * out = p.ws + at * c.dim;
 #pragma unroll
             for (int j = 0; j < NB; ++j)
               if (FULL || j < nblk) *reinterpret_cast<f4v *>(out + 16 * j + 4 * g) = o[u][j];
           }
-          if (g == 0) *reinterpret_cast<f2v *>(p.ws + (long)p.parts * total * c.dim + 2 * at) = f2v{M[u], L[u]};
+          f2v * ml = reinterpret_cast<f2v *>(p.ws + all * total * c.dim);
+          if (g == 0) ml[at] = f2v{M[u], L[u]};
+          // a sequence that shares nothing leaves the parts of groups empty
+          if (KEYS == kOwnKeys && skip == 0 && part == 0 && g == 0)
+            for (int i = 0; i < p.lead; ++i) ml[i * total + row] = f2v{kLowest, 0.0f};
         }
       }
     }
@@ -541,48 +591,52 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p, in
 
 namespace {
 
-template <int TYPE, int BITS, int DP, bool FULL, int QT, int WK> void launch_paged(const PagedParams & p, hipStream_t s)
+template <int TYPE, int BITS, int DP, bool FULL, int QT, int WK, int KEYS> void launch_paged(const PagedParams & p, hipStream_t s)
 {
-  auto kern = paged_attn_kernel<TYPE, BITS, DP, FULL, QT, WK>;
+  auto kern = paged_attn_kernel<TYPE, BITS, DP, FULL, QT, WK, KEYS>;
   const size_t lds = (size_t)(WK / 2) * (4 / WK) * 16 * QT * (DP + 4 + 2) * sizeof(float);
-  const long units = (long)p.c.batch * p.c.heads * p.parts;
+  const long units = (long)(KEYS == kSharedKeys ? p.groups : p.c.batch) * p.c.heads * p.parts;
   const dim3 grid((unsigned)((units + kXcds - 1) / kXcds * kXcds * p.row_slots)), blk(256);
   hipLaunchKernelGGL(kern, grid, blk, lds, s, p, (int)units);
 }
 
-template <int TYPE, int BITS, int DP, bool FULL> void launch_paged_rows(const PagedParams & p, hipStream_t s)
+template <int TYPE, int BITS, int DP, bool FULL, int KEYS> void launch_paged_rows(const PagedParams & p, hipStream_t s)
 {
   constexpr int MOST = DP <= 64 ? 2 : 1;
   if (p.row_waves == 1) {
-    if (p.row_tiles == 1) launch_paged<TYPE, BITS, DP, FULL, 1, 4>(p, s);
-    else launch_paged<TYPE, BITS, DP, FULL, MOST, 4>(p, s);
+    if (p.row_tiles == 1) launch_paged<TYPE, BITS, DP, FULL, 1, 4, KEYS>(p, s);
+    else launch_paged<TYPE, BITS, DP, FULL, MOST, 4, KEYS>(p, s);
   } else if (p.row_waves == 2) {
-    launch_paged<TYPE, BITS, DP, FULL, MOST, 2>(p, s);
+    launch_paged<TYPE, BITS, DP, FULL, MOST, 2, KEYS>(p, s);
   } else {
-    launch_paged<TYPE, BITS, DP, FULL, MOST, 1>(p, s);
+    launch_paged<TYPE, BITS, DP, FULL, MOST, 1, KEYS>(p, s);
   }
 }
 
-template <int TYPE, int BITS> void launch_paged_dim(const PagedParams & p, hipStream_t s)
+template <int TYPE, int BITS, int KEYS = kAllKeys> void launch_paged_dim(const PagedParams & p, hipStream_t s)
 {
-  if (p.c.dim == 64) launch_paged_rows<TYPE, BITS, 64, true>(p, s);
-  else if (p.c.dim < 64) launch_paged_rows<TYPE, BITS, 64, false>(p, s);
-  else if (p.c.dim == 128) launch_paged_rows<TYPE, BITS, 128, true>(p, s);
-  else if (p.c.dim < 128) launch_paged_rows<TYPE, BITS, 128, false>(p, s);
-  else if (p.c.dim == 256) launch_paged_rows<TYPE, BITS, 256, true>(p, s);
-  else launch_paged_rows<TYPE, BITS, 256, false>(p, s);
+  if (p.c.dim == 64) launch_paged_rows<TYPE, BITS, 64, true, KEYS>(p, s);
+  else if (p.c.dim < 64) launch_paged_rows<TYPE, BITS, 64, false, KEYS>(p, s);
+  else if (p.c.dim == 128) launch_paged_rows<TYPE, BITS, 128, true, KEYS>(p, s);
+  else if (p.c.dim < 128) launch_paged_rows<TYPE, BITS, 128, false, KEYS>(p, s);
+  else if (p.c.dim == 256) launch_paged_rows<TYPE, BITS, 256, true, KEYS>(p, s);
+  else launch_paged_rows<TYPE, BITS, 256, false, KEYS>(p, s);
+}
+
+template <int TYPE> void launch_paged_join(const PagedParams & p, hipStream_t s)
+{
+  // a lot for every two parts where lanes allow it, and where a launch holds the work-groups (fewer than 2^24)
+  const long rows = (long)p.c.tokens * p.heads;
+  const int lanes = p.c.dim / 4, lots = rows < 1L << 23 ? std::max(1, std::min(p.parts / 2, 256 / lanes)) : 1, per = 256 / (lanes * lots);
+  const dim3 grid((unsigned)((rows + per - 1) / per));
+  hipLaunchKernelGGL((paged_join_kernel<TYPE>), grid, dim3(256), 0, s, p, lots);
 }
 
 template <int TYPE> void launch_paged_type(const PagedParams & p, hipStream_t s)
 {
   if (p.c.bits == 8) launch_paged_dim<TYPE, 8>(p, s);
   else launch_paged_dim<TYPE, 16>(p, s);
-  if (p.parts > 1) {
-    // a lot for every two parts where lanes allow it
-    const int lanes = p.c.dim / 4, lots = std::max(1, std::min(p.parts / 2, 256 / lanes)), per = 256 / (lanes * lots);
-    const dim3 grid((unsigned)(((long)p.c.tokens * p.heads + per - 1) / per));
-    hipLaunchKernelGGL((paged_join_kernel<TYPE>), grid, dim3(256), 0, s, p, lots);
-  }
+  if (p.parts > 1) launch_paged_join<TYPE>(p, s);
 }
 
 }  // namespace

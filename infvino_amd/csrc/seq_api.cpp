@@ -169,6 +169,63 @@ ivh::PagedParams paged(const ivh_paged_attn_desc * d, int batch, int tokens, siz
   return p;
 }
 
+ivh::PrefixParams prefix(const ivh_prefix_attn_desc * d, int batch, int groups, int tokens, size_t * bytes)
+{
+  need(d, "null descriptor");
+  ivh::PrefixParams p;
+  ivh::PagedParams & o = p.own;
+  o.c = cache(d->cache);
+  check_counts(batch, tokens);
+  need(groups >= 0 && groups <= kMaxBatch, "groups must be in [0, 2^20]");
+  need(d->heads >= 1 && d->heads % d->cache.heads == 0, "heads must be a multiple of the cache's heads");
+  need((int64_t)tokens * d->heads <= kMaxTokens && (int64_t)std::max(batch, groups) * d->cache.heads <= kMaxHeads, "too many rows for a call");
+  need(std::isfinite(d->scale * kLog2E), "scale must be finite");
+  need(d->max_new >= 0 && d->max_len >= 0 && d->max_shared >= 0, "max_new, max_len and max_shared must not be negative");
+  o.c.batch = batch;
+  o.c.tokens = tokens;
+  o.heads = d->heads;
+  o.group = d->heads / d->cache.heads;
+  o.scale_log2 = d->scale * kLog2E;
+  o.groups = groups;
+  const int most = d->cache.table_width * d->cache.page;
+  *bytes = batch && tokens ? ivh::prefix_split(p, d->max_new ? d->max_new : tokens, d->max_len ? d->max_len : most,
+                                               d->max_shared ? std::min(d->max_shared, most) : d->max_len ? std::min(d->max_len, most) : most) : 0;
+  return p;
+}
+
+// most states times heads, and rows times heads, of a call: a launch's work-groups are counted in 31 bits
+constexpr int kMaxStates = 1 << 22;
+
+void linear(const ivh_linear_attn_desc * d, int batch, int tokens)
+{
+  need(d, "null descriptor");
+  check_type(d->type);
+  check_counts(batch, tokens);
+  need(d->heads >= 1 && d->heads <= 4096 && d->key_heads >= 1 && d->heads % d->key_heads == 0,
+       "heads must be a multiple of the key heads, at most 4096");
+  need(d->key_dim >= 16 && d->key_dim <= 256 && d->key_dim % 16 == 0 && d->dim >= 16 && d->dim <= 256 && d->dim % 16 == 0,
+       "key_dim and dim must be multiples of 16, at most 256");
+  need((int64_t)batch * d->heads <= kMaxStates, "too many states for a call");
+  need(std::isfinite(d->scale), "scale must be finite");
+  need(d->slots >= 0 && d->max_new >= 0, "slots and max_new must not be negative");
+  need(d->g_token >= 0 && d->g_head >= 0, "decays: bad strides");
+}
+
+ivh::SampleParams sampling(const ivh_sample_desc * d, int rows)
+{
+  need(d, "null descriptor");
+  need(d->type == IVH_F16 || d->type == IVH_BF16 || d->type == IVH_F32, "type must be IVH_F16, IVH_BF16 or IVH_F32");
+  need(d->vocab >= 1 && d->vocab <= 1 << 19, "vocab must be in [1, 2^19]");
+  need(d->row >= 0, "sample: bad stride of rows");
+  need(rows >= 0 && rows <= 1 << 20, "rows must be in [0, 2^20]");
+  ivh::SampleParams p;
+  p.type = d->type;
+  p.vocab = d->vocab;
+  p.rows = rows;
+  p.row = d->row;
+  return p;
+}
+
 }  // namespace
 
 extern "C" {
@@ -329,6 +386,147 @@ int ivh_attention(const ivh_attn_desc * d, const void * q, const void * k, const
     p.o_head = d->o_head;
     ivh::launch_ragged_attention(p, static_cast<hipStream_t>(stream));
     check_launch("attention");
+  });
+}
+
+int ivh_prefix_attention_workspace(const ivh_prefix_attn_desc * d, int batch, int groups, int tokens, size_t * bytes)
+{
+  return guard([&] {
+    need(bytes, "null bytes");
+    prefix(d, batch, groups, tokens, bytes);
+  });
+}
+
+int ivh_prefix_attention(const ivh_prefix_attn_desc * d, const void * q, const void * kc, const void * vc, const float * ks,
+                         const float * vs, const int32_t * cu, const int32_t * lens, const int32_t * table, const int32_t * group,
+                         const int32_t * shared, void * o, int batch, int groups, int tokens, void * workspace, size_t workspace_bytes,
+                         void * stream)
+{
+  return guard([&] {
+    size_t bytes = 0;
+    ivh::PrefixParams p = prefix(d, batch, groups, tokens, &bytes);
+    if (batch == 0 || tokens == 0) return;
+    check_rows(q, d->q_token, d->q_head, 8, "queries");
+    check_rows(o, d->o_token, d->o_head, 8, "attention output");
+    check_apart(tokens, d->heads, d->cache.dim, d->o_token, d->o_head, "attention");
+    need(groups == 0 || (group && shared), "null groups");
+    need((reinterpret_cast<uintptr_t>(group) | reinterpret_cast<uintptr_t>(shared)) % 4 == 0, "misaligned groups");
+    bind(p.own.c, kc, vc, ks, vs, cu, lens, table, batch, tokens);
+    need(workspace && workspace_bytes >= bytes, "workspace too small (ivh_prefix_attention_workspace)");
+    need(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must start at a multiple of 16 bytes");
+    check_device(stream, {q, kc, vc, ks, vs, cu, lens, table, groups ? group : nullptr, groups ? shared : nullptr, o, workspace});
+    p.first.c = p.own.c;
+    for (ivh::PagedParams * x : {&p.first, &p.own}) {
+      x->q = q;
+      x->o = o;
+      x->q_token = d->q_token;
+      x->q_head = d->q_head;
+      x->o_token = d->o_token;
+      x->o_head = d->o_head;
+      x->ws = static_cast<float *>(workspace);
+      x->member = group;
+      x->shared = shared;
+    }
+    ivh::launch_prefix_attention(p, static_cast<hipStream_t>(stream));
+    check_launch("prefix attention");
+  });
+}
+
+int ivh_linear_attention_workspace(const ivh_linear_attn_desc * d, int batch, int tokens, size_t * bytes)
+{
+  return guard([&] {
+    need(bytes, "null bytes");
+    linear(d, batch, tokens);
+    *bytes = 0;
+  });
+}
+
+int ivh_linear_attention(const ivh_linear_attn_desc * d, const void * q, const void * k, const void * v, const float * g,
+                         const int32_t * cu, const int32_t * from, const int32_t * to, float * state, void * o, int batch, int tokens,
+                         void * workspace, size_t workspace_bytes, void * stream)
+{
+  return guard([&] {
+    linear(d, batch, tokens);
+    if (batch == 0) return;
+    if (tokens > 0) {
+      check_rows(q, d->q_token, d->q_head, 8, "queries");
+      check_rows(k, d->k_token, d->k_head, 8, "keys");
+      check_rows(v, d->v_token, d->v_head, 8, "values");
+      check_rows(o, d->o_token, d->o_head, 8, "attention output");
+      check_apart(tokens, d->heads, d->dim, d->o_token, d->o_head, "attention");
+      need(g, "null decays");
+    }
+    need(cu, "null sequence offsets");
+    need((reinterpret_cast<uintptr_t>(cu) | reinterpret_cast<uintptr_t>(from) | reinterpret_cast<uintptr_t>(to) |
+          reinterpret_cast<uintptr_t>(g)) % 4 == 0, "misaligned offsets, slots or decays");
+    need(state || d->slots == 0, "null states");
+    need(reinterpret_cast<uintptr_t>(state) % 16 == 0, "states must start at a multiple of 16 bytes");
+    check_device(stream, {q, k, v, g, cu, from, to, state, o});
+    ivh::LinearParams p;
+    p.type = d->type;
+    p.heads = d->heads;
+    p.group = d->heads / d->key_heads;
+    p.key_dim = d->key_dim;
+    p.dim = d->dim;
+    p.batch = batch;
+    p.tokens = tokens;
+    p.slots = d->slots;
+    p.max_new = d->max_new ? d->max_new : tokens;
+    p.scale = d->scale;
+    p.q = q;
+    p.k = k;
+    p.v = v;
+    p.g = g;
+    p.cu = cu;
+    p.from = from;
+    p.to = to;
+    p.state = state;
+    p.o = o;
+    p.q_token = d->q_token;
+    p.q_head = d->q_head;
+    p.k_token = d->k_token;
+    p.k_head = d->k_head;
+    p.v_token = d->v_token;
+    p.v_head = d->v_head;
+    p.o_token = d->o_token;
+    p.o_head = d->o_head;
+    p.g_token = d->g_token;
+    p.g_head = d->g_head;
+    ivh::launch_linear_attention(p, static_cast<hipStream_t>(stream));
+    check_launch("linear attention");
+  });
+}
+
+int ivh_sample_workspace(const ivh_sample_desc * d, int rows, size_t * bytes)
+{
+  return guard([&] {
+    need(bytes, "null bytes");
+    sampling(d, rows);
+    *bytes = 0;
+  });
+}
+
+int ivh_sample(const ivh_sample_desc * d, const void * logits, const float * temperature, const int32_t * top_k, const float * top_p,
+               const float * min_p, const float * u, int32_t * token, int rows, void * workspace, size_t workspace_bytes, void * stream)
+{
+  return guard([&] {
+    ivh::SampleParams p = sampling(d, rows);
+    if (rows == 0) return;
+    need(logits && u && token, "sample: null operand");
+    need(reinterpret_cast<uintptr_t>(logits) % (d->type == IVH_F32 ? 4 : 2) == 0, "sample: misaligned logits");
+    need((reinterpret_cast<uintptr_t>(temperature) | reinterpret_cast<uintptr_t>(top_k) | reinterpret_cast<uintptr_t>(top_p) |
+          reinterpret_cast<uintptr_t>(min_p) | reinterpret_cast<uintptr_t>(u) | reinterpret_cast<uintptr_t>(token)) % 4 == 0,
+         "sample: misaligned operand");
+    check_device(stream, {logits, temperature, top_k, top_p, min_p, u, token});
+    p.x = logits;
+    p.temperature = temperature;
+    p.top_k = top_k;
+    p.top_p = top_p;
+    p.min_p = min_p;
+    p.u = u;
+    p.token = token;
+    ivh::launch_sample(p, static_cast<hipStream_t>(stream));
+    check_launch("sample");
   });
 }
 

@@ -10,7 +10,7 @@
 
 namespace ivh {
 
-enum SeqType : int { kSeqF16 = 0, kSeqBF16 = 1 };
+enum SeqType : int { kSeqF16 = 0, kSeqBF16 = 1, kSeqF32 = 2 };  // the last: logits alone
 
 // Rotation of a head's leading `rot` channels by positions with up to four axes.
 struct RotParams {
@@ -71,12 +71,54 @@ struct PagedParams {
   int row_slots = 1;             // work-groups over the rows of a sequence and key head
   int parts = 1, part_steps = 1; // work-groups over the keys, and 64-key steps of each at least
   float * ws = nullptr;          // parts > 1: partial sums [parts][tokens][heads][dim], maxima and sums
+  // with shared first tokens: each sequence's own keys have parts `lead` .. all_parts - 1 of the workspace
+  const int32_t * member = nullptr;  // [groups + 1] first sequences
+  const int32_t * shared = nullptr;  // [groups] tokens
+  int groups = 0, lead = 0, all_parts = 1;
 };
 // Sets the split of a call with at most max_new new tokens and max_len cached ones in a
 // sequence (bounds that only steer the split); returns the workspace bytes.
 size_t paged_split(PagedParams & p, int max_new, int max_len);
 void launch_paged_attention(const PagedParams & p, hipStream_t s);
 void launch_paged_bf16(const PagedParams & p, hipStream_t s);  // its bf16 kernels, built by themselves
+
+// Attention with shared first tokens: the split of both kinds of keys, those of groups first.
+struct PrefixParams {
+  PagedParams first, own;
+};
+size_t prefix_split(PrefixParams & p, int max_new, int max_len, int max_shared);
+void launch_prefix_attention(const PrefixParams & p, hipStream_t s);
+void launch_prefix_bf16(const PrefixParams & p, hipStream_t s);
+
+struct LinearParams {
+  int type = 0, heads = 0, group = 1, key_dim = 0, dim = 0;  // group: heads that share queries and keys
+  int batch = 0, tokens = 0, slots = 0, max_new = 0;
+  float scale = 1.0f;
+  const void * q = nullptr;
+  const void * k = nullptr;
+  const void * v = nullptr;
+  const float * g = nullptr;
+  const int32_t * cu = nullptr;
+  const int32_t * from = nullptr;
+  const int32_t * to = nullptr;
+  float * state = nullptr;
+  void * o = nullptr;
+  long q_token = 0, q_head = 0, k_token = 0, k_head = 0, v_token = 0, v_head = 0, o_token = 0, o_head = 0, g_token = 0, g_head = 0;
+};
+void launch_linear_attention(const LinearParams & p, hipStream_t s);
+
+struct SampleParams {
+  int type = 0, vocab = 0, rows = 0;
+  long row = 0;
+  const void * x = nullptr;
+  const float * temperature = nullptr;
+  const int32_t * top_k = nullptr;
+  const float * top_p = nullptr;
+  const float * min_p = nullptr;
+  const float * u = nullptr;
+  int32_t * token = nullptr;
+};
+void launch_sample(const SampleParams & p, hipStream_t s);
 
 struct RaggedParams {
   int type = 0, heads = 0, group = 1, dim = 0;

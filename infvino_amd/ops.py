@@ -9,13 +9,13 @@ import ctypes as C
 
 import numpy as np
 
-from . import (AppendDesc, AttentionDesc, CacheDesc, ConvDesc, PagedAttentionDesc, RopeDesc, Rotation, _check,
-               lib)
+from . import (AppendDesc, AttentionDesc, CacheDesc, ConvDesc, LinearAttentionDesc, PagedAttentionDesc,
+               PrefixAttentionDesc, RopeDesc, Rotation, SampleDesc, _check, lib)
 
 ACT_NONE, ACT_SILU, ACT_RELU, ACT_HSWISH, ACT_HSIGMOID, ACT_SIGMOID = range(6)
 EW_ADD, EW_SUB, EW_MUL, EW_DIV = range(4)
 POOL_MAX, POOL_RESIZE = 0, 1
-F16, BF16 = 0, 1
+F16, BF16, F32 = 0, 1, 2
 
 
 def conv_desc(cin, cout, h, w, k=1, stride=1, pad=0, groups=1, act=ACT_NONE, has_bias=True,
@@ -148,3 +148,60 @@ def attention_desc(type, heads, kv_heads, dim, scale, causal=True, window=0, sin
 
 def attention(d: AttentionDesc, q, k, v, cu_q, cu_k, o, batch: int, tokens_q: int, tokens_k: int, stream=None) -> None:
     _check(lib().ivh_attention(d, q, k, v, cu_q, cu_k, o, batch, tokens_q, tokens_k, stream))
+
+
+def prefix_attention_desc(cache: CacheDesc, heads, scale, q=None, o=None, max_new=0, max_len=0, max_shared=0) -> PrefixAttentionDesc:
+    dense = (heads * cache.dim, cache.dim)
+    q, o = q or dense, o or dense
+    return PrefixAttentionDesc(cache, heads, scale, q[0], q[1], o[0], o[1], max_new, max_len, max_shared)
+
+
+def prefix_attention_workspace(d: PrefixAttentionDesc, batch: int, groups: int, tokens: int) -> int:
+    n = C.c_size_t()
+    _check(lib().ivh_prefix_attention_workspace(d, batch, groups, tokens, C.byref(n)))
+    return n.value
+
+
+def prefix_attention(d: PrefixAttentionDesc, q, kc, vc, ks, vs, cu, lens, table, group, shared, o, batch: int, groups: int,
+                     tokens: int, workspace=None, workspace_bytes=0, stream=None) -> None:
+    """group [groups + 1]: first sequence of each group; shared [groups]: tokens whose pages a group's sequences share."""
+    _check(lib().ivh_prefix_attention(d, q, kc, vc, ks, vs, cu, lens, table, group, shared, o, batch, groups, tokens, workspace,
+                                      workspace_bytes, stream))
+
+
+def linear_attention_desc(type, heads, key_heads, key_dim, dim, scale, slots, q=None, k=None, v=None, o=None, g=None,
+                          max_new=0) -> LinearAttentionDesc:
+    """g: strides of the decays, dense [tokens][heads] by default; (0, 1): one for each head."""
+    dk, dv = (key_heads * key_dim, key_dim), (heads * dim, dim)
+    q, k, v, o, g = q or dk, k or dk, v or dv, o or dv, g or (heads, 1)
+    return LinearAttentionDesc(type, heads, key_heads, key_dim, dim, scale, slots, q[0], q[1], k[0], k[1], v[0], v[1], o[0], o[1],
+                               g[0], g[1], max_new)
+
+
+def linear_attention_workspace(d: LinearAttentionDesc, batch: int, tokens: int) -> int:
+    n = C.c_size_t()
+    _check(lib().ivh_linear_attention_workspace(d, batch, tokens, C.byref(n)))
+    return n.value
+
+
+def linear_attention(d: LinearAttentionDesc, q, k, v, g, cu, start, to, state, o, batch: int, tokens: int, workspace=None,
+                     workspace_bytes=0, stream=None) -> None:
+    """start, to [batch]: the slots that sequences begin with and leave their states in, or None."""
+    _check(lib().ivh_linear_attention(d, q, k, v, g, cu, start, to, state, o, batch, tokens, workspace, workspace_bytes, stream))
+
+
+def sample_desc(type, vocab, row=None) -> SampleDesc:
+    """row: elements between two rows of logits, dense by default."""
+    return SampleDesc(type, vocab, vocab if row is None else row)
+
+
+def sample_workspace(d: SampleDesc, rows: int) -> int:
+    n = C.c_size_t()
+    _check(lib().ivh_sample_workspace(d, rows, C.byref(n)))
+    return n.value
+
+
+def sample(d: SampleDesc, logits, temperature, top_k, top_p, min_p, u, token, rows: int, workspace=None, workspace_bytes=0,
+           stream=None) -> None:
+    """temperature, top_k, top_p, min_p [rows]: None for 1 and no filter."""
+    _check(lib().ivh_sample(d, logits, temperature, top_k, top_p, min_p, u, token, rows, workspace, workspace_bytes, stream))
