@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p)
   typedef typename Logit<TYPE>::e E;
   __shared__ unsigned count[256];
   __shared__ u64 sums[256];
-  __shared__ unsigned wave_u[16], sh_code, sh_need_n;
+  __shared__ unsigned wave_u[16], sh_need_n;
   __shared__ u64 wave_s[16], sh_need_s, sh_above_s;
   __shared__ unsigned sh_above_n;
   __shared__ int sh_at;

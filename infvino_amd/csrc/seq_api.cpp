@@ -196,7 +196,7 @@ ivh::PrefixParams prefix(const ivh_prefix_attn_desc * d, int batch, int groups, 
 // most states times heads, and rows times heads, of a call: a launch's work-groups are counted in 31 bits
 constexpr int kMaxStates = 1 << 22;
 
-void linear(const ivh_linear_attn_desc * d, int batch, int tokens)
+ivh::LinearParams linear(const ivh_linear_attn_desc * d, int batch, int tokens, size_t * bytes)
 {
   need(d, "null descriptor");
   check_type(d->type);
@@ -209,6 +209,18 @@ void linear(const ivh_linear_attn_desc * d, int batch, int tokens)
   need(std::isfinite(d->scale), "scale must be finite");
   need(d->slots >= 0 && d->max_new >= 0, "slots and max_new must not be negative");
   need(d->g_token >= 0 && d->g_head >= 0, "decays: bad strides");
+  ivh::LinearParams p;
+  p.type = d->type;
+  p.heads = d->heads;
+  p.group = d->heads / d->key_heads;
+  p.key_dim = d->key_dim;
+  p.dim = d->dim;
+  p.batch = batch;
+  p.tokens = tokens;
+  p.slots = d->slots;
+  p.scale = d->scale;
+  *bytes = batch ? ivh::linear_split(p, std::min(d->max_new ? d->max_new : tokens, tokens)) : 0;
+  return p;
 }
 
 ivh::SampleParams sampling(const ivh_sample_desc * d, int rows)
@@ -436,8 +448,7 @@ int ivh_linear_attention_workspace(const ivh_linear_attn_desc * d, int batch, in
 {
   return guard([&] {
     need(bytes, "null bytes");
-    linear(d, batch, tokens);
-    *bytes = 0;
+    linear(d, batch, tokens, bytes);
   });
 }
 
@@ -446,7 +457,8 @@ int ivh_linear_attention(const ivh_linear_attn_desc * d, const void * q, const v
                          void * workspace, size_t workspace_bytes, void * stream)
 {
   return guard([&] {
-    linear(d, batch, tokens);
+    size_t bytes = 0;
+    ivh::LinearParams p = linear(d, batch, tokens, &bytes);
     if (batch == 0) return;
     if (tokens > 0) {
       check_rows(q, d->q_token, d->q_head, 8, "queries");
@@ -461,18 +473,13 @@ int ivh_linear_attention(const ivh_linear_attn_desc * d, const void * q, const v
           reinterpret_cast<uintptr_t>(g)) % 4 == 0, "misaligned offsets, slots or decays");
     need(state || d->slots == 0, "null states");
     need(reinterpret_cast<uintptr_t>(state) % 16 == 0, "states must start at a multiple of 16 bytes");
-    check_device(stream, {q, k, v, g, cu, from, to, state, o});
-    ivh::LinearParams p;
-    p.type = d->type;
-    p.heads = d->heads;
-    p.group = d->heads / d->key_heads;
-    p.key_dim = d->key_dim;
-    p.dim = d->dim;
-    p.batch = batch;
-    p.tokens = tokens;
-    p.slots = d->slots;
-    p.max_new = d->max_new ? d->max_new : tokens;
-    p.scale = d->scale;
+    need(bytes == 0 || (workspace && workspace_bytes >= bytes), "workspace too small (ivh_linear_attention_workspace)");
+    need(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must start at a multiple of 16 bytes");
+    check_device(stream, {q, k, v, g, cu, from, to, state, o, bytes ? workspace : nullptr});
+    if (bytes) {
+      p.ws = static_cast<float *>(workspace);
+      p.decay = p.ws + ((size_t)tokens / p.seg + batch) * p.heads * p.key_dim * p.dim;
+    }
     p.q = q;
     p.k = k;
     p.v = v;

@@ -92,7 +92,7 @@ void launch_prefix_bf16(const PrefixParams & p, hipStream_t s);
 
 struct LinearParams {
   int type = 0, heads = 0, group = 1, key_dim = 0, dim = 0;  // group: heads that share queries and keys
-  int batch = 0, tokens = 0, slots = 0, max_new = 0;
+  int batch = 0, tokens = 0, slots = 0;
   float scale = 1.0f;
   const void * q = nullptr;
   const void * k = nullptr;
@@ -104,7 +104,13 @@ struct LinearParams {
   float * state = nullptr;
   void * o = nullptr;
   long q_token = 0, q_head = 0, k_token = 0, k_head = 0, v_token = 0, v_head = 0, o_token = 0, o_head = 0, g_token = 0, g_head = 0;
+  // how a call is split, from linear_split
+  int seg = 0;                   // tokens of a segment, 0: token by token
+  float * ws = nullptr;          // first states of segments [tokens / seg + batch][heads][key_dim][dim], null: one each
+  float * decay = nullptr;       // of whole segments, behind them
 };
+// Sets the split of a call with at most max_new rows in a sequence; returns the workspace bytes.
+size_t linear_split(LinearParams & p, int max_new);
 void launch_linear_attention(const LinearParams & p, hipStream_t s);
 
 struct SampleParams {
