@@ -108,6 +108,7 @@ __global__ void __launch_bounds__(kStepThreads) linear_step_kernel(const LinearP
 namespace {
 
 typedef short s4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_ptr;
 
 constexpr int kChunk = 64;
 constexpr int kMaxSeg = 1 << 27;  // longer than any sequence: one segment each
@@ -161,6 +162,40 @@ __device__ __forceinline__ Segment segment_of(const LinearParams & p, int u)
 
 }  // namespace
 
+// Rows of LDS hold no padding, since copies write 64 x 16 bytes one behind the other; 16-byte pieces are permuted within a
+// row instead, piece c of row r to c ^ order(r), so that the lanes that are served together lie in distinct banks:
+// queries are read a row a lane, values four rows of 16 lanes, keys both ways.
+__device__ __forceinline__ int query_order(int r) { return r & 15; }
+__device__ __forceinline__ int key_order(int r) { return (r & 3) << 1 | (r >> 3 & 1) | (r >> 2 & 1) << 3; }
+__device__ __forceinline__ int value_order(int r) { return (r & 3) << 1; }
+
+// 64 x 16 bytes straight into LDS: lane i's from the buffer r at its offset, zeros outside it, to `to` + 16 i.  In
+// assembler, and with barriers that wait for no copy, so that copies stay in flight: the compiler would wait for all of
+// them at a barrier and before each transposing read.
+__device__ __forceinline__ void copy_to_lds(u4v r, unsigned off, void * to)
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+               :
+               : "v"(off), "s"(r), "s"((unsigned)(unsigned long)(lds_ptr *)to)
+               : "memory", "m0");
+#endif
+}
+__device__ __forceinline__ void wait_for_copies()
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(vm_wait(0));  // the compiler's own: it knows by it that its loads are there too
+  asm volatile("" ::: "memory");
+#endif
+}
+__device__ __forceinline__ void lds_barrier()
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#endif
+}
+
 // DK: key channels rounded up to 64, 128 or 256.  OUT: outputs and the last state; else the state that each
 // segment but the last adds to nothing, for linear_join_kernel.
 template <int TYPE, int DK, bool OUT>
@@ -168,14 +203,22 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
 {
   using T = St<TYPE>;
   typedef typename T::e E;
-  constexpr int ND = DK / 32;                              // 32-channel tiles of the state
-  constexpr int QP = DK + 8, KP = DK + 16, VP = 128 + 16, PP = kChunk + 8;  // LDS rows, in elements
-  constexpr int QI = kChunk * DK / 8 / 256, VI = kChunk * 128 / 8 / 256;     // 16-byte pieces of a thread
-  constexpr int PARTS = TYPE == kSeqBF16 ? 3 : 2;          // 16-bit parts of a value with its decay: 24 and 22 bits
-  __shared__ __attribute__((aligned(16))) E Q[OUT ? kChunk * QP : 8], K[kChunk * KP], V[kChunk * VP], P[OUT ? kChunk * PP : 8];
-  __shared__ __attribute__((aligned(16))) f2v age[2][kChunk];             // log2 of the decay since the chunk's start, as a sum of two
-  __shared__ float since[2][kChunk], left[2][kChunk], whole[2];  // that decay, from the row to the chunk's end, of all of it
-  __shared__ float unit[2][kChunk];          // fp16: what a row's scores were divided by, for each half of the keys
+  constexpr int ND = DK / 32;                      // 32-channel tiles of the state
+  constexpr int PK = DK / 8, MK = PK < 16 ? PK - 1 : 15;  // 16-byte pieces of a key row, and those that are permuted among themselves
+  constexpr int PP = kChunk + 8;                   // elements of a row of scores
+  constexpr int PARTS = TYPE == kSeqBF16 ? 3 : 2;  // 16-bit parts of a value with its decay: 24 and 22 bits
+  // Arrays of their own, so that the compiler sees which copy a read waits for.  Keys are read to the end of a chunk and
+  // have two; queries are done with, and values in registers, in the middle of it, when the next ones are asked for.
+  __shared__ __attribute__((aligned(16))) unsigned char K0[kChunk * DK * 2], K1[kChunk * DK * 2], V0[kChunk * 256];
+  __shared__ __attribute__((aligned(16))) unsigned char Q[OUT ? kChunk * DK * 2 : 16], V1[OUT ? 16 : kChunk * 256];
+  __shared__ __attribute__((aligned(16))) E P[OUT ? kChunk * PP : 8];
+  struct Decays {
+    f2v age[2][kChunk];     // log2 of the decay since the chunk's start, as a sum of two
+    float left[2][kChunk];  // the decay from the row to the chunk's end,
+    float since[2][kChunk], whole[2];  // since its start, and of all of it
+    float unit[2][kChunk];  // fp16: what a row's scores were divided by, for each half of the keys
+  };
+  __shared__ __attribute__((aligned(16))) Decays its;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
@@ -187,7 +230,7 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
   const Segment seg = segment_of(p, u);
   if (seg.s < 0 || seg.s >= seg.n || (!OUT && seg.s == seg.n - 1)) return;
   const int in = p.from ? p.from[seg.b] : -1, out = p.to ? p.to[seg.b] : -1;
-  const int n = seg.rows;
+  const int n = __builtin_amdgcn_readfirstlane(seg.rows), row0 = __builtin_amdgcn_readfirstlane(seg.row);
   const long one = (long)p.key_dim * p.dim;
   const int ch0 = block * 128 + 32 * wave;      // this wave's value channels
   const bool on = ch0 < p.dim;
@@ -195,23 +238,111 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
   float * first = p.ws + ((long)u * p.heads + h) * one;
 
   f16v s[ND];
-  auto state_io = [&](float * at, auto store) __attribute__((always_inline)) {
+  auto state_io = [&](float * at, auto store) __attribute__((always_inline)) {  // channels that are not there: zeros, nowhere
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(at, (short)0, (int)(one * 4), kBufDword3);
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
         const int dk = 32 * d + result_row(v, half);
-        if (store) {
-          if (dk < p.key_dim && dv < p.dim) at[(unsigned)(dk * p.dim + dv)] = s[d][v];
-        } else {
-          const float x = at[(unsigned)(min(dk, p.key_dim - 1) * p.dim + min(dv, p.dim - 1))];
-          s[d][v] = dk < p.key_dim && dv < p.dim ? x : 0.0f;
-        }
+        const unsigned off = dv < p.dim ? (unsigned)(dk * p.dim + dv) * 4u : kBufOOB;  // rows from key_dim on lie behind the end
+        const float x = s[d][v];  // by itself: a bit cast of an element is one of the vector's start
+        if (store) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x), r, (int)off, 0, 0);
+        else s[d][v] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, (int)off, 0, 0));
       }
   };
   constexpr std::integral_constant<bool, true> store{};
   constexpr std::integral_constant<bool, false> load{};
-  auto begin = [&]() __attribute__((always_inline)) {
+  constexpr std::integral_constant<int, 0> even{};
+  constexpr std::integral_constant<int, 1> odd_one{};
+
+  const E * q = static_cast<const E *>(p.q) + (long)row0 * p.q_token + (long)kh * p.q_head;
+  const E * k = static_cast<const E *>(p.k) + (long)row0 * p.k_token + (long)kh * p.k_head;
+  const E * v = static_cast<const E *>(p.v) + (long)row0 * p.v_token + (long)h * p.v_head + block * 128;
+  const float * g = p.g + (long)row0 * p.g_token + (long)h * p.g_head;
+  E * o = static_cast<E *>(p.o) + (long)row0 * p.o_token + (long)h * p.o_head + ch0;
+  const int chunks = (n + kChunk - 1) / kChunk, width = min(128, p.dim - block * 128);
+
+  // what this lane copies: position pos of a row holds a piece of it; channels and rows that are not there become zeros
+  auto copy = [&](const E * at, long token, int channels, int c, auto pieces, auto order, unsigned char * to) __attribute__((always_inline)) {
+    const int rows = min(n - c * kChunk, kChunk);
+    const unsigned bytes = (unsigned)((rows - 1) * (int)token + channels) * 2u;
+    const unsigned long base = reinterpret_cast<unsigned long>(at + (long)c * kChunk * token);
+    const u4v r = {(unsigned)__builtin_amdgcn_readfirstlane((int)base), (unsigned)__builtin_amdgcn_readfirstlane((int)(base >> 32)),
+                   (unsigned)__builtin_amdgcn_readfirstlane((int)bytes), (unsigned)kBufDword3};
+#pragma unroll
+    for (int i = 0; i < pieces / 4; ++i) {
+      const int at16 = 64 * (wave + 4 * i) + lane, row = at16 / pieces, ch = (at16 % pieces ^ order(row)) * 8;
+      const unsigned off = ch < channels ? (unsigned)(row * (int)token + ch) * 2u : kBufOOB;
+      copy_to_lds(r, off, to + 1024 * (wave + 4 * i));
+    }
+  };
+  constexpr std::integral_constant<int, PK> key_pieces{};
+  constexpr std::integral_constant<int, 16> value_pieces{};
+  auto copy_q = [&](int c) __attribute__((always_inline)) { copy(q, p.q_token, p.key_dim, c, key_pieces, [](int r) { return query_order(r) & MK; }, Q); };
+  auto copy_k = [&](int c, auto side) __attribute__((always_inline)) {
+    copy(k, p.k_token, p.key_dim, c, key_pieces, [](int r) { return key_order(r) & MK; }, side == 0 ? K0 : K1);
+  };
+  auto copy_v = [&](int c, auto side) __attribute__((always_inline)) {
+    copy(v, p.v_token, width, c, value_pieces, [](int r) { return value_order(r); }, side == 0 ? V0 : V1);
+  };
+
+  // Decays of chunk c, by one wave, a row a lane: sums of logarithms in 64 bits, since slow decays add up over thousands
+  // of tokens and differences are taken.  A decay below 2^-256 is 0 whatever it multiplies.
+  double total = 0.0;
+  auto ask_decay = [&](int c) { return g[(long)min(c * kChunk + lane, n - 1) * p.g_token]; };
+  auto decays = [&](int c, float log_decay) __attribute__((always_inline)) {
+    double x = c * kChunk + lane < n ? (double)log_decay * 1.4426950408889634 : 0.0;
+    x = x < -256.0 ? -256.0 : x;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const double y = __shfl_up(x, d);
+      if (lane >= d) x += y;
+    }
+    const double end = __shfl(x, 63);
+    const float hi = (float)x;
+    its.age[c & 1][lane] = f2v{hi, (float)(x - (double)hi)};
+    its.since[c & 1][lane] = (float)exp2(x);
+    its.left[c & 1][lane] = (float)exp2(end - x);
+    if (lane == 0) its.whole[c & 1] = (float)exp2(end);
+    total += end;
+  };
+
+  // LDS byte offsets of this lane's fragments: of channels 16 i + 8 half of a row, whose permuted bits an exclusive or
+  // sets, and of transposed operands: 4 rows of 16 lanes, runs in the order of turned()
+  const int krow = turned(col), run = (lane & 1) << 1 | (lane >> 1 & 1), tr = lane >> 2 & 3, side16 = lane >> 4 & 1;
+  const unsigned qat = (unsigned)(col * DK * 2 + ((half ^ query_order(col)) & MK) * 16);
+  const unsigned kat = (unsigned)(krow * DK * 2 + ((half ^ key_order(krow)) & MK) * 16);
+  const unsigned ktr = (unsigned)((8 * half + tr) * DK * 2 + (((2 * side16 + (run >> 1)) ^ key_order(8 * half + tr)) & MK) * 16 + (run & 1) * 8);
+  const unsigned vtr = (unsigned)((8 * half + tr) * 256 + ((4 * wave + 2 * side16 + (run >> 1)) ^ value_order(tr)) * 16 + (run & 1) * 8);
+  auto piece = [&](const unsigned char * rows, unsigned at, int i) __attribute__((always_inline)) {  // i: 32-byte steps
+    return *reinterpret_cast<const u4v *>(rows + (at ^ (unsigned)(2 * i & MK) * 16u) + (unsigned)(2 * i & ~MK) * 16u);
+  };
+  // 16 tokens from 16 j on of channels 32 d ..
+  auto keys_of = [&](const unsigned char * rows, int j, int d) __attribute__((always_inline)) {
+    const unsigned low = (unsigned)(4 * d & MK) * 16u, high = (unsigned)(4 * d & ~MK) * 16u, flip = (unsigned)(8 & MK) * 16u;
+    const u2v x = read_transposed(rows + (ktr ^ low) + high + 16 * j * DK * 2), y = read_transposed(rows + (ktr ^ low ^ flip) + high + (16 * j + 4) * DK * 2);
+    return u4v{x[0], x[1], y[0], y[1]};
+  };
+  auto values_of = [&](const unsigned char * rows, int j) __attribute__((always_inline)) {
+    const u2v x = read_transposed(rows + vtr + 16 * j * 256), y = read_transposed(rows + vtr + (16 * j + 4) * 256);
+    return u4v{x[0], x[1], y[0], y[1]};
+  };
+
+  // of the chunk after next, asked for before the next one's rows: they are there when those are
+  float next_decay = 0.0f;
+  if (chunks > 0) {
+    float log_decay = 0.0f;
+    if (wave == 3) {
+      log_decay = ask_decay(0);
+      next_decay = ask_decay(1);
+    }
+    copy_k(0, even);
+    if (OUT) copy_q(0);
+    copy_v(0, even);
+    if (wave == 3) decays(0, log_decay);
+  }
+  if (on) {
     if (OUT && seg.n > 1) {
       state_io(first, load);
     } else if (seg.s == 0 && (unsigned)in < (unsigned)p.slots) {
@@ -222,142 +353,70 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
 #pragma unroll
         for (int v = 0; v < 16; ++v) s[d][v] = 0.0f;
     }
-  };
-  if (on) begin();
-  if (!OUT && seg.s == 0 && on) state_io(first, store);  // the slot may be written while other segments run
-
-  const E * q = static_cast<const E *>(p.q) + (long)seg.row * p.q_token + (long)kh * p.q_head;
-  const E * k = static_cast<const E *>(p.k) + (long)seg.row * p.k_token + (long)kh * p.k_head;
-  const E * v = static_cast<const E *>(p.v) + (long)seg.row * p.v_token + (long)h * p.v_head + block * 128;
-  const float * g = p.g + (long)seg.row * p.g_token + (long)h * p.g_head;
-  E * o = static_cast<E *>(p.o) + (long)seg.row * p.o_token + (long)h * p.o_head + ch0;
-  const int chunks = (n + kChunk - 1) / kChunk;
-
-  u4v qr[QI], kr[QI], vr[VI];
-  auto ask = [&](int c) __attribute__((always_inline)) {  // rows that are not there read the last one
-#pragma unroll
-    for (int i = 0; i < QI; ++i) {
-      const int piece = tid + 256 * i, row = min(c * kChunk + piece / (DK / 8), n - 1), ch = min(piece % (DK / 8) * 8, p.key_dim - 8);
-      if (OUT) qr[i] = *reinterpret_cast<const u4v *>(q + (long)row * p.q_token + ch);
-      kr[i] = *reinterpret_cast<const u4v *>(k + (long)row * p.k_token + ch);
-    }
-#pragma unroll
-    for (int i = 0; i < VI; ++i) {
-      const int piece = tid + 256 * i, row = min(c * kChunk + piece / 16, n - 1), ch = min(piece % 16 * 8, p.dim - 8 - block * 128);
-      vr[i] = *reinterpret_cast<const u4v *>(v + (long)row * p.v_token + ch);
-    }
-  };
-  auto put = [&](int c) __attribute__((always_inline)) {
-    const u4v zero = {0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < QI; ++i) {
-      const int piece = tid + 256 * i, row = piece / (DK / 8), ch = piece % (DK / 8) * 8;
-      const bool there = c * kChunk + row < n && ch < p.key_dim;
-      if (OUT) *reinterpret_cast<u4v *>(Q + row * QP + ch) = there ? qr[i] : zero;
-      *reinterpret_cast<u4v *>(K + row * KP + ch) = there ? kr[i] : zero;
-    }
-#pragma unroll
-    for (int i = 0; i < VI; ++i) {
-      const int piece = tid + 256 * i, row = piece / 16, ch = piece % 16 * 8;
-      *reinterpret_cast<u4v *>(V + row * VP + ch) = c * kChunk + row < n && block * 128 + ch < p.dim ? vr[i] : zero;
-    }
-  };
-  // Decays of chunk c, by one wave, a row a lane: sums of logarithms in 64 bits, since slow decays add up over thousands
-  // of tokens and differences are taken.  A decay below 2^-256 is 0 whatever it multiplies.
-  double total = 0.0;
-  auto ask_decay = [&](int c) { return g[(long)min(c * kChunk + lane, n - 1) * p.g_token]; };
-  auto decays = [&](int c, float its) __attribute__((always_inline)) {
-    double x = c * kChunk + lane < n ? (double)its * 1.4426950408889634 : 0.0;
-    x = x < -256.0 ? -256.0 : x;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const double y = __shfl_up(x, d);
-      if (lane >= d) x += y;
-    }
-    const double end = __shfl(x, 63);
-    const float hi = (float)x;
-    age[c & 1][lane] = f2v{hi, (float)(x - (double)hi)};
-    since[c & 1][lane] = (float)exp2(x);
-    left[c & 1][lane] = (float)exp2(end - x);
-    if (lane == 0) whole[c & 1] = (float)exp2(end);
-    total += end;
-  };
-
-  // LDS offsets of this lane's pieces of transposed operands: 4 rows of 16 lanes, runs in the order of turned()
-  const int run = 16 * (lane >> 4 & 1) + 4 * ((lane & 1) << 1 | (lane >> 1 & 1)), tr = 8 * half + (lane >> 2 & 3);
-  const E * kt = K + tr * KP + run;
-  const E * vt = V + tr * VP + 32 * wave + run;
-
-  // of the chunk after next, asked for before the next one's rows: they are there when those are
-  float next_decay = 0.0f;
-  if (chunks > 0) {
-    if (wave == 3) {
-      const float its = ask_decay(0);
-      next_decay = ask_decay(1);
-      decays(0, its);
-    }
-    ask(0);
+    if (!OUT && seg.s == 0) state_io(first, store);  // the slot may be written while other segments run
   }
-  for (int c = 0; c < chunks; ++c) {
-    put(c);
-    __syncthreads();
-    const float its_decay = next_decay;
-    if (c + 1 < chunks) {
+  wait_for_copies();
+  lds_barrier();
+
+  auto chunk = [&](int c, auto side) __attribute__((always_inline)) {
+    constexpr int SIDE = decltype(side)::value;
+    constexpr std::integral_constant<int, 1 - SIDE> other{};
+    const unsigned char * K = SIDE == 0 ? K0 : K1;
+    const bool more = c + 1 < chunks;
+    const float decay_then = next_decay;
+    if (more) {
       if (wave == 3) next_decay = ask_decay(c + 2);
-      ask(c + 1);
+      copy_k(c + 1, other);
+      if (!OUT) copy_v(c + 1, other);
     }
     f16v acc[2];
     float fit = 1.0f;  // fp16: the state's power of two
     auto from_state = [&]() __attribute__((always_inline)) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int x = 0; x < 16; ++x) acc[t][x] = 0.0f;
+      for (int t = 0; t < 2; ++t) acc[t] = f16v{};
 #pragma unroll
       for (int i = 0; i < 2 * ND; ++i) {
-        u4v hi, lo;
+        u4v part[2];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           unsigned y[2];
           split<TYPE>(f2v{s[i / 2][8 * (i % 2) + 2 * x], s[i / 2][8 * (i % 2) + 2 * x + 1]}, f2v{fit, fit}, y);
-          hi[x] = y[0];
-          lo[x] = y[1];
+          part[0][x] = y[0];
+          part[1][x] = y[1];
         }
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const u4v y = *reinterpret_cast<const u4v *>(Q + (32 * t + col) * QP + 16 * i + 8 * half);
-          acc[t] = T::mma32(hi, y, acc[t]);
-          acc[t] = T::mma32(lo, y, acc[t]);
-        }
+        const u4v y0 = piece(Q, qat, i), y1 = piece(Q + 32 * DK * 2, qat, i);
+        acc[0] = T::mma32(part[0], y0, acc[0]);
+        acc[1] = T::mma32(part[0], y1, acc[1]);
+        acc[0] = T::mma32(part[1], y0, acc[0]);
+        acc[1] = T::mma32(part[1], y1, acc[1]);
       }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const float f = since[c & 1][32 * t + col] / fit;
+        const float f = its.since[SIDE][32 * t + col] / fit;
 #pragma unroll
         for (int x = 0; x < 16; ++x) acc[t][x] *= f;
       }
     };
+    u4v vf[4], y[4];
+    unsigned odd_row = kChunk;
+    bool odd = false;
     if constexpr (OUT) {
       // scores of a 32 x 32 part, keys in rows; of those above the diagonal none
       if (wave < 3) {
         const int t0 = wave ? 32 : 0, s0 = wave == 2 ? 32 : 0;
-        f16v x;
+        f16v x = {};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 2 * ND; ++i)
-          x = T::mma32(*reinterpret_cast<const u4v *>(K + (s0 + turned(col)) * KP + 16 * i + 8 * half),
-                       *reinterpret_cast<const u4v *>(Q + (t0 + col) * QP + 16 * i + 8 * half), x);
-        const f2v mine = age[c & 1][t0 + col];
+        for (int i = 0; i < 2 * ND; ++i) x = T::mma32(piece(K + s0 * DK * 2, kat, i), piece(Q + t0 * DK * 2, qat, i), x);
+        const f2v mine = its.age[SIDE][t0 + col];
         float most = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
           const int row = s0 + result_row(i, half);
-          const f4v its = *reinterpret_cast<const f4v *>(&age[c & 1][row]);
+          const f4v key = *reinterpret_cast<const f4v *>(&its.age[SIDE][row]);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const bool seen = row + e <= t0 + col;
-            const float decay = __builtin_amdgcn_exp2f(seen ? (mine[0] - its[2 * e]) + (mine[1] - its[2 * e + 1]) : -200.0f);
+            const float decay = __builtin_amdgcn_exp2f(seen ? (mine[0] - key[2 * e]) + (mine[1] - key[2 * e + 1]) : -200.0f);
             x[i + e] = (seen ? x[i + e] : 0.0f) * decay;
             if (TYPE == kSeqF16) most = fmaxf(most, fabsf(x[i + e]));
           }
@@ -367,7 +426,7 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
           const int e = min(max(__builtin_amdgcn_frexp_expf(most) - 14, -40), 60);
 #pragma unroll
           for (int i = 0; i < 16; ++i) x[i] = __builtin_ldexpf(x[i], -e);
-          if (half == 0) unit[s0 / 32][t0 + col] = __builtin_ldexpf(1.0f, e);
+          if (half == 0) its.unit[s0 / 32][t0 + col] = __builtin_ldexpf(1.0f, e);
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -376,9 +435,9 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
                   pack2<TYPE>(x[8 * i + 6], x[8 * i + 7])};
       }
     }
-    if (wave == 3 && c + 1 < chunks) decays(c + 1, its_decay);
-    if constexpr (OUT) {
-      if (on) {
+    if (wave == 3 && more) decays(c + 1, decay_then);
+    if (on) {
+      if constexpr (OUT) {
         if constexpr (TYPE == kSeqF16) {
           float most = 0.0f;
 #pragma unroll
@@ -386,78 +445,84 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
 #pragma unroll
             for (int x = 0; x < 16; ++x) most = fmaxf(most, fabsf(s[d][x]));
 #pragma unroll
-          for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
+          for (int d = 1; d < 16; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
+          most = across16(across32(most, MaxOp()), MaxOp());
           fit = __builtin_ldexpf(1.0f, min(max(14 - __builtin_amdgcn_frexp_expf(most), -100), 100));
         }
         from_state();
       }
-      __syncthreads();
-    }
-    u4v vf[4];
-    if (on) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const u2v a = read_transposed(vt + 16 * j * VP), b = read_transposed(vt + (16 * j + 4) * VP);
-        vf[j] = u4v{a[0], a[1], b[0], b[1]};
-      }
+      for (int j = 0; j < 4; ++j) vf[j] = values_of(SIDE && !OUT ? V1 : V0, j);
     }
     if constexpr (OUT) {
+      // An infinity or NaN among the values would reach earlier rows of the chunk as 0 times it: left out of the product
+      // it makes NaN of its channel from its row on, and of the state's.
+      if (on) {
+        typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+        us2 most = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) most = __builtin_elementwise_max(most, __builtin_bit_cast(us2, vf[j][x] & 0x7fff7fffu));
+        if (__any(T::odd_bits(__builtin_bit_cast(unsigned, most)) != 0)) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const unsigned bad = T::odd_bits(vf[j][x]), at = 16 * j + 8 * half + 2 * x;
+              if (bad) odd_row = min(odd_row, bad & 0x8000u ? at : at + 1);
+              vf[j][x] &= ~((bad >> 15) * 0xffffu);
+            }
+          odd_row = min(odd_row, (unsigned)__shfl_xor((int)odd_row, 32));
+          odd = true;
+        }
+      }
+      lds_barrier();
       if (on) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           float back = 1.0f;
 #pragma unroll
-          for (int y = 0; y <= t; ++y) {  // halves of the keys
+          for (int z = 0; z <= t; ++z) {  // halves of the keys
             if constexpr (TYPE == kSeqF16) {
-              const float mine = unit[y][32 * t + col], f = back / mine;
+              const float mine = its.unit[z][32 * t + col], f = back / mine;
 #pragma unroll
               for (int x = 0; x < 16; ++x) acc[t][x] *= f;
               back = mine;
             }
 #pragma unroll
-            for (int j = 2 * y; j < 2 * y + 2; ++j)
+            for (int j = 2 * z; j < 2 * z + 2; ++j)
               acc[t] = T::mma32(vf[j], *reinterpret_cast<const u4v *>(P + (32 * t + col) * PP + 16 * j + 8 * half), acc[t]);
           }
           if constexpr (TYPE == kSeqF16)
 #pragma unroll
             for (int x = 0; x < 16; ++x) acc[t][x] *= back;
         }
-        // An infinity or NaN among the values reaches earlier rows of the chunk as 0 times it.  If a result is not
-        // finite, the chunk's part is summed again over the keys that a row sees.
-        bool odd = false;
+      }
+      if (odd) {
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          const unsigned from = (unsigned)__shfl((int)odd_row, turned(result_row(x, half)));
+#pragma unroll
+          for (int t = 0; t < 2; ++t) acc[t][x] = 32u * t + col >= from ? __builtin_nanf("") : acc[t][x];
+        }
+      }
+      if (more) {
+        copy_q(c + 1);
+        copy_v(c + 1, even);
+      }
+      if (on) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int x = 0; x < 16; ++x) odd = odd || !(fabsf(acc[t][x]) < __builtin_inff());
-        if (__any(odd)) {
-          from_state();
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
-            for (int y = 0; y <= 32 * t + col; ++y) {
-              float z = (float)P[(32 * t + col) * PP + y];
-              if (TYPE == kSeqF16) z *= unit[y / 32][32 * t + col];
-#pragma unroll
-              for (int x = 0; x < 16; ++x) acc[t][x] = fmaf(z, (float)V[y * VP + 32 * wave + result_row(x, half)], acc[t][x]);
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int row = c * kChunk + 32 * t + col;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (row >= n || ch0 + 16 * i + 8 * half >= p.dim) continue;
-            float y[8];
-#pragma unroll
-            for (int x = 0; x < 8; ++x) y[x] = acc[t][8 * i + x] * p.scale;
-            *reinterpret_cast<u4v *>(o + (long)row * p.o_token + 16 * i + 8 * half) =
-                u4v{pack2<TYPE>(y[0], y[1]), pack2<TYPE>(y[2], y[3]), pack2<TYPE>(y[4], y[5]), pack2<TYPE>(y[6], y[7])};
-          }
-        }
+            for (int x = 0; x < 4; ++x) y[2 * t + i][x] = pack2<TYPE>(acc[t][8 * i + 2 * x] * p.scale, acc[t][8 * i + 2 * x + 1] * p.scale);
       }
     }
     // the state: values with their decays to the chunk's end in parts of 16 bits, which together have fp32's precision
     if (on) {
-      const float a = whole[c & 1];
+      const float a = its.whole[SIDE];
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -465,34 +530,50 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         u4v part[PARTS];
+        const f4v l0 = *reinterpret_cast<const f4v *>(&its.left[SIDE][16 * j + 8 * half]), l1 = *reinterpret_cast<const f4v *>(&its.left[SIDE][16 * j + 8 * half + 4]);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const int row = 16 * j + 8 * half + 2 * x;
-          unsigned y[PARTS];
-          split<TYPE>(unpack2<TYPE>(vf[j][x]), f2v{left[c & 1][row], left[c & 1][row + 1]}, y);
+          unsigned z[PARTS];
+          split<TYPE>(unpack2<TYPE>(vf[j][x]), x < 2 ? f2v{l0[2 * x], l0[2 * x + 1]} : f2v{l1[2 * x - 4], l1[2 * x - 3]}, z);
 #pragma unroll
-          for (int i = 0; i < PARTS; ++i) part[i][x] = y[i];
+          for (int i = 0; i < PARTS; ++i) part[i][x] = z[i];
         }
+        u4v kf[ND];
 #pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          const u2v a = read_transposed(kt + 16 * j * KP + 32 * d), b = read_transposed(kt + (16 * j + 4) * KP + 32 * d);
-          const u4v x = {a[0], a[1], b[0], b[1]};
+        for (int d = 0; d < ND; ++d) kf[d] = keys_of(K, j, d);
 #pragma unroll
-          for (int i = 0; i < PARTS; ++i) s[d] = T::mma32(x, part[i], s[d]);
-        }
+        for (int i = 0; i < PARTS; ++i)
+#pragma unroll
+          for (int d = 0; d < ND; ++d) s[d] = T::mma32(kf[d], part[i], s[d]);
+      }
+      if (OUT && odd && odd_row < (unsigned)kChunk)
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) s[d][x] = __builtin_nanf("");
+    }
+    wait_for_copies();  // the next chunk's rows; outputs go behind them and are waited for a chunk later
+    if (OUT && on) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int row = c * kChunk + 32 * t + col;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (row < n && ch0 + 16 * i + 8 * half < p.dim) *reinterpret_cast<u4v *>(o + (long)row * p.o_token + 16 * i + 8 * half) = y[2 * t + i];
       }
     }
-    __syncthreads();
+    lds_barrier();
+  };
+  for (int c = 0; c < chunks; c += 2) {
+    chunk(c, even);
+    if (c + 1 < chunks) chunk(c + 1, odd_one);
   }
-  if (!on) {
-    if (!OUT && wave == 3 && lane == 0 && block == 0) p.decay[(long)u * p.heads + h] = (float)exp2(total);
-    return;
-  }
+  if (!OUT && wave == 3 && lane == 0 && block == 0) p.decay[(long)u * p.heads + h] = (float)exp2(total);
+  if (!on) return;
   if constexpr (OUT) {
     if (seg.s == seg.n - 1 && (unsigned)out < (unsigned)p.slots) state_io(p.state + ((long)out * p.heads + h) * one, store);
   } else {
     state_io(first + (long)p.heads * one, store);
-    if (wave == 3 && lane == 0 && block == 0) p.decay[(long)u * p.heads + h] = (float)exp2(total);
   }
 }
 
@@ -552,17 +633,25 @@ template <int TYPE> void launch_linear_type(const LinearParams & p, hipStream_t 
 
 size_t linear_split(LinearParams & p, int max_new)
 {
+  // token by token a state is read and written once as well, and 16 tokens of it cost less than a chunk's start
   p.seg = 0;
   if (max_new <= 16) return 0;
-  const long blocks = (p.dim + 127) / 128;
-  const long each = (long)p.tokens * p.heads * blocks / 512;
-  p.seg = (int)((std::max<long>(each, 512) + kChunk - 1) / kChunk * kChunk);
-  if (max_new <= 2 * p.seg) {
-    p.seg = (max_new + kChunk - 1) / kChunk * kChunk;
-    p.seg = kMaxSeg;
-    return 0;
+  // Rounds of work-groups, two a CU (one above 128 key channels), times the tokens of each, for sequences of the same length
+  // or the longest one.  Segments cost a second pass over keys and values, and their first states.
+  const long cap = p.key_dim <= 128 ? 512 : 256, wgs = (long)p.heads * ((p.dim + 127) / 128), mean = std::max(1, p.tokens / p.batch);
+  auto rounds = [&](long units) { return (units * wgs + cap - 1) / cap; };
+  const long whole = std::max(rounds(p.batch) * mean, (long)max_new);
+  long best = 0, cost = whole * 10 / 17;
+  for (long seg = 256; seg < max_new; seg += kChunk) {
+    const long c = rounds(p.batch * ((mean + seg - 1) / seg)) * seg;
+    if (c < cost || (best > 0 && c == cost)) {
+      best = seg;
+      cost = c;
+    }
+    if (seg > cost) break;
   }
-  return ((size_t)p.tokens / p.seg + p.batch) * p.heads * ((size_t)p.key_dim * p.dim + 1) * sizeof(float);
+  p.seg = best ? (int)best : kMaxSeg;
+  return best ? ((size_t)p.tokens / p.seg + p.batch) * p.heads * ((size_t)p.key_dim * p.dim + 1) * sizeof(float) : 0;
 }
 
 void launch_linear_attention(const LinearParams & p, hipStream_t s)

@@ -467,6 +467,7 @@ int ivh_linear_attention(const ivh_linear_attn_desc * d, const void * q, const v
       check_rows(o, d->o_token, d->o_head, 8, "attention output");
       check_apart(tokens, d->heads, d->dim, d->o_token, d->o_head, "attention");
       need(g, "null decays");
+      need(d->q_token < (1 << 23) && d->k_token < (1 << 23) && d->v_token < (1 << 23), "query, key and value rows must lie less than 2^23 elements apart");
     }
     need(cu, "null sequence offsets");
     need((reinterpret_cast<uintptr_t>(cu) | reinterpret_cast<uintptr_t>(from) | reinterpret_cast<uintptr_t>(to) |
