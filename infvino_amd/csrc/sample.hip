@@ -1,11 +1,25 @@
 // The next token of each row of logits: temperature, top-k, top-p, min-p, and the inverse of what is left
 // at a given random number, on gfx950.
 //
-// Weights w = exp((x - max) / T) are whole multiples of 2^-44: their sums over up to 2^19 tokens fit in
+// Weights w = 2^z, z = (x - max) log2 e / T, are whole multiples of 2^-44: their sums over up to 2^19 tokens fit in
 // 63 bits and are the same in any order, so cuts and draws do not depend on how a row is split, and no atomic's
-// order can change a token.  A weight below 2^-45 of the largest is 0.  The exponential is formed in 64 bits to 2^-50.
+// order can change a token.  What lies 45 powers of two below the largest is out.  Exponentials are formed in 64 bits.
+//
+// Every filter keeps a leading part of the descending order (equal logits by index), so that all of them together are one
+// cut, a code of a logit and how many of those that equal it are in, and nothing is sorted.  Rows of up to 8192 tokens
+// stay in the registers of one work-group.  Longer ones are read three times in pieces of 4096 tokens, by as many
+// work-groups as fill the chip:
+//   1. the largest logit of each part;
+//   2. counts and sums of weights in 256 bins of z, 8 to a power of two down to 2^-28 (rows with top-k or top-p alone);
+//   3. the bins say in which of them the cut lies: sums of what is surely kept for each piece, and a list
+//      of the tokens of those bins;
+// and a last kernel, a work-group a row, finds the cut among the listed ones by digits of their codes, adds
+// them to their pieces' sums, and reads the one piece that u falls in.  Where more than 8192 tokens fall into those
+// bins, as in rows of equal logits, it reads the row itself instead.
+#include <algorithm>
 #include <cmath>
 #include <stdexcept>
+#include <type_traits>
 
 #include "conv_common.hpp"
 #include "seq_common.hpp"
@@ -16,9 +30,15 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kThreads = 1024;
-constexpr double kOne = 17592186044416.0;  // 2^44, the largest weight
-constexpr u64 kAll = 1ull << 63;           // no sum is larger
+constexpr int kPiece = 4096;      // tokens of a piece
+constexpr int kMaxPieces = 128;   // of a row
+constexpr int kList = 8192;       // listed tokens of a row, and tokens of a row that one work-group keeps
+constexpr int kBins = 256;
+constexpr int kThreads = 256;     // of the kernels over pieces
+constexpr int kLast = 1024;       // of the last kernel
+constexpr u64 kOne = 1ull << 44;  // the largest weight
+constexpr u64 kAll = 1ull << 63;  // no sum is larger
+constexpr unsigned kNone = 0x007fffffu;  // code of -infinity
 
 template <int TYPE> struct Logit;
 template <> struct Logit<kSeqF16> { typedef _Float16 e; };
@@ -33,17 +53,419 @@ __device__ __forceinline__ unsigned code_of(float x)
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(unsigned code) { return __builtin_bit_cast(float, code & 0x80000000u ? code & 0x7fffffffu : ~code); }
-constexpr unsigned kNone = 0x007fffffu;  // of -infinity
 
-// the weight of a token in units of 2^-44; scale: log2 e / T in 64 bits
+// z of a token; not above -45 if it has no weight
+__device__ __forceinline__ double power_of(unsigned code, unsigned top, double scale)
+{
+  const double z = ((double)value_of(code) - (double)value_of(top)) * scale;
+  return code == top ? 0.0 : code <= kNone ? -1000.0 : z;
+}
+// 2^z in units of 2^-44, z in (-45, 0]: Taylor's polynomial of e^t, |t| <= log 2 / 2, off by 2^-52 before rounding; adding
+// 2^52 leaves the nearest whole number in a double's low bits
+__device__ __forceinline__ u64 weight_at(double z)
+{
+  const double n = rint(z), t = (z - n) * 0.693147180559945309;
+  double y = 1.0 / 6227020800.0;
+  constexpr double c[] = {1.0 / 479001600.0, 1.0 / 39916800.0, 1.0 / 3628800.0, 1.0 / 362880.0, 1.0 / 40320.0, 1.0 / 5040.0,
+                          1.0 / 720.0, 1.0 / 120.0, 1.0 / 24.0, 1.0 / 6.0, 0.5, 1.0, 1.0};
+#pragma unroll
+  for (int i = 0; i < 13; ++i) y = fma(y, t, c[i]);
+  const double w = __builtin_amdgcn_ldexp(y, (int)n + 44) + 4503599627370496.0;
+  return max(__builtin_bit_cast(u64, w) & 0xfffffffffffffull, 1ull);
+}
 __device__ __forceinline__ u64 weight_of(unsigned code, unsigned top, double scale)
 {
-  if (code == top) return (u64)kOne;
-  if (code <= kNone) return 0;
-  const double z = ((double)value_of(code) - (double)value_of(top)) * scale;
-  if (!(z > -46.0)) return 0;
-  return (u64)rint(exp2(z) * kOne);
+  const double z = power_of(code, top, scale);
+  return z > -45.0 ? weight_at(z) : 0;
 }
+// bin of a power in (-45, 0], the largest first; does not decrease as z falls
+__device__ __forceinline__ int bin_of(double z)
+{
+  const float a = -(float)z;
+  return a < 28.0f ? (int)(a * 8.0f) : min(224 + (int)((a - 28.0f) * 1.9f), kBins - 1);
+}
+
+// What a row asks for.
+struct Filters {
+  float t;
+  int k;
+  float p;
+  u64 least;  // the smallest weight that min-p keeps
+  bool has_k, has_p;
+};
+__device__ __forceinline__ Filters filters_of(const SampleParams & s, int row)
+{
+  Filters f;
+  f.t = s.temperature ? s.temperature[row] : 1.0f;
+  f.k = s.top_k ? s.top_k[row] : 0;
+  f.p = s.top_p ? s.top_p[row] : 1.0f;
+  const float m = s.min_p ? s.min_p[row] : 0.0f;
+  f.least = m > 0.0f ? max((u64)ceil((double)fminf(m, 1.0f) * (double)kOne), 1ull) : 1;
+  f.has_k = f.k > 0 && f.k < s.vocab;
+  f.has_p = f.p < 1.0f;
+  return f;
+}
+__device__ __forceinline__ double scale_of(float t) { return 1.4426950408889634 / (double)t; }
+// the fewest units that reach p of a sum
+__device__ __forceinline__ u64 share_of(float p, u64 sum) { return max((u64)ceil(fmax((double)p, 0.0) * (double)sum), 1ull); }
+
+// What the kernels over pieces leave for the last one.
+struct RowHead {
+  unsigned listed;    // tokens in the list
+  unsigned first;     // bins before it are kept
+  unsigned mode;
+  unsigned deep;      // the sum of the top k is known from the listed tokens alone
+  u64 before_n, before_s, need_s;  // of the bins before; the sum that top-p asks for, unless deep
+};
+enum Mode : unsigned { kNoCut, kCutListed, kCutLong };
+
+// A row's part of the workspace.
+struct RowSpace {
+  uint2 * list;     // [kList] codes and indexes
+  u64 * bin_sum;    // [parts][kBins]
+  u64 * piece;      // [pieces] sums of what is surely kept
+  RowHead * head;
+  uint2 * top;      // [parts] largest code and its first index
+  unsigned * bin_n; // [parts][kBins]
+};
+__device__ __host__ __forceinline__ size_t row_bytes(int parts, int pieces)
+{
+  return ((size_t)kList * 8 + (size_t)parts * (12 * kBins + 8) + (size_t)pieces * 8 + sizeof(RowHead) + 255) / 256 * 256;
+}
+__device__ __forceinline__ RowSpace space_of(const SampleParams & s, int row)
+{
+  RowSpace r;
+  r.list = reinterpret_cast<uint2 *>(static_cast<char *>(s.ws) + (size_t)row * row_bytes(s.parts, s.pieces));
+  r.bin_sum = reinterpret_cast<u64 *>(r.list + kList);
+  r.piece = r.bin_sum + s.parts * kBins;
+  r.head = reinterpret_cast<RowHead *>(r.piece + s.pieces);
+  r.top = reinterpret_cast<uint2 *>(r.head + 1);
+  r.bin_n = reinterpret_cast<unsigned *>(r.top + s.parts);
+  return r;
+}
+
+// the largest code with its first index, over a wave
+__device__ __forceinline__ void wave_top(unsigned & code, unsigned & at)
+{
+#pragma unroll
+  for (int d = 32; d >= 1; d /= 2) {
+    const unsigned c = __shfl_xor(code, d), j = __shfl_xor(at, d);
+    if (c > code || (c == code && j < at)) {
+      code = c;
+      at = j;
+    }
+  }
+}
+__device__ __forceinline__ void row_top(const RowSpace & r, int parts, unsigned & code, unsigned & at)
+{
+  code = 0;
+  at = 0xffffffffu;
+  for (int i = threadIdx.x & 63; i < parts; i += 64) {
+    const uint2 x = r.top[i];
+    if (x.x > code || (x.x == code && x.y < at)) {
+      code = x.x;
+      at = x.y;
+    }
+  }
+  wave_top(code, at);
+}
+
+// The smallest code whose token lies in a bin before `bin`, by a 64-wide search of one wave.
+__device__ __forceinline__ unsigned code_before(int bin, unsigned top, double scale)
+{
+  const unsigned lane = threadIdx.x & 63;
+  unsigned low = 0, width = top;  // the code is in [low, low + width]: that of the largest is in bin 0
+  if (bin <= 0) return 0xffffffffu;
+  while (width > 0) {
+    const unsigned step = width / 64 + 1, c = low + min(step * lane, width);
+    const double z = power_of(c, top, scale);
+    const u64 in = __ballot(z > -45.0 && bin_of(z) < bin);
+    const unsigned i = in ? __builtin_ctzll(in) : 64;  // the first of them
+    const unsigned from = i ? min(step * (i - 1) + 1, width) : 0;
+    width = (i < 64 ? min(step * i, width) : width) - from;
+    low += from;
+  }
+  return __builtin_amdgcn_readfirstlane(low);
+}
+
+template <class T> __device__ __forceinline__ T wave_scan(T x)  // inclusive
+{
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const T y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  return x;
+}
+
+typedef u4v u4v_of_halves __attribute__((aligned(2)));
+typedef u4v u4v_of_floats __attribute__((aligned(4)));
+template <class E> __device__ __forceinline__ u4v load_any(const E * x)
+{
+  if constexpr (sizeof(E) == 2) return *reinterpret_cast<const u4v_of_halves *>(x);
+  else return *reinterpret_cast<const u4v_of_floats *>(x);
+}
+
+// The 16 tokens of a piece that a thread has: fn(i, code, index), runs of 16 bytes at any alignment, 256 threads
+// side by side.
+template <int TYPE, class Fn> __device__ __forceinline__ void each_of_piece(const typename Logit<TYPE>::e * x, int base, int n, Fn && fn)
+{
+  typedef typename Logit<TYPE>::e E;
+  constexpr int RUN = 16 / sizeof(E), RUNS = 16 / RUN;
+  const int first = base + (int)threadIdx.x * RUN;
+  if (base + kPiece <= n) {
+    u4v run[RUNS];
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i) run[i] = load_any(x + first + i * kThreads * RUN);
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const unsigned y = run[i][j];
+        const int at = first + i * kThreads * RUN + j * (RUN / 4);
+        if constexpr (TYPE == kSeqF32) {
+          fn(i * RUN + j, code_of(__builtin_bit_cast(float, y)), at);
+        } else {
+          const f2v z = unpack2<TYPE>(y);
+          fn(i * RUN + 2 * j, code_of(z[0]), at);
+          fn(i * RUN + 2 * j + 1, code_of(z[1]), at + 1);
+        }
+      }
+  } else {
+    E run[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) run[i] = x[min(first + i / RUN * kThreads * RUN + i % RUN, n - 1)];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int at = first + i / RUN * kThreads * RUN + i % RUN;
+      const unsigned code = code_of((float)run[i]);
+      fn(i, at < n ? code : 0u, at);
+    }
+  }
+}
+
+}  // namespace
+
+// 1. The largest logit of each part.
+template <int TYPE>
+__global__ void __launch_bounds__(kThreads) sample_top_kernel(const SampleParams p)
+{
+  typedef typename Logit<TYPE>::e E;
+  __shared__ unsigned code[4], at[4];
+  const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
+  const E * x = static_cast<const E *>(p.x) + (long)row * p.row;
+  const RowSpace r = space_of(p, row);
+  if (part == 0 && threadIdx.x == 0) r.head->listed = 0;
+  unsigned top = 0, first = 0xffffffffu;
+  for (int i = part * p.per; i < min(p.pieces, (part + 1) * p.per); ++i)
+    each_of_piece<TYPE>(x, i * kPiece, p.vocab, [&](int, unsigned c, int j) {
+      if (c > top) {  // a thread's indexes grow
+        top = c;
+        first = (unsigned)j;
+      }
+    });
+  wave_top(top, first);
+  if ((threadIdx.x & 63) == 0) {
+    code[threadIdx.x / 64] = top;
+    at[threadIdx.x / 64] = first;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 4; ++i)
+      if (code[i] > top || (code[i] == top && at[i] < first)) {
+        top = code[i];
+        first = at[i];
+      }
+    r.top[part] = uint2{top, first};
+  }
+}
+
+// 2. Counts and sums of each part's bins.
+template <int TYPE>
+__global__ void __launch_bounds__(kThreads) sample_bins_kernel(const SampleParams p)
+{
+  typedef typename Logit<TYPE>::e E;
+  constexpr int COPIES = 4;  // of the bins, for lanes side by side
+  __shared__ u64 sum[COPIES * (kBins + 1)];
+  __shared__ unsigned count[COPIES * (kBins + 1)];
+  const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
+  const Filters f = filters_of(p, row);
+  if (!(f.has_k || f.has_p) || !(f.t > 0.0f)) return;
+  const E * x = static_cast<const E *>(p.x) + (long)row * p.row;
+  const RowSpace r = space_of(p, row);
+  for (int i = threadIdx.x; i < COPIES * (kBins + 1); i += kThreads) {
+    sum[i] = 0;
+    count[i] = 0;
+  }
+  unsigned top, at;
+  row_top(r, p.parts, top, at);
+  const double scale = scale_of(f.t);
+  const int mine = (threadIdx.x & (COPIES - 1)) * (kBins + 1);
+  __syncthreads();
+  for (int i = part * p.per; i < min(p.pieces, (part + 1) * p.per); ++i)
+    each_of_piece<TYPE>(x, i * kPiece, p.vocab, [&](int, unsigned c, int) {
+      const double z = power_of(c, top, scale);
+      if (!(z > -45.0)) return;
+      const int b = mine + bin_of(z);
+      atomicAdd(&count[b], 1u);
+      if (f.has_p) atomicAdd(&sum[b], weight_at(z));
+    });
+  __syncthreads();
+  const int b = threadIdx.x;
+  u64 s = 0;
+  unsigned n = 0;
+#pragma unroll
+  for (int i = 0; i < COPIES; ++i) {
+    s += sum[i * (kBins + 1) + b];
+    n += count[i * (kBins + 1) + b];
+  }
+  r.bin_sum[part * kBins + b] = s;
+  r.bin_n[part * kBins + b] = n;
+}
+
+// 3. Where the cut lies; each piece's sum of what is surely kept; the tokens among which the cut is.
+template <int TYPE>
+__global__ void __launch_bounds__(kThreads) sample_list_kernel(const SampleParams p)
+{
+  typedef typename Logit<TYPE>::e E;
+  __shared__ u64 wave_s[4];
+  __shared__ unsigned wave_n[4], lowest[4][3];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
+  const Filters f = filters_of(p, row);
+  if (!(f.t > 0.0f)) return;
+  const E * x = static_cast<const E *>(p.x) + (long)row * p.row;
+  const RowSpace r = space_of(p, row);
+  unsigned top, at;
+  row_top(r, p.parts, top, at);
+  if (top <= kNone) return;
+  const double scale = scale_of(f.t);
+  int first = kBins, end = kBins;  // bins of the cut
+  bool listed = false, inside = false;
+  if (f.has_k || f.has_p) {
+    u64 own_s = 0;
+    unsigned own_n = 0;
+#pragma unroll 8
+    for (int i = 0; i < p.parts; ++i) {
+      own_s += r.bin_sum[i * kBins + tid];
+      own_n += r.bin_n[i * kBins + tid];
+    }
+    u64 s = wave_scan(own_s);
+    unsigned n = wave_scan(own_n);
+    if (lane == 63) {
+      wave_s[wave] = s;
+      wave_n[wave] = n;
+    }
+    __syncthreads();
+    for (int i = 0; i < wave; ++i) {
+      s += wave_s[i];
+      n += wave_n[i];
+    }
+    const u64 all_s = wave_s[0] + wave_s[1] + wave_s[2] + wave_s[3];
+    const unsigned all_n = wave_n[0] + wave_n[1] + wave_n[2] + wave_n[3];
+    // the first bin for which a condition holds, of those that rise with the bin
+    auto first_bin = [&](bool holds, int slot) {
+      const u64 m = __ballot(holds);
+      if (lane == 0) lowest[wave][slot] = m ? wave * 64 + __builtin_ctzll(m) : kBins;
+    };
+    __shared__ u64 kept_s[2];
+    __shared__ unsigned kept_n;
+    const bool cut_k = f.has_k && all_n > (unsigned)f.k;
+    if (cut_k) {  // sums of the top k lie between those of the bins before its last one and with it
+      first_bin(n >= (unsigned)f.k, 0);
+      __syncthreads();
+      const int b = (int)min(min(lowest[0][0], lowest[1][0]), min(lowest[2][0], lowest[3][0]));
+      if (tid == b) {
+        kept_s[0] = n == (unsigned)f.k ? s : s - own_s;
+        kept_s[1] = s;
+        kept_n = n;
+      }
+      __syncthreads();
+      inside = kept_n != (unsigned)f.k;  // else the bin's end is the cut
+      end = b + 1;
+      first = inside ? b : end;
+    } else if (tid == 0) {
+      kept_s[0] = kept_s[1] = all_s;
+    }
+    if (f.has_p) {
+      __syncthreads();
+      first_bin(s >= share_of(f.p, kept_s[0]), 1);
+      first_bin(s >= share_of(f.p, kept_s[1]), 2);
+      __syncthreads();
+      const int lo = (int)min(min(lowest[0][1], lowest[1][1]), min(lowest[2][1], lowest[3][1]));
+      const int hi = (int)min(min(lowest[0][2], lowest[1][2]), min(lowest[2][2], lowest[3][2]));
+      first = lo;
+      if (!inside) end = hi + 1;  // else the sum of the top k needs its last bin's tokens
+    }
+    __shared__ unsigned span_n[2];
+    __shared__ u64 before_s;
+    __syncthreads();
+    if (tid == 0) {
+      span_n[0] = 0;
+      before_s = 0;
+    }
+    __syncthreads();
+    if (tid == first - 1) {
+      span_n[0] = n;
+      before_s = s;
+    }
+    if (tid == end - 1) span_n[1] = n;
+    __syncthreads();
+    const unsigned many = first < end ? span_n[1] - span_n[0] : 0;
+    listed = many > 0 && many <= (unsigned)kList;
+    if (part == 0 && tid == 0) {
+      r.head->first = first;
+      r.head->mode = first >= end ? kNoCut : listed ? kCutListed : kCutLong;
+      r.head->deep = inside;
+      r.head->before_n = span_n[0];
+      r.head->before_s = before_s;
+      r.head->need_s = f.has_p ? share_of(f.p, kept_s[0]) : kAll;
+    }
+    if (first < end && !listed) return;
+  } else if (part == 0 && tid == 0) {
+    r.head->first = kBins;
+    r.head->mode = kNoCut;
+  }
+  const unsigned sure = code_before(first, top, scale), maybe = listed ? code_before(end, top, scale) : sure;
+  for (int i = part * p.per; i < min(p.pieces, (part + 1) * p.per); ++i) {
+    u64 sum = 0;
+    unsigned mask = 0, codes[16];
+    int places[16];
+    each_of_piece<TYPE>(x, i * kPiece, p.vocab, [&](int j, unsigned c, int place) {
+      codes[j] = c;
+      places[j] = place;
+      if (c >= sure) {
+        const u64 w = weight_at(power_of(c, top, scale));
+        sum += w >= f.least ? w : 0;
+      } else if (c >= maybe) {
+        mask |= 1u << j;
+      }
+    });
+    if (listed) {
+      const unsigned mine = __popc(mask), upto = wave_scan(mine), all = __shfl(upto, 63);
+      if (all) {
+        unsigned base = 0;
+        if (lane == 0) base = atomicAdd(&r.head->listed, all);
+        base = __shfl(base, 0) + upto - mine;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (mask >> j & 1) {
+            if (base < (unsigned)kList) r.list[base] = uint2{codes[j], (unsigned)places[j]};
+            ++base;
+          }
+      }
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d /= 2) sum += __shfl_xor(sum, d);
+    __syncthreads();
+    if (lane == 0) wave_s[wave] = sum;
+    __syncthreads();
+    if (tid == 0) r.piece[i] = wave_s[0] + wave_s[1] + wave_s[2] + wave_s[3];
+  }
+}
+
+namespace {
 
 struct Cut {
   unsigned code;  // kept: codes above, and the first `ties` of this one
@@ -51,175 +473,341 @@ struct Cut {
   u64 sum;        // of what is kept
 };
 
-}  // namespace
+struct LastSpace {
+  u64 sum[kBins], piece[kMaxPieces], wave_s[16], found_s, before_s;
+  unsigned count[kBins], tie[kMaxPieces], wave_n[16], found_n, before_n;
+  int at;
+};
 
-template <int TYPE>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p)
+// The shortest leading part of the descending order of some tokens that has need_n of them or a sum of need_s, by 8-bit digits of
+// their codes.  each(fn): fn(code) for every token of this thread that has a weight; of them all, codes
+// agree with `same` above bit `shift`.  All are kept if neither is reached.
+template <class Each, class Weight> __device__ __forceinline__ Cut descend(LastSpace & l, unsigned need_n, u64 need_s, unsigned same, int shift, Each && each, Weight && weight)
 {
-  typedef typename Logit<TYPE>::e E;
-  __shared__ unsigned count[256];
-  __shared__ u64 sums[256];
-  __shared__ unsigned wave_u[16], sh_need_n;
-  __shared__ u64 wave_s[16], sh_need_s, sh_above_s;
-  __shared__ unsigned sh_above_n;
-  __shared__ int sh_at;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x;
-  const E * x = static_cast<const E *>(p.x) + (long)row * p.row;
-  const int n = p.vocab;
-
-  // the largest and its first place
-  unsigned top = 0;
-  int at = n;
-  for (int i = tid; i < n; i += kThreads) {
-    const unsigned c = code_of((float)x[i]);
-    if (c > top) {
-      top = c;
-      at = i;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  unsigned before_n = 0, prefix = shift < 32 ? same >> shift : 0;
+  u64 before_s = 0;
+  for (;;) {
+    const int next = max(shift - 8, 0), width = shift - next;
+    if (tid < kBins) {
+      l.count[tid] = 0;
+      l.sum[tid] = 0;
     }
-  }
-  for (int d = 32; d >= 1; d /= 2) {
-    const unsigned c = __shfl_xor(top, d);
-    const int j = __shfl_xor(at, d);
-    if (c > top || (c == top && j < at)) {
-      top = c;
-      at = j;
+    if (tid == 0) l.at = -1;
+    __syncthreads();
+    each([&](unsigned c) {
+      if (shift < 32 && c >> shift != prefix) return;
+      const unsigned b = (1u << width) - 1 - ((c >> next) & ((1u << width) - 1));  // the largest first
+      atomicAdd(&l.count[b], 1u);
+      atomicAdd(&l.sum[b], weight(c));
+    });
+    __syncthreads();
+    unsigned n = 0, own_n = 0;
+    u64 s = 0, own_s = 0;
+    if (tid < kBins) {
+      own_n = l.count[tid];
+      own_s = l.sum[tid];
+      n = wave_scan(own_n);
+      s = wave_scan(own_s);
+      if (lane == 63) {
+        l.wave_n[wave] = n;
+        l.wave_s[wave] = s;
+      }
     }
-  }
-  if (lane == 0) {
-    wave_u[wave] = top;
-    wave_s[wave] = (u64)at;
-  }
-  __syncthreads();
-  for (int i = 0; i < 16; ++i) {
-    const unsigned c = wave_u[i];
-    const int j = (int)wave_s[i];
-    if (c > top || (c == top && j < at)) {
-      top = c;
-      at = j;
+    __syncthreads();
+    if (tid < kBins) {
+      for (int i = 0; i < wave; ++i) {
+        n += l.wave_n[i];
+        s += l.wave_s[i];
+      }
+      const bool reached = before_n + n >= need_n || before_s + s >= need_s;
+      const bool earlier = before_n + (n - own_n) >= need_n || before_s + (s - own_s) >= need_s;
+      if (reached && !earlier) {
+        l.at = tid;
+        l.found_n = own_n;
+        l.before_n = before_n + (n - own_n);
+        l.before_s = before_s + (s - own_s);
+      }
+      if (tid == kBins - 1) l.found_s = before_s + s;
     }
-  }
-  __syncthreads();
-  const float t = p.temperature ? p.temperature[row] : 1.0f;
-  if (top <= kNone || !(t > 0.0f)) {
-    if (tid == 0) p.token[row] = top <= kNone ? -1 : at;
-    return;
-  }
-  const double scale = 1.4426950408889634 / (double)t;
-
-  // the shortest prefix of the descending order that has need_n tokens or a sum of need_s, by digits of the code
-  auto descend = [&](unsigned need_n, u64 need_s) {
-    unsigned prefix = 0, above_n = 0;
-    u64 above_s = 0;
-    Cut cut = {0, 0, 0};
-    for (int digit = 3; digit >= 0; --digit) {
-      for (int i = tid; i < 256; i += kThreads) {
-        count[i] = 0;
-        sums[i] = 0;
-      }
-      __syncthreads();
-      for (int i = tid; i < n; i += kThreads) {
-        const unsigned c = code_of((float)x[i]);
-        if (digit < 3 && c >> (8 * digit + 8) != prefix) continue;
-        const u64 w = weight_of(c, top, scale);
-        if (w == 0) continue;
-        atomicAdd(&count[c >> (8 * digit) & 255], 1u);
-        atomicAdd(&sums[c >> (8 * digit) & 255], w);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        int found = -1;
-        for (int i = 255; i >= 0; --i) {
-          if (count[i] == 0) continue;
-          found = i;
-          if (above_n + count[i] >= need_n || above_s + sums[i] >= need_s) break;
-          above_n += count[i];
-          above_s += sums[i];
-          found = -1;
-        }
-        sh_at = found;
-        sh_above_n = above_n;
-        sh_above_s = above_s;
-        if (found >= 0) {
-          sh_need_n = count[found];
-          sh_need_s = sums[found];
-        }
-      }
-      __syncthreads();
-      above_n = sh_above_n;
-      above_s = sh_above_s;
-      const int found = sh_at;
-      if (found < 0) return Cut{0, 0, above_s};  // all are kept
-      prefix = prefix << 8 | (unsigned)found;
-      if (digit == 0) {
-        const u64 w = weight_of(prefix, top, scale);
-        u64 ties = sh_need_n;
-        ties = min(ties, (u64)(need_n - above_n));
-        if (need_s > above_s) ties = min(ties, (need_s - above_s + w - 1) / w);
-        cut = Cut{prefix, (unsigned)ties, above_s + ties * w};
-      }
-      __syncthreads();
-    }
-    return cut;
-  };
-  const int k = p.top_k ? p.top_k[row] : 0;
-  Cut cut = descend(k > 0 ? (unsigned)k : 0xffffffffu, kAll);
-  const float tp = p.top_p ? p.top_p[row] : 1.0f, mp = p.min_p ? p.min_p[row] : 0.0f;
-  if (tp < 1.0f) {
-    const double need = ceil(fmax((double)tp, 0.0) * (double)cut.sum);
-    cut = descend(0xffffffffu, max((u64)need, (u64)1));
-  }
-  const u64 least = mp > 0.0f ? (u64)ceil((double)fminf(mp, 1.0f) * kOne) : 1;
-
-  // the kept weights in the order of the vocabulary: their sum, then the token at u of it
-  const float u = p.u[row];
-  u64 total = 0, goal = 0;
-  for (int pass = 0; pass < 2; ++pass) {
-    u64 before_s = 0;
-    unsigned before_n = 0;
-    if (tid == 0) sh_at = -1;
-    for (int base = 0; base < n; base += kThreads) {
-      const int i = base + tid;
-      const unsigned c = i < n ? code_of((float)x[i]) : 0;
-      u64 w = weight_of(c, top, scale);
-      if (w < least || c < cut.code) w = 0;
-      const bool tie = w != 0 && c == cut.code;
-      const unsigned long long ties = __ballot(tie);
-      if (lane == 0) wave_u[wave] = __popcll(ties);
-      __syncthreads();
-      unsigned rank = before_n + __popcll(ties & ((1ull << lane) - 1));
-      for (int j = 0; j < 16; ++j) {
-        if (j < wave) rank += wave_u[j];
-        before_n += wave_u[j];
-      }
-      if (tie && rank >= cut.ties) w = 0;
-      u64 run = w;
-      for (int d = 1; d < 64; d *= 2) {
-        const u64 y = __shfl_up(run, d);
-        if (lane >= d) run += y;
-      }
-      if (lane == 63) wave_s[wave] = run;
-      __syncthreads();
-      u64 mine = before_s + run;
-      for (int j = 0; j < 16; ++j) {
-        if (j < wave) mine += wave_s[j];
-        before_s += wave_s[j];
-      }
-      if (pass == 1 && w != 0 && mine > goal && mine - w <= goal) p.token[row] = i;
-      __syncthreads();
-    }
-    if (pass == 0) {
-      total = before_s;
-      goal = u > 0.0f ? (u < 1.0f ? min((u64)((double)u * (double)total), total - 1) : total - 1) : 0;
+    __syncthreads();
+    const int at = l.at;
+    if (at < 0) return Cut{0, 0, l.found_s};
+    before_n = l.before_n;
+    before_s = l.before_s;
+    const unsigned found = l.found_n;
+    prefix = (shift < 32 ? prefix << width : 0) | ((1u << width) - 1 - at);
+    shift = next;
+    __syncthreads();
+    if (shift == 0) {
+      const u64 w = weight(prefix);
+      u64 ties = min((u64)found, (u64)(need_n - before_n));
+      if (need_s > before_s) ties = min(ties, (need_s - before_s + w - 1) / w);
+      return Cut{prefix, (unsigned)ties, before_s + ties * w};
     }
   }
 }
 
+}  // namespace
+
+namespace {
+
+// sum over a work-group's lower threads; all: over all
+template <class T> __device__ __forceinline__ T block_before(T x, T (&wave_x)[16], T & all)
+{
+  const int wave = threadIdx.x >> 6;
+  const T upto = wave_scan(x);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) wave_x[wave] = upto;
+  __syncthreads();
+  T before = upto - x;
+  all = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const T y = wave_x[i];
+    before += i < wave ? y : 0;
+    all += y;
+  }
+  return before;
+}
+
+// floor(u times a sum), so that a larger sum lies beyond u of it
+__device__ __forceinline__ u64 goal_of(float u, u64 sum)
+{
+  return u > 0.0f ? u < 1.0f ? min((u64)((double)u * (double)sum), sum - 1) : sum - 1 : 0;
+}
+
+}  // namespace
+
+// 4. The token.  ROW: of a row that is in registers; else by what the kernels above found.
+template <int TYPE, bool ROW>
+__global__ void __launch_bounds__(kLast) sample_last_kernel(const SampleParams p)
+{
+  typedef typename Logit<TYPE>::e E;
+  constexpr int MINE = kList / kLast;
+  __shared__ LastSpace l;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x;
+  const E * x = static_cast<const E *>(p.x) + (long)row * p.row;
+  const int n = p.vocab;
+  const Filters f = filters_of(p, row);
+  const float u = p.u[row];
+  RowSpace r = {};
+  unsigned code[MINE], index[MINE];  // of the tokens at hand
+  unsigned top = 0, at = 0xffffffffu;
+  if constexpr (ROW) {
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      index[i] = tid * MINE + i;
+      code[i] = code_of((float)x[min((int)index[i], n - 1)]);
+      if (index[i] >= (unsigned)n) code[i] = 0;
+      if (code[i] > top) {
+        top = code[i];
+        at = index[i];
+      }
+    }
+    wave_top(top, at);
+    if (lane == 0) {
+      l.wave_n[wave] = top;
+      l.count[wave] = at;
+    }
+    __syncthreads();
+    top = l.wave_n[lane & 15];
+    at = l.count[lane & 15];
+    wave_top(top, at);
+    __syncthreads();
+  } else {
+    r = space_of(p, row);
+    row_top(r, p.parts, top, at);
+  }
+  if (top <= kNone || !(f.t > 0.0f)) {
+    if (tid == 0) p.token[row] = top <= kNone ? -1 : (int)at;
+    return;
+  }
+  const double scale = scale_of(f.t);
+  auto weight = [&](unsigned c) { return weight_of(c, top, scale); };
+  auto kept_weight = [&](unsigned c) {
+    const u64 w = weight_of(c, top, scale);
+    return w >= f.least ? w : 0;
+  };
+
+  // ---- the cut
+  RowHead head = {0, 0, f.has_k || f.has_p ? (unsigned)kCutListed : (unsigned)kNoCut, f.has_k, 0, 0, kAll};
+  if (!ROW) head = *r.head;
+  Cut cut = {head.mode == kNoCut && !ROW ? 0xffffffffu : 0u, 0, 0};  // none: what the bins say
+  if (head.mode == kCutListed) {
+    if constexpr (!ROW) {
+      head.listed = min(head.listed, (unsigned)kList);
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) {
+        const unsigned j = i * kLast + tid;
+        const uint2 y = r.list[min(j, head.listed - 1)];
+        code[i] = j < head.listed ? y.x : 0;
+        index[i] = y.y;
+      }
+    }
+    unsigned differ = 0, has = 0;  // bits in which codes differ from the largest; which tokens have a weight
+    u64 s = 0;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      const u64 w = weight(code[i]);
+      s += w;
+      if (w == 0) continue;
+      has |= 1u << i;
+      differ |= code[i] ^ top;
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d /= 2) differ |= __shfl_xor(differ, d);
+    if (lane == 0) l.wave_n[wave] = differ;
+    __syncthreads();
+    differ = 0;
+    for (int i = 0; i < 16; ++i) differ |= l.wave_n[i];
+    __syncthreads();
+    const int shift = differ ? 32 - __clz(differ) : 1;
+    auto each = [&](auto fn) {
+#pragma unroll
+      for (int i = 0; i < MINE; ++i)
+        if (has >> i & 1) fn(code[i]);
+    };
+    if (f.has_k && head.deep) cut = descend(l, (unsigned)f.k - (unsigned)head.before_n, kAll, top, shift, each, weight);
+    if (f.has_p) {
+      u64 need = head.need_s;
+      if (ROW && !f.has_k) {
+        block_before(s, l.wave_s, cut.sum);
+        __syncthreads();
+      }
+      if (ROW || head.deep) need = share_of(f.p, head.before_s + cut.sum);
+      cut = descend(l, 0xffffffffu, need - head.before_s, top, shift, each, weight);
+    }
+  } else if (head.mode == kCutLong) {
+    auto each = [&](auto fn) {
+      for (int i = tid; i < n; i += kLast) {
+        const unsigned c = code_of((float)x[i]);
+        if (power_of(c, top, scale) > -45.0) fn(c);
+      }
+    };
+    // without top-k the sum of all
+    cut = descend(l, f.has_k ? (unsigned)f.k : 0xffffffffu, kAll, 0, 32, each, weight);
+    if (f.has_p) cut = descend(l, 0xffffffffu, share_of(f.p, cut.sum), 0, 32, each, weight);
+  }
+
+  // ---- the piece that u falls in
+  const u64 tied = kept_weight(cut.code);  // of a token that equals the cut
+  u64 goal = 0;
+  unsigned ties = cut.ties;
+  int base = 0;
+  if constexpr (!ROW) {
+    if (tid < kMaxPieces) {
+      l.piece[tid] = head.mode != kCutLong && tid < p.pieces ? r.piece[tid] : 0;
+      l.tie[tid] = 0;
+    }
+    if (tid == 0) {
+      l.at = 0;
+      l.before_n = 0;
+      l.before_s = 0;
+    }
+    __syncthreads();
+    auto add = [&](unsigned c, unsigned i) {
+      if (c == cut.code) atomicAdd(&l.tie[i / kPiece], 1u);
+      else if (c > cut.code) atomicAdd(&l.piece[i / kPiece], kept_weight(c));
+    };
+    if (head.mode == kCutListed) {
+#pragma unroll
+      for (int i = 0; i < MINE; ++i)
+        if (i * kLast + tid < (int)head.listed) add(code[i], index[i]);
+    } else if (head.mode == kCutLong) {
+      for (int i = tid; i < n; i += kLast) add(code_of((float)x[i]), (unsigned)i);
+    }
+    __syncthreads();
+    const unsigned mine = tid < kMaxPieces ? l.tie[tid] : 0;
+    unsigned all_n;
+    const unsigned before_n = block_before(mine, l.wave_n, all_n), in = min(mine, ties - min(ties, before_n));
+    const u64 own = tid < kMaxPieces ? l.piece[tid] + in * tied : 0;
+    u64 all_s;
+    const u64 before_s = block_before(own, l.wave_s, all_s);
+    goal = goal_of(u, all_s);
+    if (before_s <= goal && goal - before_s < own) {
+      l.at = tid;
+      l.before_n = before_n;
+      l.before_s = before_s;
+    }
+    __syncthreads();
+    base = l.at * kPiece;
+    ties -= min(ties, l.before_n);
+    goal -= l.before_s;
+  }
+
+  // ---- the token: a thread's in order of the vocabulary
+  constexpr int HERE = ROW ? MINE : kPiece / kLast;
+  unsigned equal = 0;
+  if constexpr (!ROW) {
+#pragma unroll
+    for (int i = 0; i < HERE; ++i) {
+      const int j = base + tid * HERE + i;
+      code[i] = code_of((float)x[min(j, n - 1)]);
+      if (j >= n) code[i] = 0;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < HERE; ++i) equal += code[i] == cut.code;
+  unsigned all_n;
+  unsigned rank = block_before(equal, l.wave_n, all_n);
+  u64 w[HERE], own = 0;
+#pragma unroll
+  for (int i = 0; i < HERE; ++i) {
+    const double z = power_of(code[i], top, scale);
+    bool kept = code[i] > cut.code || (code[i] == cut.code && rank < ties);
+    if (!ROW) kept = kept || (z > -45.0 && bin_of(z) < (int)head.first && head.mode == kNoCut);
+    rank += code[i] == cut.code;
+    w[i] = kept && z > -45.0 ? weight_at(z) : 0;
+    if (w[i] < f.least) w[i] = 0;
+    own += w[i];
+  }
+  u64 all_s;
+  u64 before = block_before(own, l.wave_s, all_s);
+  if (ROW) goal = goal_of(u, all_s);
+  if (before <= goal && goal - before < own) {
+#pragma unroll
+    for (int i = 0; i < HERE; ++i) {
+      if (before <= goal && goal - before < w[i]) p.token[row] = base + tid * HERE + i;
+      before += w[i];
+    }
+  }
+}
+
+namespace {
+
+template <int TYPE> void launch_sample_type(const SampleParams & p, hipStream_t s)
+{
+  if (p.parts == 0) {
+    hipLaunchKernelGGL((sample_last_kernel<TYPE, true>), dim3((unsigned)p.rows), dim3(kLast), 0, s, p);
+    return;
+  }
+  const dim3 grid((unsigned)p.rows * (unsigned)p.parts), blk(kThreads);
+  hipLaunchKernelGGL((sample_top_kernel<TYPE>), grid, blk, 0, s, p);
+  if (p.top_k || p.top_p) hipLaunchKernelGGL((sample_bins_kernel<TYPE>), grid, blk, 0, s, p);
+  hipLaunchKernelGGL((sample_list_kernel<TYPE>), grid, blk, 0, s, p);
+  hipLaunchKernelGGL((sample_last_kernel<TYPE, false>), dim3((unsigned)p.rows), dim3(kLast), 0, s, p);
+}
+
+}  // namespace
+
+size_t sample_split(SampleParams & p)
+{
+  p.pieces = (p.vocab + kPiece - 1) / kPiece;
+  p.parts = p.per = 0;
+  if (p.vocab <= kList || p.rows == 0) return 0;
+  // eight work-groups a CU, of whole pieces
+  const int want = std::min(p.pieces, (2048 + p.rows - 1) / p.rows);
+  p.per = (p.pieces + want - 1) / want;
+  p.parts = (p.pieces + p.per - 1) / p.per;
+  return (size_t)p.rows * row_bytes(p.parts, p.pieces);
+}
+
 void launch_sample(const SampleParams & p, hipStream_t s)
 {
-  const dim3 grid((unsigned)p.rows), blk(kThreads);
-  if (p.type == kSeqF16) hipLaunchKernelGGL((sample_kernel<kSeqF16>), grid, blk, 0, s, p);
-  else if (p.type == kSeqBF16) hipLaunchKernelGGL((sample_kernel<kSeqBF16>), grid, blk, 0, s, p);
-  else hipLaunchKernelGGL((sample_kernel<kSeqF32>), grid, blk, 0, s, p);
+  if (p.type == kSeqF16) launch_sample_type<kSeqF16>(p, s);
+  else if (p.type == kSeqBF16) launch_sample_type<kSeqBF16>(p, s);
+  else launch_sample_type<kSeqF32>(p, s);
 }
 
 }  // namespace ivh

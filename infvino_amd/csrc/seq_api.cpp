@@ -509,8 +509,8 @@ int ivh_sample_workspace(const ivh_sample_desc * d, int rows, size_t * bytes)
 {
   return guard([&] {
     need(bytes, "null bytes");
-    sampling(d, rows);
-    *bytes = 0;
+    ivh::SampleParams p = sampling(d, rows);
+    *bytes = ivh::sample_split(p);
   });
 }
 
@@ -525,7 +525,11 @@ int ivh_sample(const ivh_sample_desc * d, const void * logits, const float * tem
     need((reinterpret_cast<uintptr_t>(temperature) | reinterpret_cast<uintptr_t>(top_k) | reinterpret_cast<uintptr_t>(top_p) |
           reinterpret_cast<uintptr_t>(min_p) | reinterpret_cast<uintptr_t>(u) | reinterpret_cast<uintptr_t>(token)) % 4 == 0,
          "sample: misaligned operand");
-    check_device(stream, {logits, temperature, top_k, top_p, min_p, u, token});
+    const size_t bytes = ivh::sample_split(p);
+    need(bytes == 0 || (workspace && workspace_bytes >= bytes), "workspace too small (ivh_sample_workspace)");
+    need(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must start at a multiple of 16 bytes");
+    check_device(stream, {logits, temperature, top_k, top_p, min_p, u, token, bytes ? workspace : nullptr});
+    p.ws = bytes ? workspace : nullptr;
     p.x = logits;
     p.temperature = temperature;
     p.top_k = top_k;

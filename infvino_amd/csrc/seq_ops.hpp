@@ -123,7 +123,12 @@ struct SampleParams {
   const float * min_p = nullptr;
   const float * u = nullptr;
   int32_t * token = nullptr;
+  // how a call is split, from sample_split
+  int pieces = 0, parts = 0, per = 0;  // pieces of a row, work-groups over them and pieces of each; 0 parts: one work-group a row
+  void * ws = nullptr;
 };
+// Sets the split of a call; returns the workspace bytes.
+size_t sample_split(SampleParams & p);
 void launch_sample(const SampleParams & p, hipStream_t s);
 
 struct RaggedParams {
