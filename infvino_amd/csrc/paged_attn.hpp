@@ -59,8 +59,8 @@ __device__ __forceinline__ Steps key_steps(int full, int imin, int imax, int win
 __device__ __forceinline__ int step_key(const Steps & s, int n) { return 64 * (n < s.first ? n : s.from + n - s.first); }
 
 // Which keys a build takes: all of a sequence; those behind what its group shares; a group's shared ones,
-// for the rows of all its sequences.
-enum KeysOf : int { kAllKeys, kOwnKeys, kSharedKeys };
+// for the rows of all its sequences; or the last two side by side, `shared_wgs` work-groups for the latter.
+enum KeysOf : int { kAllKeys, kOwnKeys, kSharedKeys, kBothKeys };
 
 // Group g's first sequence and rows, and the leading keys that are taken once for all of them: whole
 // pages and steps, of which the first new row of every sequence sees each, so that nothing is masked.
@@ -97,6 +97,10 @@ __device__ __forceinline__ int keys_shared(const PagedParams & p, int b)
 template <int TYPE, int BITS, int DP, bool FULL, int QT, int WK, int KEYS>
 __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(const PagedParams p, int units)
 {
+  const bool shared = KEYS == kSharedKeys || (KEYS == kBothKeys && (int)blockIdx.x < p.shared_wgs);
+  const int block = blockIdx.x - (KEYS == kBothKeys && !shared ? p.shared_wgs : 0);
+  const int row_slots = KEYS == kBothKeys && shared ? p.shared_slots : p.row_slots;
+  const int parts = KEYS == kBothKeys && shared ? p.lead : p.parts, part_steps = KEYS == kBothKeys && shared ? p.shared_steps : p.part_steps;
   using T = St<TYPE>;
   typedef typename T::e E;
   constexpr int EK = BITS == 8 ? 16 : 8;        // channels of a 16-byte key piece
@@ -118,17 +122,18 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
   // A unit (part of the keys, sequence, key head) has row_slots work-groups, on one XCD; units go
   // round the XCDs, so that each gets its share of long and short sequences, and of their last parts,
   // which only long ones have and which come last.
-  int w = blockIdx.x / kXcds;
-  const int slot = w % p.row_slots;
-  w = w / p.row_slots * kXcds + blockIdx.x % kXcds;
-  if (w >= units) return;
-  const int seqs = (KEYS == kSharedKeys ? p.groups : c.batch) * c.heads, part = w / seqs;
+  int w = block / kXcds;
+  const int slot = w % row_slots;
+  w = w / row_slots * kXcds + block % kXcds;
+  const int seqs = (KEYS != kAllKeys && shared ? p.groups : c.batch) * c.heads;
+  if (w >= (KEYS == kBothKeys ? seqs * parts : units)) return;
+  const int part = w / seqs;
   w -= part * seqs;
   const int h = w % c.heads, b = w / c.heads;
 
   int c0, c1, full, place0, skip = 0;  // place0: of the first new token
   const int32_t * table = c.table;
-  if constexpr (KEYS == kSharedKeys) {
+  if (KEYS != kAllKeys && shared) {
     const SharedPart part_of = shared_part(p, b);
     if (part_of.keys == 0) return;
     c0 = part_of.c0;
@@ -142,7 +147,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
     full = (int)min(max(len, 0L), (long)c.width * c.page);
     place0 = (int)max(len, 0L) - (c1 - c0);
     table += (long)b * c.width;
-    if constexpr (KEYS == kOwnKeys) skip = keys_shared(p, b);
+    if (KEYS != kAllKeys) skip = keys_shared(p, b);
   }
   const int nnew = c1 - c0, rows = nnew * p.group;
   const int lp = 31 - __clz(c.page);  // page is a power of two
@@ -152,13 +157,13 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
   const float scale = fmaxf(fabsf(p.scale_log2), 1.2e-38f);  // not 0: masked scores stay -inf
   const unsigned flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
 
-  for (int tile = slot; tile * ROWS < rows; tile += p.row_slots) {
+  for (int tile = slot; tile * ROWS < rows; tile += row_slots) {
     const int row0 = tile * ROWS + wr * 16 * QT, rend = min(rows, row0 + 16 * QT);  // this wave's rows
     const int wg_last = min(rows, tile * ROWS + ROWS) - 1;
     // the steps are the work-group's, the masks this wave's (which may have no rows)
     const Steps steps = key_steps(full, place0 + tile * ROWS / p.group, place0 + wg_last / p.group, p.window, p.sinks, skip);
     const int imin = place0 + row0 / p.group, imax = place0 + (max(rend, row0 + 1) - 1) / p.group;
-    const int per = max(p.part_steps, (steps.total + p.parts - 1) / p.parts);
+    const int per = max(part_steps, (steps.total + parts - 1) / parts);
     const int n0 = part * per, n1 = rend > row0 ? min(steps.total, n0 + per) : 0;
 
     // what this lane's query of each row tile sees: keys lo .. lo + n and the first `first`
@@ -514,7 +519,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
             *reinterpret_cast<u2v *>(out + 16 * j + 4 * g) = y;
           }
         } else {
-          const long total = (long)c.tokens * p.heads, at = (long)(part + (KEYS == kOwnKeys ? p.lead : 0)) * total + row;
+          const long total = (long)c.tokens * p.heads, at = (long)(part + (KEYS != kAllKeys && !shared ? p.lead : 0)) * total + row;
           const long all = KEYS == kAllKeys ? p.parts : p.all_parts;
           if (n0 < n1) {
             float * out = p.ws + at * c.dim;
@@ -525,7 +530,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
           f2v * ml = reinterpret_cast<f2v *>(p.ws + all * total * c.dim);
           if (g == 0) ml[at] = f2v{M[u], L[u]};
           // a sequence that shares nothing leaves the parts of groups empty
-          if (KEYS == kOwnKeys && skip == 0 && part == 0 && g == 0)
+          if (KEYS != kAllKeys && !shared && skip == 0 && part == 0 && g == 0)
             for (int i = 0; i < p.lead; ++i) ml[i * total + row] = f2v{kLowest, 0.0f};
         }
       }
@@ -596,7 +601,7 @@ template <int TYPE, int BITS, int DP, bool FULL, int QT, int WK, int KEYS> void 
   auto kern = paged_attn_kernel<TYPE, BITS, DP, FULL, QT, WK, KEYS>;
   const size_t lds = (size_t)(WK / 2) * (4 / WK) * 16 * QT * (DP + 4 + 2) * sizeof(float);
   const long units = (long)(KEYS == kSharedKeys ? p.groups : p.c.batch) * p.c.heads * p.parts;
-  const dim3 grid((unsigned)((units + kXcds - 1) / kXcds * kXcds * p.row_slots)), blk(256);
+  const dim3 grid((unsigned)((units + kXcds - 1) / kXcds * kXcds * p.row_slots + (KEYS == kBothKeys ? p.shared_wgs : 0))), blk(256);
   hipLaunchKernelGGL(kern, grid, blk, lds, s, p, (int)units);
 }
 

@@ -4,6 +4,10 @@
 
 namespace ivh {
 
+namespace {
+constexpr long kSharedWgs = 768;  // work-groups over shared keys
+}  // namespace
+
 size_t prefix_split(PrefixParams & p, int max_new, int max_len, int max_shared)
 {
   const CacheParams & c = p.own.c;
@@ -11,11 +15,30 @@ size_t prefix_split(PrefixParams & p, int max_new, int max_len, int max_shared)
   p.own.lead = 0;
   if (p.own.groups > 0) {
     p.first.c.batch = p.own.groups;
-    paged_split(p.first, (c.tokens + p.own.groups - 1) / p.own.groups, max_shared);
+    const long tokens = (c.tokens + p.own.groups - 1) / p.own.groups, rows = tokens * p.own.group;
+    p.many = rows >= 512 && max_shared >= 8192;
+    if (p.many) {
+      PagedParams & f = p.first;
+      const long wgs0 = (long)p.own.groups * c.heads, steps = std::max(1, max_shared / 64);
+      f.row_slots = (int)std::min<long>({(rows + 127) / 128, 1024, std::max<long>(1, (1L << 23) / wgs0)});
+      const long wgs = wgs0 * f.row_slots, want = std::max<long>(1, kSharedWgs / wgs);
+      f.parts = (int)std::min<long>({want, steps, 256, std::max<long>(1, (1L << 23) / wgs)});
+      f.part_steps = (int)((steps + f.parts - 1) / f.parts);
+      f.parts = (int)((steps + f.part_steps - 1) / f.part_steps);
+    } else {
+      paged_split(p.first, (int)tokens, max_shared);
+    }
     p.own.lead = p.first.parts;
     p.first.c.batch = c.batch;
   }
   paged_split(p.own, max_new, std::max(1, max_len - (p.own.groups > 0 ? max_shared : 0)));
+  p.both = p.own.lead > 0 && !p.many && p.first.row_tiles == p.own.row_tiles && p.first.row_waves == p.own.row_waves;
+  if (p.both) {
+    const long units = (long)p.own.groups * c.heads * p.first.parts;
+    p.own.shared_wgs = (int)((units + kXcds - 1) / kXcds * kXcds * p.first.row_slots);
+    p.own.shared_slots = p.first.row_slots;
+    p.own.shared_steps = p.first.part_steps;
+  }
   p.own.all_parts = p.first.all_parts = p.own.lead + p.own.parts;
   return (size_t)p.own.all_parts * c.tokens * p.own.heads * (c.dim + 2) * sizeof(float);
 }

@@ -75,6 +75,7 @@ struct PagedParams {
   const int32_t * member = nullptr;  // [groups + 1] first sequences
   const int32_t * shared = nullptr;  // [groups] tokens
   int groups = 0, lead = 0, all_parts = 1;
+  int shared_wgs = 0, shared_slots = 1, shared_steps = 1;  // both kinds of keys in one launch: the split of the shared ones
 };
 // Sets the split of a call with at most max_new new tokens and max_len cached ones in a
 // sequence (bounds that only steer the split); returns the workspace bytes.
@@ -85,6 +86,8 @@ void launch_paged_bf16(const PagedParams & p, hipStream_t s);  // its bf16 kerne
 // Attention with shared first tokens: the split of both kinds of keys, those of groups first.
 struct PrefixParams {
   PagedParams first, own;
+  int many = 0;  // shared keys by work-groups of 128 rows
+  int both = 0;  // both kinds of keys in one launch
 };
 size_t prefix_split(PrefixParams & p, int max_new, int max_len, int max_shared);
 void launch_prefix_attention(const PrefixParams & p, hipStream_t s);
