@@ -238,6 +238,7 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
   float * first = p.ws + ((long)u * p.heads + h) * one;
 
   f16v s[ND];
+  float held = 1.0f;  // fp16: what the column is held times, a power of two, so that the parts below are normal numbers
   auto state_io = [&](float * at, auto store) __attribute__((always_inline)) {  // channels that are not there: zeros, nowhere
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(at, (short)0, (int)(one * 4), kBufDword3);
 #pragma unroll
@@ -246,7 +247,7 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
       for (int v = 0; v < 16; ++v) {
         const int dk = 32 * d + result_row(v, half);
         const unsigned off = dv < p.dim ? (unsigned)(dk * p.dim + dv) * 4u : kBufOOB;  // rows from key_dim on lie behind the end
-        const float x = s[d][v];  // by itself: a bit cast of an element is one of the vector's start
+        const float x = TYPE == kSeqF16 ? s[d][v] / held : s[d][v];  // by itself: a bit cast of an element is one of the vector's start
         if (store) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x), r, (int)off, 0, 0);
         else s[d][v] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, (int)off, 0, 0));
       }
@@ -370,7 +371,7 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
       if (!OUT) copy_v(c + 1, other);
     }
     f16v acc[2];
-    float fit = 1.0f;  // fp16: the state's power of two
+    float fit = 1.0f, back = 1.0f;  // fp16: what brings this lane's column of the state to about 2^14, and what it comes back by
     auto from_state = [&]() __attribute__((always_inline)) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) acc[t] = f16v{};
@@ -390,11 +391,12 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
         acc[0] = T::mma32(part[1], y0, acc[0]);
         acc[1] = T::mma32(part[1], y1, acc[1]);
       }
+      const float f0 = its.since[SIDE][col], f1 = its.since[SIDE][32 + col];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const float f = its.since[SIDE][32 * t + col] / fit;
-#pragma unroll
-        for (int x = 0; x < 16; ++x) acc[t][x] *= f;
+      for (int x = 0; x < 16; ++x) {
+        const float y = TYPE == kSeqF16 ? __shfl(back, turned(result_row(x, half))) : 1.0f;
+        acc[0][x] *= f0 * y;
+        acc[1][x] *= f1 * y;
       }
     };
     u4v vf[4], y[4];
@@ -444,10 +446,9 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
           for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int x = 0; x < 16; ++x) most = fmaxf(most, fabsf(s[d][x]));
-#pragma unroll
-          for (int d = 1; d < 16; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
-          most = across16(across32(most, MaxOp()), MaxOp());
+          most = across32(most, MaxOp());
           fit = __builtin_ldexpf(1.0f, min(max(14 - __builtin_amdgcn_frexp_expf(most), -100), 100));
+          back = 1.0f / (fit * held);
         }
         from_state();
       }
@@ -522,7 +523,21 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
     }
     // the state: values with their decays to the chunk's end in parts of 16 bits, which together have fp32's precision
     if (on) {
-      const float a = its.whole[SIDE];
+      float a = its.whole[SIDE];
+      if constexpr (TYPE == kSeqF16) {
+        float most = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const f2v y = unpack2<TYPE>(vf[j][x]), z = *reinterpret_cast<const f2v *>(&its.left[SIDE][16 * j + 8 * half + 2 * x]);
+            most = fmaxf(most, fmaxf(fabsf(y[0] * z[0]), fabsf(y[1] * z[1])));
+          }
+        most = across32(most, MaxOp());
+        const float next = most > 0.0f ? __builtin_ldexpf(1.0f, min(max(14 - __builtin_amdgcn_frexp_expf(most), -2), 40)) : held;
+        a *= next / held;
+        held = next;
+      }
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -534,7 +549,7 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           unsigned z[PARTS];
-          split<TYPE>(unpack2<TYPE>(vf[j][x]), x < 2 ? f2v{l0[2 * x], l0[2 * x + 1]} : f2v{l1[2 * x - 4], l1[2 * x - 3]}, z);
+          split<TYPE>(unpack2<TYPE>(vf[j][x]), (x < 2 ? f2v{l0[2 * x], l0[2 * x + 1]} : f2v{l1[2 * x - 4], l1[2 * x - 3]}) * held, z);
 #pragma unroll
           for (int i = 0; i < PARTS; ++i) part[i][x] = z[i];
         }
@@ -578,13 +593,13 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
 }
 
 // The first states of a sequence's segments from those that the segments add: four elements a thread.
-__global__ void __launch_bounds__(256) linear_join_kernel(const LinearParams p, int blocks)
+__global__ void __launch_bounds__(256) linear_join_kernel(const LinearParams p)
 {
   const long one = (long)p.key_dim * p.dim;
-  const int block = blockIdx.x % blocks, h = blockIdx.x / blocks % p.heads, b = blockIdx.x / blocks / p.heads;
+  const int h = blockIdx.x % p.heads, b = blockIdx.x / p.heads;
   const int c0 = min(max(p.cu[b], 0), p.tokens), rows = min(max(p.cu[b + 1], c0), p.tokens) - c0;
   const int n = (rows + p.seg - 1) / p.seg;
-  const long u = (long)(c0 / p.seg) + b, i = 4L * (block * 256 + threadIdx.x);
+  const long u = (long)(c0 / p.seg) + b, i = 4L * (blockIdx.y * 256 + threadIdx.x);
   if (n < 3 || i >= one) return;
   float * at = p.ws + (u * p.heads + h) * one + i;
   f4v x = *reinterpret_cast<const f4v *>(at + p.heads * one);
@@ -609,7 +624,7 @@ template <int TYPE, int DK> void launch_linear_chunks(const LinearParams & p, hi
   if (p.ws) {
     hipLaunchKernelGGL((linear_chunk_kernel<TYPE, DK, false>), grid, blk, 0, s, p, units, blocks);
     const int parts = (p.key_dim * p.dim + 1023) / 1024;
-    hipLaunchKernelGGL(linear_join_kernel, dim3((unsigned)((long)p.batch * p.heads * parts)), blk, 0, s, p, parts);
+    hipLaunchKernelGGL(linear_join_kernel, dim3((unsigned)(p.batch * p.heads), (unsigned)parts), blk, 0, s, p);
   }
   hipLaunchKernelGGL((linear_chunk_kernel<TYPE, DK, true>), grid, blk, 0, s, p, units, blocks);
 }
@@ -642,7 +657,9 @@ size_t linear_split(LinearParams & p, int max_new)
   auto rounds = [&](long units) { return (units * wgs + cap - 1) / cap; };
   const long whole = std::max(rounds(p.batch) * mean, (long)max_new);
   long best = 0, cost = whole * 10 / 17;
-  for (long seg = 256; seg < max_new; seg += kChunk) {
+  // a launch holds fewer than 2^24 work-groups
+  const long least = std::max<long>(256, ((long)p.tokens * wgs >> 22) / kChunk * kChunk + kChunk);
+  for (long seg = least; seg < max_new; seg += std::max<long>(kChunk, seg / 16 / kChunk * kChunk)) {
     const long c = rounds(p.batch * ((mean + seg - 1) / seg)) * seg;
     if (c < cost || (best > 0 && c == cost)) {
       best = seg;

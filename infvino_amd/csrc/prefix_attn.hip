@@ -35,6 +35,7 @@ size_t prefix_split(PrefixParams & p, int max_new, int max_len, int max_shared)
   p.both = p.own.lead > 0 && !p.many && p.first.row_tiles == p.own.row_tiles && p.first.row_waves == p.own.row_waves;
   if (p.both) {
     const long units = (long)p.own.groups * c.heads * p.first.parts;
+    p.both = units * p.first.row_slots < 1L << 22;  // of the 2^24 that a launch holds
     p.own.shared_wgs = (int)((units + kXcds - 1) / kXcds * kXcds * p.first.row_slots);
     p.own.shared_slots = p.first.row_slots;
     p.own.shared_steps = p.first.part_steps;

@@ -193,8 +193,8 @@ ivh::PrefixParams prefix(const ivh_prefix_attn_desc * d, int batch, int groups, 
   return p;
 }
 
-// most states times heads, and rows times heads, of a call: a launch's work-groups are counted in 31 bits
-constexpr int kMaxStates = 1 << 22;
+// sequences times heads of a call: a launch has up to 8 work-groups for each, of fewer than 2^24
+constexpr int kMaxStates = 1 << 20;
 
 ivh::LinearParams linear(const ivh_linear_attn_desc * d, int batch, int tokens, size_t * bytes)
 {
