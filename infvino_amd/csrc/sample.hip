@@ -7,7 +7,7 @@
 //
 // Every filter keeps a leading part of the descending order (equal logits by index), so that all of them together are one
 // cut, a code of a logit and how many of those that equal it are in, and nothing is sorted.  Rows of up to 8192 tokens
-// stay in the registers of one work-group.  Longer ones are read three times in pieces of 4096 tokens, by as many
+// are left to one work-group.  Longer ones are read three times in pieces of 4096 tokens, by as many
 // work-groups as fill the chip:
 //   1. the largest logit of each part;
 //   2. counts and sums of weights in 256 bins of z, 8 to a power of two down to 2^-28 (rows with top-k or top-p alone);
@@ -32,10 +32,11 @@ typedef unsigned long long u64;
 
 constexpr int kPiece = 4096;      // tokens of a piece
 constexpr int kMaxPieces = 128;   // of a row
-constexpr int kList = 8192;       // listed tokens of a row, and tokens of a row that one work-group keeps
+constexpr int kList = 8192;       // listed tokens of a row, and tokens of a row that is left to one work-group
 constexpr int kBins = 256;
 constexpr int kThreads = 256;     // of the kernels over pieces
-constexpr int kLast = 1024;       // of the last kernel
+constexpr int kLast = 512;        // of the last kernel, two work-groups a CU,
+constexpr int kLastWaves = kLast / 64;
 constexpr u64 kOne = 1ull << 44;  // the largest weight
 constexpr u64 kAll = 1ull << 63;  // no sum is larger
 constexpr unsigned kNone = 0x007fffffu;  // code of -infinity
@@ -54,28 +55,27 @@ __device__ __forceinline__ unsigned code_of(float x)
 }
 __device__ __forceinline__ float value_of(unsigned code) { return __builtin_bit_cast(float, code & 0x80000000u ? code & 0x7fffffffu : ~code); }
 
-// z of a token; not above -45 if it has no weight
-__device__ __forceinline__ double power_of(unsigned code, unsigned top, double scale)
+// z of a logit x (NaN where none can be formed): above -45 if it has a weight.  x may be NaN or infinite
+__device__ __forceinline__ double power_of(float x, float top, double scale)
 {
-  const double z = ((double)value_of(code) - (double)value_of(top)) * scale;
-  return code == top ? 0.0 : code <= kNone ? -1000.0 : z;
+  return x == top ? 0.0 : ((double)x - (double)top) * scale;
 }
-// 2^z in units of 2^-44, z in (-45, 0]: Taylor's polynomial of e^t, |t| <= log 2 / 2, off by 2^-52 before rounding; adding
+// 2^z in units of 2^-44, z in (-45, 0]: Taylor's polynomial of e^t, |t| <= log 2 / 2, off by 2^-47 before rounding; adding
 // 2^52 leaves the nearest whole number in a double's low bits
 __device__ __forceinline__ u64 weight_at(double z)
 {
   const double n = rint(z), t = (z - n) * 0.693147180559945309;
-  double y = 1.0 / 6227020800.0;
-  constexpr double c[] = {1.0 / 479001600.0, 1.0 / 39916800.0, 1.0 / 3628800.0, 1.0 / 362880.0, 1.0 / 40320.0, 1.0 / 5040.0,
+  double y = 1.0 / 39916800.0;
+  constexpr double c[] = {1.0 / 3628800.0, 1.0 / 362880.0, 1.0 / 40320.0, 1.0 / 5040.0,
                           1.0 / 720.0, 1.0 / 120.0, 1.0 / 24.0, 1.0 / 6.0, 0.5, 1.0, 1.0};
 #pragma unroll
-  for (int i = 0; i < 13; ++i) y = fma(y, t, c[i]);
+  for (int i = 0; i < 11; ++i) y = fma(y, t, c[i]);
   const double w = __builtin_amdgcn_ldexp(y, (int)n + 44) + 4503599627370496.0;
   return max(__builtin_bit_cast(u64, w) & 0xfffffffffffffull, 1ull);
 }
-__device__ __forceinline__ u64 weight_of(unsigned code, unsigned top, double scale)
+__device__ __forceinline__ u64 weight_of(float x, float top, double scale)
 {
-  const double z = power_of(code, top, scale);
+  const double z = power_of(x, top, scale);
   return z > -45.0 ? weight_at(z) : 0;
 }
 // bin of a power in (-45, 0], the largest first; does not decrease as z falls
@@ -112,10 +112,10 @@ __device__ __forceinline__ u64 share_of(float p, u64 sum) { return max((u64)ceil
 // What the kernels over pieces leave for the last one.
 struct RowHead {
   unsigned listed;    // tokens in the list
-  unsigned first;     // bins before it are kept
   unsigned mode;
   unsigned deep;      // the sum of the top k is known from the listed tokens alone
-  u64 before_n, before_s, need_s;  // of the bins before; the sum that top-p asks for, unless deep
+  unsigned sure;      // codes from here on are kept, whatever is listed
+  u64 before_n, before_s, need_s;  // of the surely kept; the sum that top-p asks for, unless deep
 };
 enum Mode : unsigned { kNoCut, kCutListed, kCutLong };
 
@@ -178,8 +178,8 @@ __device__ __forceinline__ unsigned code_before(int bin, unsigned top, double sc
   if (bin <= 0) return 0xffffffffu;
   while (width > 0) {
     const unsigned step = width / 64 + 1, c = low + min(step * lane, width);
-    const double z = power_of(c, top, scale);
-    const u64 in = __ballot(z > -45.0 && bin_of(z) < bin);
+    const double z = power_of(value_of(c), value_of(top), scale);
+    const u64 in = __ballot(c > kNone && z > -45.0 && bin_of(z) < bin);  // codes up to that of -infinity are NaN's
     const unsigned i = in ? __builtin_ctzll(in) : 64;  // the first of them
     const unsigned from = i ? min(step * (i - 1) + 1, width) : 0;
     width = (i < 64 ? min(step * i, width) : width) - from;
@@ -207,8 +207,8 @@ template <class E> __device__ __forceinline__ u4v load_any(const E * x)
   else return *reinterpret_cast<const u4v_of_floats *>(x);
 }
 
-// The 16 tokens of a piece that a thread has: fn(i, code, index), runs of 16 bytes at any alignment, 256 threads
-// side by side.
+// The 16 tokens of a piece that a thread has: fn(i, logit, index), runs of 16 bytes at any alignment, 256 threads
+// side by side; -infinity behind the last.
 template <int TYPE, class Fn> __device__ __forceinline__ void each_of_piece(const typename Logit<TYPE>::e * x, int base, int n, Fn && fn)
 {
   typedef typename Logit<TYPE>::e E;
@@ -225,11 +225,11 @@ template <int TYPE, class Fn> __device__ __forceinline__ void each_of_piece(cons
         const unsigned y = run[i][j];
         const int at = first + i * kThreads * RUN + j * (RUN / 4);
         if constexpr (TYPE == kSeqF32) {
-          fn(i * RUN + j, code_of(__builtin_bit_cast(float, y)), at);
+          fn(i * RUN + j, __builtin_bit_cast(float, y), at);
         } else {
           const f2v z = unpack2<TYPE>(y);
-          fn(i * RUN + 2 * j, code_of(z[0]), at);
-          fn(i * RUN + 2 * j + 1, code_of(z[1]), at + 1);
+          fn(i * RUN + 2 * j, z[0], at);
+          fn(i * RUN + 2 * j + 1, z[1], at + 1);
         }
       }
   } else {
@@ -239,8 +239,7 @@ template <int TYPE, class Fn> __device__ __forceinline__ void each_of_piece(cons
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int at = first + i / RUN * kThreads * RUN + i % RUN;
-      const unsigned code = code_of((float)run[i]);
-      fn(i, at < n ? code : 0u, at);
+      fn(i, at < n ? (float)run[i] : -__builtin_inff(), at);
     }
   }
 }
@@ -257,14 +256,16 @@ __global__ void __launch_bounds__(kThreads) sample_top_kernel(const SampleParams
   const E * x = static_cast<const E *>(p.x) + (long)row * p.row;
   const RowSpace r = space_of(p, row);
   if (part == 0 && threadIdx.x == 0) r.head->listed = 0;
-  unsigned top = 0, first = 0xffffffffu;
+  float most = -__builtin_inff();
+  unsigned first = 0xffffffffu;
   for (int i = part * p.per; i < min(p.pieces, (part + 1) * p.per); ++i)
-    each_of_piece<TYPE>(x, i * kPiece, p.vocab, [&](int, unsigned c, int j) {
-      if (c > top) {  // a thread's indexes grow
-        top = c;
+    each_of_piece<TYPE>(x, i * kPiece, p.vocab, [&](int, float y, int j) {
+      if (y > most) {  // a thread's indexes grow
+        most = y;
         first = (unsigned)j;
       }
     });
+  unsigned top = code_of(most);
   wave_top(top, first);
   if ((threadIdx.x & 63) == 0) {
     code[threadIdx.x / 64] = top;
@@ -301,11 +302,13 @@ __global__ void __launch_bounds__(kThreads) sample_bins_kernel(const SampleParam
   unsigned top, at;
   row_top(r, p.parts, top, at);
   const double scale = scale_of(f.t);
+  const float most = value_of(top);
   const int mine = (threadIdx.x & (COPIES - 1)) * (kBins + 1);
+  if (top <= kNone) return;
   __syncthreads();
   for (int i = part * p.per; i < min(p.pieces, (part + 1) * p.per); ++i)
-    each_of_piece<TYPE>(x, i * kPiece, p.vocab, [&](int, unsigned c, int) {
-      const double z = power_of(c, top, scale);
+    each_of_piece<TYPE>(x, i * kPiece, p.vocab, [&](int, float y, int) {
+      const double z = power_of(y, most, scale);
       if (!(z > -45.0)) return;
       const int b = mine + bin_of(z);
       atomicAdd(&count[b], 1u);
@@ -341,8 +344,10 @@ __global__ void __launch_bounds__(kThreads) sample_list_kernel(const SampleParam
   row_top(r, p.parts, top, at);
   if (top <= kNone) return;
   const double scale = scale_of(f.t);
+  const float most = value_of(top);
   int first = kBins, end = kBins;  // bins of the cut
-  bool listed = false, inside = false;
+  bool listed = false, inside = false, none = false;
+  float kept = -__builtin_inff(), maybe = 0.0f;  // logits that are surely kept, and listed, from here on; none: none surely
   if (f.has_k || f.has_p) {
     u64 own_s = 0;
     unsigned own_n = 0;
@@ -414,31 +419,32 @@ __global__ void __launch_bounds__(kThreads) sample_list_kernel(const SampleParam
     __syncthreads();
     const unsigned many = first < end ? span_n[1] - span_n[0] : 0;
     listed = many > 0 && many <= (unsigned)kList;
+    const unsigned sure = code_before(first, top, scale);
     if (part == 0 && tid == 0) {
-      r.head->first = first;
       r.head->mode = first >= end ? kNoCut : listed ? kCutListed : kCutLong;
       r.head->deep = inside;
+      r.head->sure = sure;
       r.head->before_n = span_n[0];
       r.head->before_s = before_s;
       r.head->need_s = f.has_p ? share_of(f.p, kept_s[0]) : kAll;
     }
     if (first < end && !listed) return;
-  } else if (part == 0 && tid == 0) {
-    r.head->first = kBins;
-    r.head->mode = kNoCut;
+    kept = first > 0 ? value_of(sure) : __builtin_inff();
+    none = first == 0;
+    if (listed) maybe = value_of(code_before(end, top, scale));
   }
-  const unsigned sure = code_before(first, top, scale), maybe = listed ? code_before(end, top, scale) : sure;
   for (int i = part * p.per; i < min(p.pieces, (part + 1) * p.per); ++i) {
     u64 sum = 0;
-    unsigned mask = 0, codes[16];
+    unsigned mask = 0;
+    float logits[16];
     int places[16];
-    each_of_piece<TYPE>(x, i * kPiece, p.vocab, [&](int j, unsigned c, int place) {
-      codes[j] = c;
+    each_of_piece<TYPE>(x, i * kPiece, p.vocab, [&](int j, float y, int place) {
+      logits[j] = y;
       places[j] = place;
-      if (c >= sure) {
-        const u64 w = weight_at(power_of(c, top, scale));
+      if (y >= kept && !none) {
+        const u64 w = weight_of(y, most, scale);
         sum += w >= f.least ? w : 0;
-      } else if (c >= maybe) {
+      } else if (listed && y >= maybe) {
         mask |= 1u << j;
       }
     });
@@ -451,7 +457,7 @@ __global__ void __launch_bounds__(kThreads) sample_list_kernel(const SampleParam
 #pragma unroll
         for (int j = 0; j < 16; ++j)
           if (mask >> j & 1) {
-            if (base < (unsigned)kList) r.list[base] = uint2{codes[j], (unsigned)places[j]};
+            if (base < (unsigned)kList) r.list[base] = uint2{code_of(logits[j]), (unsigned)places[j]};
             ++base;
           }
       }
@@ -473,87 +479,16 @@ struct Cut {
   u64 sum;        // of what is kept
 };
 
+constexpr int kDigit = 11, kDigits = 1 << kDigit;  // of a code
+
 struct LastSpace {
-  u64 sum[kBins], piece[kMaxPieces], wave_s[16], found_s, before_s;
-  unsigned count[kBins], tie[kMaxPieces], wave_n[16], found_n, before_n;
+  u64 sum[kDigits], piece[kMaxPieces], wave_s[kLastWaves], found_s, before_s;
+  unsigned count[kDigits], tie[kMaxPieces], wave_n[kLastWaves], found_n, before_n;
   int at;
 };
 
-// The shortest leading part of the descending order of some tokens that has need_n of them or a sum of need_s, by 8-bit digits of
-// their codes.  each(fn): fn(code) for every token of this thread that has a weight; of them all, codes
-// agree with `same` above bit `shift`.  All are kept if neither is reached.
-template <class Each, class Weight> __device__ __forceinline__ Cut descend(LastSpace & l, unsigned need_n, u64 need_s, unsigned same, int shift, Each && each, Weight && weight)
-{
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  unsigned before_n = 0, prefix = shift < 32 ? same >> shift : 0;
-  u64 before_s = 0;
-  for (;;) {
-    const int next = max(shift - 8, 0), width = shift - next;
-    if (tid < kBins) {
-      l.count[tid] = 0;
-      l.sum[tid] = 0;
-    }
-    if (tid == 0) l.at = -1;
-    __syncthreads();
-    each([&](unsigned c) {
-      if (shift < 32 && c >> shift != prefix) return;
-      const unsigned b = (1u << width) - 1 - ((c >> next) & ((1u << width) - 1));  // the largest first
-      atomicAdd(&l.count[b], 1u);
-      atomicAdd(&l.sum[b], weight(c));
-    });
-    __syncthreads();
-    unsigned n = 0, own_n = 0;
-    u64 s = 0, own_s = 0;
-    if (tid < kBins) {
-      own_n = l.count[tid];
-      own_s = l.sum[tid];
-      n = wave_scan(own_n);
-      s = wave_scan(own_s);
-      if (lane == 63) {
-        l.wave_n[wave] = n;
-        l.wave_s[wave] = s;
-      }
-    }
-    __syncthreads();
-    if (tid < kBins) {
-      for (int i = 0; i < wave; ++i) {
-        n += l.wave_n[i];
-        s += l.wave_s[i];
-      }
-      const bool reached = before_n + n >= need_n || before_s + s >= need_s;
-      const bool earlier = before_n + (n - own_n) >= need_n || before_s + (s - own_s) >= need_s;
-      if (reached && !earlier) {
-        l.at = tid;
-        l.found_n = own_n;
-        l.before_n = before_n + (n - own_n);
-        l.before_s = before_s + (s - own_s);
-      }
-      if (tid == kBins - 1) l.found_s = before_s + s;
-    }
-    __syncthreads();
-    const int at = l.at;
-    if (at < 0) return Cut{0, 0, l.found_s};
-    before_n = l.before_n;
-    before_s = l.before_s;
-    const unsigned found = l.found_n;
-    prefix = (shift < 32 ? prefix << width : 0) | ((1u << width) - 1 - at);
-    shift = next;
-    __syncthreads();
-    if (shift == 0) {
-      const u64 w = weight(prefix);
-      u64 ties = min((u64)found, (u64)(need_n - before_n));
-      if (need_s > before_s) ties = min(ties, (need_s - before_s + w - 1) / w);
-      return Cut{prefix, (unsigned)ties, before_s + ties * w};
-    }
-  }
-}
-
-}  // namespace
-
-namespace {
-
 // sum over a work-group's lower threads; all: over all
-template <class T> __device__ __forceinline__ T block_before(T x, T (&wave_x)[16], T & all)
+template <class T> __device__ __forceinline__ T block_before(T x, T (&wave_x)[kLastWaves], T & all)
 {
   const int wave = threadIdx.x >> 6;
   const T upto = wave_scan(x);
@@ -563,12 +498,83 @@ template <class T> __device__ __forceinline__ T block_before(T x, T (&wave_x)[16
   T before = upto - x;
   all = 0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < kLastWaves; ++i) {
     const T y = wave_x[i];
     before += i < wave ? y : 0;
     all += y;
   }
   return before;
+}
+
+// The shortest leading part of the descending order of some tokens that has need_n of them or a sum of need_s, by digits of their
+// codes of up to 11 bits.  each(fn): fn(code, weight) for every token of this thread that has a weight; of them all, codes
+// agree with `same` from bit `shift` on and below bit `low`.  All are kept if neither is reached.
+template <class Each> __device__ __forceinline__ Cut descend(LastSpace & l, unsigned need_n, u64 need_s, unsigned same, int shift, int low, Each && each)
+{
+  constexpr int OWN = kDigits / kLast;
+  const int tid = threadIdx.x;
+  unsigned before_n = 0, prefix = shift < 32 ? same >> shift : 0;
+  u64 before_s = 0;
+  for (;;) {
+    const int next = max(shift - kDigit, low), width = shift - next;
+    const unsigned mask = (1u << width) - 1;
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      l.count[tid * OWN + i] = 0;
+      l.sum[tid * OWN + i] = 0;
+    }
+    if (tid == 0) l.at = -1;
+    __syncthreads();
+    each([&](unsigned c, u64 w) {
+      if (shift < 32 && c >> shift != prefix) return;
+      const unsigned b = mask - ((c >> next) & mask);  // the largest first
+      atomicAdd(&l.count[b], 1u);
+      atomicAdd(&l.sum[b], w);
+    });
+    __syncthreads();
+    unsigned own_n = 0, all_n;
+    u64 own_s = 0, all_s;
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      own_n += l.count[tid * OWN + i];
+      own_s += l.sum[tid * OWN + i];
+    }
+    unsigned n = before_n + block_before(own_n, l.wave_n, all_n);
+    u64 s = before_s + block_before(own_s, l.wave_s, all_s);
+    if (!(n >= need_n || s >= need_s)) {
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) {
+        const unsigned here_n = l.count[tid * OWN + i];
+        const u64 here_s = l.sum[tid * OWN + i];
+        if (n + here_n >= need_n || s + here_s >= need_s) {
+          l.at = tid * OWN + i;
+          l.found_n = here_n;
+          l.found_s = here_s;
+          l.before_n = n;
+          l.before_s = s;
+          break;
+        }
+        n += here_n;
+        s += here_s;
+      }
+    }
+    __syncthreads();
+    const int at = l.at;
+    if (at < 0) return Cut{0, 0, before_s + all_s};
+    before_n = l.before_n;
+    before_s = l.before_s;
+    const unsigned found_n = l.found_n;
+    const u64 found_s = l.found_s;
+    prefix = (shift < 32 ? prefix << width : 0) | (mask - at);
+    shift = next;
+    __syncthreads();
+    if (shift == low) {
+      const u64 w = found_s / found_n;  // of each: they are equal
+      u64 ties = min((u64)found_n, (u64)(need_n - before_n));
+      if (need_s > before_s) ties = min(ties, (need_s - before_s + w - 1) / w);
+      return Cut{prefix << low | (same & ((1u << low) - 1)), (unsigned)ties, before_s + ties * w};
+    }
+  }
 }
 
 // floor(u times a sum), so that a larger sum lies beyond u of it
@@ -579,12 +585,11 @@ __device__ __forceinline__ u64 goal_of(float u, u64 sum)
 
 }  // namespace
 
-// 4. The token.  ROW: of a row that is in registers; else by what the kernels above found.
+// 4. The token.  ROW: of a row of up to kList tokens; else by what the kernels above found.
 template <int TYPE, bool ROW>
-__global__ void __launch_bounds__(kLast) sample_last_kernel(const SampleParams p)
+__global__ void __launch_bounds__(kLast, 4) sample_last_kernel(const SampleParams p)
 {
   typedef typename Logit<TYPE>::e E;
-  constexpr int MINE = kList / kLast;
   __shared__ LastSpace l;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x;
   const E * x = static_cast<const E *>(p.x) + (long)row * p.row;
@@ -592,17 +597,13 @@ __global__ void __launch_bounds__(kLast) sample_last_kernel(const SampleParams p
   const Filters f = filters_of(p, row);
   const float u = p.u[row];
   RowSpace r = {};
-  unsigned code[MINE], index[MINE];  // of the tokens at hand
   unsigned top = 0, at = 0xffffffffu;
   if constexpr (ROW) {
-#pragma unroll
-    for (int i = 0; i < MINE; ++i) {
-      index[i] = tid * MINE + i;
-      code[i] = code_of((float)x[min((int)index[i], n - 1)]);
-      if (index[i] >= (unsigned)n) code[i] = 0;
-      if (code[i] > top) {
-        top = code[i];
-        at = index[i];
+    for (int i = tid; i < n; i += kLast) {
+      const unsigned c = code_of((float)x[i]);
+      if (c > top) {
+        top = c;
+        at = i;
       }
     }
     wave_top(top, at);
@@ -611,8 +612,8 @@ __global__ void __launch_bounds__(kLast) sample_last_kernel(const SampleParams p
       l.count[wave] = at;
     }
     __syncthreads();
-    top = l.wave_n[lane & 15];
-    at = l.count[lane & 15];
+    top = l.wave_n[lane & (kLastWaves - 1)];
+    at = l.count[lane & (kLastWaves - 1)];
     wave_top(top, at);
     __syncthreads();
   } else {
@@ -624,78 +625,60 @@ __global__ void __launch_bounds__(kLast) sample_last_kernel(const SampleParams p
     return;
   }
   const double scale = scale_of(f.t);
-  auto weight = [&](unsigned c) { return weight_of(c, top, scale); };
+  const float most = value_of(top);
   auto kept_weight = [&](unsigned c) {
-    const u64 w = weight_of(c, top, scale);
+    const u64 w = c > kNone ? weight_of(value_of(c), most, scale) : 0;
     return w >= f.least ? w : 0;
   };
 
   // ---- the cut
-  RowHead head = {0, 0, f.has_k || f.has_p ? (unsigned)kCutListed : (unsigned)kNoCut, f.has_k, 0, 0, kAll};
-  if (!ROW) head = *r.head;
-  Cut cut = {head.mode == kNoCut && !ROW ? 0xffffffffu : 0u, 0, 0};  // none: what the bins say
+  const bool filtered = f.has_k || f.has_p;
+  RowHead head = {0, filtered ? (unsigned)(ROW ? kCutLong : kCutListed) : (unsigned)kNoCut, f.has_k, 0, 0, 0, kAll};
+  if (!ROW && filtered) head = *r.head;
+  head.listed = min(head.listed, (unsigned)kList);
+  Cut cut = {head.mode == kNoCut ? 0xffffffffu : 0u, 0, 0};  // none: codes from head.sure on
   if (head.mode == kCutListed) {
-    if constexpr (!ROW) {
-      head.listed = min(head.listed, (unsigned)kList);
-#pragma unroll
-      for (int i = 0; i < MINE; ++i) {
-        const unsigned j = i * kLast + tid;
-        const uint2 y = r.list[min(j, head.listed - 1)];
-        code[i] = j < head.listed ? y.x : 0;
-        index[i] = y.y;
+    auto each = [&](auto fn) {
+      for (unsigned i = tid; i < head.listed; i += kLast) {
+        const unsigned c = r.list[i].x;
+        fn(c, weight_of(value_of(c), most, scale));
       }
-    }
-    unsigned differ = 0, has = 0;  // bits in which codes differ from the largest; which tokens have a weight
-    u64 s = 0;
-#pragma unroll
-    for (int i = 0; i < MINE; ++i) {
-      const u64 w = weight(code[i]);
-      s += w;
-      if (w == 0) continue;
-      has |= 1u << i;
-      differ |= code[i] ^ top;
-    }
+    };
+    unsigned differ = 0;  // bits in which codes differ from the largest
+    for (unsigned i = tid; i < head.listed; i += kLast) differ |= r.list[i].x ^ top;
 #pragma unroll
     for (int d = 32; d >= 1; d /= 2) differ |= __shfl_xor(differ, d);
     if (lane == 0) l.wave_n[wave] = differ;
     __syncthreads();
     differ = 0;
-    for (int i = 0; i < 16; ++i) differ |= l.wave_n[i];
+    for (int i = 0; i < kLastWaves; ++i) differ |= l.wave_n[i];
     __syncthreads();
-    const int shift = differ ? 32 - __clz(differ) : 1;
-    auto each = [&](auto fn) {
-#pragma unroll
-      for (int i = 0; i < MINE; ++i)
-        if (has >> i & 1) fn(code[i]);
-    };
-    if (f.has_k && head.deep) cut = descend(l, (unsigned)f.k - (unsigned)head.before_n, kAll, top, shift, each, weight);
+    const int shift = differ ? 32 - __clz(differ) : 1, low = differ ? __ffs(differ) - 1 : 0;
+    if (f.has_k && head.deep) cut = descend(l, (unsigned)f.k - (unsigned)head.before_n, kAll, top, shift, low, each);
     if (f.has_p) {
-      u64 need = head.need_s;
-      if (ROW && !f.has_k) {
-        block_before(s, l.wave_s, cut.sum);
-        __syncthreads();
-      }
-      if (ROW || head.deep) need = share_of(f.p, head.before_s + cut.sum);
-      cut = descend(l, 0xffffffffu, need - head.before_s, top, shift, each, weight);
+      const u64 need = head.deep ? share_of(f.p, head.before_s + cut.sum) : head.need_s;
+      cut = descend(l, 0xffffffffu, need - head.before_s, top, shift, low, each);
     }
   } else if (head.mode == kCutLong) {
     auto each = [&](auto fn) {
       for (int i = tid; i < n; i += kLast) {
-        const unsigned c = code_of((float)x[i]);
-        if (power_of(c, top, scale) > -45.0) fn(c);
+        const float y = (float)x[i];
+        const u64 w = weight_of(y, most, scale);
+        if (w) fn(code_of(y), w);
       }
     };
     // without top-k the sum of all
-    cut = descend(l, f.has_k ? (unsigned)f.k : 0xffffffffu, kAll, 0, 32, each, weight);
-    if (f.has_p) cut = descend(l, 0xffffffffu, share_of(f.p, cut.sum), 0, 32, each, weight);
+    cut = descend(l, f.has_k ? (unsigned)f.k : 0xffffffffu, kAll, 0, 32, 0, each);
+    if (f.has_p) cut = descend(l, 0xffffffffu, share_of(f.p, cut.sum), 0, 32, 0, each);
   }
 
   // ---- the piece that u falls in
-  const u64 tied = kept_weight(cut.code);  // of a token that equals the cut
+  constexpr int HERE = ROW ? kList / kLast : kPiece / kLast;  // tokens of a thread below
   u64 goal = 0;
   unsigned ties = cut.ties;
   int base = 0;
   if constexpr (!ROW) {
+    const u64 tied = kept_weight(cut.code);  // of a token that equals the cut
     if (tid < kMaxPieces) {
       l.piece[tid] = head.mode != kCutLong && tid < p.pieces ? r.piece[tid] : 0;
       l.tie[tid] = 0;
@@ -711,9 +694,7 @@ __global__ void __launch_bounds__(kLast) sample_last_kernel(const SampleParams p
       else if (c > cut.code) atomicAdd(&l.piece[i / kPiece], kept_weight(c));
     };
     if (head.mode == kCutListed) {
-#pragma unroll
-      for (int i = 0; i < MINE; ++i)
-        if (i * kLast + tid < (int)head.listed) add(code[i], index[i]);
+      for (unsigned i = tid; i < head.listed; i += kLast) add(r.list[i].x, r.list[i].y);
     } else if (head.mode == kCutLong) {
       for (int i = tid; i < n; i += kLast) add(code_of((float)x[i]), (unsigned)i);
     }
@@ -737,39 +718,33 @@ __global__ void __launch_bounds__(kLast) sample_last_kernel(const SampleParams p
   }
 
   // ---- the token: a thread's in order of the vocabulary
-  constexpr int HERE = ROW ? MINE : kPiece / kLast;
-  unsigned equal = 0;
-  if constexpr (!ROW) {
-#pragma unroll
-    for (int i = 0; i < HERE; ++i) {
-      const int j = base + tid * HERE + i;
-      code[i] = code_of((float)x[min(j, n - 1)]);
-      if (j >= n) code[i] = 0;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < HERE; ++i) equal += code[i] == cut.code;
-  unsigned all_n;
-  unsigned rank = block_before(equal, l.wave_n, all_n);
-  u64 w[HERE], own = 0;
+  unsigned code[HERE], equal = 0;
 #pragma unroll
   for (int i = 0; i < HERE; ++i) {
-    const double z = power_of(code[i], top, scale);
-    bool kept = code[i] > cut.code || (code[i] == cut.code && rank < ties);
-    if (!ROW) kept = kept || (z > -45.0 && bin_of(z) < (int)head.first && head.mode == kNoCut);
-    rank += code[i] == cut.code;
-    w[i] = kept && z > -45.0 ? weight_at(z) : 0;
-    if (w[i] < f.least) w[i] = 0;
-    own += w[i];
+    const int j = base + tid * HERE + i;
+    code[i] = code_of((float)x[min(j, n - 1)]);
+    if (j >= n) code[i] = 0;
+    equal += code[i] == cut.code;
   }
-  u64 all_s;
+  unsigned all_n, rank = block_before(equal, l.wave_n, all_n);
+  auto weight_here = [&](int i) {  // in order: ties count up
+    const bool tie = code[i] == cut.code, in = code[i] > cut.code || (tie && rank < ties) || (head.mode == kNoCut && code[i] >= head.sure);
+    rank += tie;
+    return in ? kept_weight(code[i]) : 0;
+  };
+  u64 own = 0, all_s;
+  const unsigned first = rank;
+#pragma unroll
+  for (int i = 0; i < HERE; ++i) own += weight_here(i);
   u64 before = block_before(own, l.wave_s, all_s);
   if (ROW) goal = goal_of(u, all_s);
   if (before <= goal && goal - before < own) {
+    rank = first;
 #pragma unroll
     for (int i = 0; i < HERE; ++i) {
-      if (before <= goal && goal - before < w[i]) p.token[row] = base + tid * HERE + i;
-      before += w[i];
+      const u64 w = weight_here(i);
+      if (before <= goal && goal - before < w) p.token[row] = base + tid * HERE + i;
+      before += w;
     }
   }
 }
