@@ -207,40 +207,63 @@ template <class E> __device__ __forceinline__ u4v load_any(const E * x)
   else return *reinterpret_cast<const u4v_of_floats *>(x);
 }
 
-// The 16 tokens of a piece that a thread has: fn(i, logit, index), runs of 16 bytes at any alignment, 256 threads
-// side by side; -infinity behind the last.
-template <int TYPE, class Fn> __device__ __forceinline__ void each_of_piece(const typename Logit<TYPE>::e * x, int base, int n, Fn && fn)
-{
+// The 16 tokens of a piece that a thread has, in runs of 16 bytes at any alignment, 256 threads side by side; -infinity
+// behind the row's end.
+template <int TYPE> struct Piece {
   typedef typename Logit<TYPE>::e E;
-  constexpr int RUN = 16 / sizeof(E), RUNS = 16 / RUN;
-  const int first = base + (int)threadIdx.x * RUN;
-  if (base + kPiece <= n) {
-    u4v run[RUNS];
+  static constexpr int RUN = 16 / sizeof(E), RUNS = 16 / RUN;
+  u4v run[RUNS];
+  static __device__ __forceinline__ int first(int i) { return (i * kThreads + (int)threadIdx.x) * RUN; }
+  // place of token j of a thread
+  static __device__ __forceinline__ int place(int j) { return first(j / RUN) + j % RUN; }
+  __device__ __forceinline__ void load(const E * x, int base, int n)
+  {
+    constexpr unsigned NONE = TYPE == kSeqF32 ? 0xff800000u : TYPE == kSeqF16 ? 0xfc00u : 0xff80u;  // -infinity
+    if (base + kPiece <= n) {
 #pragma unroll
-    for (int i = 0; i < RUNS; ++i) run[i] = load_any(x + first + i * kThreads * RUN);
+      for (int i = 0; i < RUNS; ++i) run[i] = load_any(x + base + first(i));
+    } else {
+#pragma unroll
+      for (int i = 0; i < RUNS; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int at = base + first(i) + j * (RUN / 4);
+          if constexpr (TYPE == kSeqF32) {
+            const E y = x[min(at, n - 1)];
+            run[i][j] = at < n ? __builtin_bit_cast(unsigned, y) : NONE;
+          } else {
+            const E y = x[min(at, n - 1)], z = x[min(at + 1, n - 1)];
+            run[i][j] = (at < n ? __builtin_bit_cast(unsigned short, y) : NONE) | (at + 1 < n ? (unsigned)__builtin_bit_cast(unsigned short, z) : NONE) << 16;
+          }
+        }
+    }
+  }
+  template <class Fn> __device__ __forceinline__ void each(Fn && fn) const  // fn(j, logit)
+  {
 #pragma unroll
     for (int i = 0; i < RUNS; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const unsigned y = run[i][j];
-        const int at = first + i * kThreads * RUN + j * (RUN / 4);
         if constexpr (TYPE == kSeqF32) {
-          fn(i * RUN + j, __builtin_bit_cast(float, y), at);
+          fn(i * RUN + j, __builtin_bit_cast(float, y));
         } else {
           const f2v z = unpack2<TYPE>(y);
-          fn(i * RUN + 2 * j, z[0], at);
-          fn(i * RUN + 2 * j + 1, z[1], at + 1);
+          fn(i * RUN + 2 * j, z[0]);
+          fn(i * RUN + 2 * j + 1, z[1]);
         }
       }
-  } else {
-    E run[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) run[i] = x[min(first + i / RUN * kThreads * RUN + i % RUN, n - 1)];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int at = first + i / RUN * kThreads * RUN + i % RUN;
-      fn(i, at < n ? (float)run[i] : -__builtin_inff(), at);
-    }
+  }
+};
+
+// The pieces of a part, the next one on its way while one is worked on: fn(piece, first token), the first
+// from `ahead`, which is asked for before what the work needs is known.
+template <int TYPE, class Fn> __device__ __forceinline__ void each_piece(Piece<TYPE> & ahead, const typename Logit<TYPE>::e * x, int from, int to, int n, Fn && fn)
+{
+  for (int i = from; i < to; ++i) {
+    const Piece<TYPE> now = ahead;
+    if (i + 1 < to) ahead.load(x, (i + 1) * kPiece, n);
+    fn(now, i);
   }
 }
 
@@ -258,13 +281,17 @@ __global__ void __launch_bounds__(kThreads) sample_top_kernel(const SampleParams
   if (part == 0 && threadIdx.x == 0) r.head->listed = 0;
   float most = -__builtin_inff();
   unsigned first = 0xffffffffu;
-  for (int i = part * p.per; i < min(p.pieces, (part + 1) * p.per); ++i)
-    each_of_piece<TYPE>(x, i * kPiece, p.vocab, [&](int, float y, int j) {
+  const int from = part * p.per, to = min(p.pieces, from + p.per);
+  Piece<TYPE> ahead;
+  ahead.load(x, from * kPiece, p.vocab);
+  each_piece<TYPE>(ahead, x, from, to, p.vocab, [&](const Piece<TYPE> & now, int i) {
+    now.each([&](int j, float y) {
       if (y > most) {  // a thread's indexes grow
         most = y;
-        first = (unsigned)j;
+        first = (unsigned)(i * kPiece + Piece<TYPE>::place(j));
       }
     });
+  });
   unsigned top = code_of(most);
   wave_top(top, first);
   if ((threadIdx.x & 63) == 0) {
@@ -295,6 +322,9 @@ __global__ void __launch_bounds__(kThreads) sample_bins_kernel(const SampleParam
   if (!(f.has_k || f.has_p) || !(f.t > 0.0f)) return;
   const E * x = static_cast<const E *>(p.x) + (long)row * p.row;
   const RowSpace r = space_of(p, row);
+  const int from = part * p.per, to = min(p.pieces, from + p.per);
+  Piece<TYPE> ahead;
+  ahead.load(x, from * kPiece, p.vocab);
   for (int i = threadIdx.x; i < COPIES * (kBins + 1); i += kThreads) {
     sum[i] = 0;
     count[i] = 0;
@@ -306,14 +336,15 @@ __global__ void __launch_bounds__(kThreads) sample_bins_kernel(const SampleParam
   const int mine = (threadIdx.x & (COPIES - 1)) * (kBins + 1);
   if (top <= kNone) return;
   __syncthreads();
-  for (int i = part * p.per; i < min(p.pieces, (part + 1) * p.per); ++i)
-    each_of_piece<TYPE>(x, i * kPiece, p.vocab, [&](int, float y, int) {
+  each_piece<TYPE>(ahead, x, from, to, p.vocab, [&](const Piece<TYPE> & now, int) {
+    now.each([&](int, float y) {
       const double z = power_of(y, most, scale);
       if (!(z > -45.0)) return;
       const int b = mine + bin_of(z);
       atomicAdd(&count[b], 1u);
       if (f.has_p) atomicAdd(&sum[b], weight_at(z));
     });
+  });
   __syncthreads();
   const int b = threadIdx.x;
   u64 s = 0;
@@ -340,6 +371,9 @@ __global__ void __launch_bounds__(kThreads) sample_list_kernel(const SampleParam
   if (!(f.t > 0.0f)) return;
   const E * x = static_cast<const E *>(p.x) + (long)row * p.row;
   const RowSpace r = space_of(p, row);
+  const int from = part * p.per, to = min(p.pieces, from + p.per);
+  Piece<TYPE> ahead;
+  ahead.load(x, from * kPiece, p.vocab);
   unsigned top, at;
   row_top(r, p.parts, top, at);
   if (top <= kNone) return;
@@ -351,7 +385,7 @@ __global__ void __launch_bounds__(kThreads) sample_list_kernel(const SampleParam
   if (f.has_k || f.has_p) {
     u64 own_s = 0;
     unsigned own_n = 0;
-#pragma unroll 8
+#pragma unroll 16
     for (int i = 0; i < p.parts; ++i) {
       own_s += r.bin_sum[i * kBins + tid];
       own_n += r.bin_n[i * kBins + tid];
@@ -433,14 +467,10 @@ __global__ void __launch_bounds__(kThreads) sample_list_kernel(const SampleParam
     none = first == 0;
     if (listed) maybe = value_of(code_before(end, top, scale));
   }
-  for (int i = part * p.per; i < min(p.pieces, (part + 1) * p.per); ++i) {
+  each_piece<TYPE>(ahead, x, from, to, p.vocab, [&](const Piece<TYPE> & now, int i) {
     u64 sum = 0;
     unsigned mask = 0;
-    float logits[16];
-    int places[16];
-    each_of_piece<TYPE>(x, i * kPiece, p.vocab, [&](int j, float y, int place) {
-      logits[j] = y;
-      places[j] = place;
+    now.each([&](int j, float y) {
       if (y >= kept && !none) {
         const u64 w = weight_of(y, most, scale);
         sum += w >= f.least ? w : 0;
@@ -454,12 +484,11 @@ __global__ void __launch_bounds__(kThreads) sample_list_kernel(const SampleParam
         unsigned base = 0;
         if (lane == 0) base = atomicAdd(&r.head->listed, all);
         base = __shfl(base, 0) + upto - mine;
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (mask >> j & 1) {
-            if (base < (unsigned)kList) r.list[base] = uint2{code_of(logits[j]), (unsigned)places[j]};
-            ++base;
-          }
+        now.each([&](int j, float y) {
+          if (!(mask >> j & 1)) return;
+          if (base < (unsigned)kList) r.list[base] = uint2{code_of(y), (unsigned)(i * kPiece + Piece<TYPE>::place(j))};
+          ++base;
+        });
       }
     }
 #pragma unroll
@@ -468,7 +497,7 @@ __global__ void __launch_bounds__(kThreads) sample_list_kernel(const SampleParam
     if (lane == 0) wave_s[wave] = sum;
     __syncthreads();
     if (tid == 0) r.piece[i] = wave_s[0] + wave_s[1] + wave_s[2] + wave_s[3];
-  }
+  });
 }
 
 namespace {
