@@ -59,46 +59,92 @@ __device__ __forceinline__ Steps key_steps(int full, int imin, int imax, int win
 __device__ __forceinline__ int step_key(const Steps & s, int n) { return 64 * (n < s.first ? n : s.from + n - s.first); }
 
 // Which keys a build takes: all of a sequence; those behind what its group shares; a group's shared ones,
-// for the rows of all its sequences; or the last two side by side, `shared_wgs` work-groups for the latter.
-enum KeysOf : int { kAllKeys, kOwnKeys, kSharedKeys, kBothKeys };
+// for the rows of all its sequences; or the last two side by side, `shared_wgs` work-groups for the latter, in
+// tiles of 16 rows or by shared_rows.
+enum KeysOf : int { kAllKeys, kOwnKeys, kSharedKeys, kBothKeys, kBothWide };
 
-// Group g's first sequence and rows, and the leading keys that are taken once for all of them: whole
+// A group's first sequence and rows, and the leading keys that are taken once for all of them: whole
 // pages and steps, of which the first new row of every sequence sees each, so that nothing is masked.
 struct SharedPart {
   int first, c0, c1, keys;
 };
-__device__ __forceinline__ SharedPart shared_part(const PagedParams & p, int g)
+__device__ __forceinline__ int whole_keys(const CacheParams & c, int keys)
 {
-  const CacheParams & c = p.c;
-  const int b0 = min(max(p.member[g], 0), c.batch), b1 = min(max(p.member[g + 1], b0), c.batch);
-  int keys = min(max(p.shared[g], 0), c.width * c.page);
-  for (int b = b0 + (threadIdx.x & 63); b < b1; b += 64) {
-    const int c0 = min(max(c.cu[b], 0), c.tokens), c1 = min(max(c.cu[b + 1], c0), c.tokens);
-    if (c1 > c0) keys = min(keys, max(max(c.lens[b], 0) - (c1 - c0) + 1, 0));
-  }
 #pragma unroll
   for (int i = 32; i >= 1; i /= 2) keys = min(keys, __shfl_xor(keys, i));
   const int unit = max(c.page, 64);
-  const int c0 = min(max(c.cu[b0], 0), c.tokens), c1 = min(max(c.cu[b1], c0), c.tokens);
-  return SharedPart{b0, c0, c1, __builtin_amdgcn_readfirstlane(keys / unit * unit)};
+  return __builtin_amdgcn_readfirstlane(keys / unit * unit);
 }
-// keys that sequence b leaves to its group
-__device__ __forceinline__ int keys_shared(const PagedParams & p, int b)
+// of group g, or where that is -1 of sequence b's group (no keys if it has none)
+__device__ __forceinline__ SharedPart shared_part(const PagedParams & p, int g, int b)
 {
-  if (p.groups == 0) return 0;
-  const int g = find_seq(p.groups, b, [&](int i) { return (long)p.member[i]; });
-  return p.member[g] <= b && b < p.member[g + 1] ? shared_part(p, g).keys : 0;
+  const CacheParams & c = p.c;
+  const int lane = threadIdx.x & 63;
+  auto seq = [&](int i) { return min(max(i, 0), c.batch); };
+  auto row = [&](int i) { return min(max(i, 0), c.tokens); };
+  if (p.groups < 64 && c.batch <= 128) {
+    // what is read does not wait for one another: a trip to memory instead of four
+    const int m = p.member[min(lane, p.groups)], s = p.shared[min(lane, p.groups - 1)];
+    int r0[2], r1[2], len[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = min(lane + 64 * i, c.batch - 1);
+      r0[i] = c.cu[at];
+      r1[i] = c.cu[at + 1];
+      len[i] = c.lens[at];
+    }
+    if (g < 0) {
+      const unsigned long long below = __ballot(lane < p.groups && m <= b);
+      if (below == 0) return SharedPart{0, 0, 0, 0};
+      g = 63 - __clzll(below);
+      if (b >= __builtin_amdgcn_readlane(m, g + 1)) return SharedPart{0, 0, 0, 0};
+    }
+    const int b0 = seq(__builtin_amdgcn_readlane(m, g)), b1 = max(seq(__builtin_amdgcn_readlane(m, g + 1)), b0);
+    if (b1 == b0) return SharedPart{0, 0, 0, 0};
+    int keys = min(max(__builtin_amdgcn_readlane(s, g), 0), c.width * c.page);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = lane + 64 * i, c0 = row(r0[i]), n = max(row(r1[i]), c0) - c0;
+      if (at >= b0 && at < b1 && n > 0) keys = min(keys, max(max(len[i], 0) - n + 1, 0));
+    }
+    const int c0 = row(b0 < 64 ? __builtin_amdgcn_readlane(r0[0], b0) : __builtin_amdgcn_readlane(r0[1], b0 - 64));
+    const int c1 = row(b1 <= 64 ? __builtin_amdgcn_readlane(r1[0], b1 - 1) : __builtin_amdgcn_readlane(r1[1], b1 - 65));
+    return SharedPart{b0, c0, max(c1, c0), whole_keys(c, keys)};
+  }
+  if (g < 0) {
+    g = find_seq(p.groups, b, [&](int i) { return (long)p.member[i]; });
+    if (p.member[g] > b || b >= p.member[g + 1]) return SharedPart{0, 0, 0, 0};
+  }
+  const int b0 = seq(p.member[g]), b1 = max(seq(p.member[g + 1]), b0);
+  int keys = min(max(p.shared[g], 0), c.width * c.page);
+  for (int i = b0 + lane; i < b1; i += 64) {
+    const int c0 = row(c.cu[i]), n = max(row(c.cu[i + 1]), c0) - c0;
+    if (n > 0) keys = min(keys, max(max(c.lens[i], 0) - n + 1, 0));
+  }
+  const int c0 = row(c.cu[b0]);
+  return SharedPart{b0, c0, max(row(c.cu[b1]), c0), whole_keys(c, keys)};
 }
 
 }  // namespace
+
+// A group's shared keys for 32 rows (prefix_attn.hpp).
+template <int TYPE, int BITS, int DP, bool FULL> __device__ __forceinline__ void shared_rows(const PagedParams & p, int block, float * lds);
 
 // QT: 16-row tiles of a wave; WK: waves that share rows and split the keys, 4 / WK row ranges.
 // DP: head size rounded up to 64, 128 or 256; FULL: it is that size.
 template <int TYPE, int BITS, int DP, bool FULL, int QT, int WK, int KEYS>
 __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(const PagedParams p, int units)
 {
-  const bool shared = KEYS == kSharedKeys || (KEYS == kBothKeys && (int)blockIdx.x < p.shared_wgs);
-  const int block = blockIdx.x - (KEYS == kBothKeys && !shared ? p.shared_wgs : 0);
+  extern __shared__ __attribute__((aligned(16))) float lds[];
+  constexpr bool BOTH = KEYS == kBothKeys || KEYS == kBothWide;
+  const bool shared = KEYS == kSharedKeys || (BOTH && (int)blockIdx.x < p.shared_wgs);
+  const int block = blockIdx.x - (BOTH && !shared ? p.shared_wgs : 0);
+  if constexpr (KEYS == kBothWide) {
+    if (shared) {
+      shared_rows<TYPE, BITS, DP, FULL>(p, block, lds);
+      return;
+    }
+  }
   const int row_slots = KEYS == kBothKeys && shared ? p.shared_slots : p.row_slots;
   const int parts = KEYS == kBothKeys && shared ? p.lead : p.parts, part_steps = KEYS == kBothKeys && shared ? p.shared_steps : p.part_steps;
   using T = St<TYPE>;
@@ -113,7 +159,6 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
   // numbers then and the largest is below 2^15; in bf16 small ones stay above fp32's lowest exponent
   // where pages' scales are 2^120 for the type's largest values and 2^-32 for zeros
   constexpr int UP = TYPE == kSeqF16 ? 7 : BITS == 8 ? 64 : 0;
-  extern __shared__ __attribute__((aligned(16))) float lds[];
 
   const CacheParams & c = p.c;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -126,7 +171,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
   const int slot = w % row_slots;
   w = w / row_slots * kXcds + block % kXcds;
   const int seqs = (KEYS != kAllKeys && shared ? p.groups : c.batch) * c.heads;
-  if (w >= (KEYS == kBothKeys ? seqs * parts : units)) return;
+  if (w >= (BOTH ? seqs * parts : units)) return;
   const int part = w / seqs;
   w -= part * seqs;
   const int h = w % c.heads, b = w / c.heads;
@@ -134,7 +179,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
   int c0, c1, full, place0, skip = 0;  // place0: of the first new token
   const int32_t * table = c.table;
   if (KEYS != kAllKeys && shared) {
-    const SharedPart part_of = shared_part(p, b);
+    const SharedPart part_of = shared_part(p, b, 0);
     if (part_of.keys == 0) return;
     c0 = part_of.c0;
     c1 = part_of.c1;
@@ -147,7 +192,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
     full = (int)min(max(len, 0L), (long)c.width * c.page);
     place0 = (int)max(len, 0L) - (c1 - c0);
     table += (long)b * c.width;
-    if (KEYS != kAllKeys) skip = keys_shared(p, b);
+    if (KEYS != kAllKeys && p.groups > 0) skip = shared_part(p, -1, b).keys;
   }
   const int nnew = c1 - c0, rows = nnew * p.group;
   const int lp = 31 - __clz(c.page);  // page is a power of two
@@ -599,9 +644,10 @@ namespace {
 template <int TYPE, int BITS, int DP, bool FULL, int QT, int WK, int KEYS> void launch_paged(const PagedParams & p, hipStream_t s)
 {
   auto kern = paged_attn_kernel<TYPE, BITS, DP, FULL, QT, WK, KEYS>;
-  const size_t lds = (size_t)(WK / 2) * (4 / WK) * 16 * QT * (DP + 4 + 2) * sizeof(float);
+  const size_t own = (size_t)(WK / 2) * (4 / WK) * 16 * QT * (DP + 4 + 2) * sizeof(float), wide = (size_t)2 * 32 * (DP + 4 + 2) * sizeof(float);
+  const size_t lds = KEYS == kBothWide ? std::max(own, wide) : own;
   const long units = (long)(KEYS == kSharedKeys ? p.groups : p.c.batch) * p.c.heads * p.parts;
-  const dim3 grid((unsigned)((units + kXcds - 1) / kXcds * kXcds * p.row_slots + (KEYS == kBothKeys ? p.shared_wgs : 0))), blk(256);
+  const dim3 grid((unsigned)((units + kXcds - 1) / kXcds * kXcds * p.row_slots + (KEYS == kBothKeys || KEYS == kBothWide ? p.shared_wgs : 0))), blk(256);
   hipLaunchKernelGGL(kern, grid, blk, lds, s, p, (int)units);
 }
 
@@ -624,6 +670,7 @@ template <int TYPE, int BITS, int KEYS = kAllKeys> void launch_paged_dim(const P
   else if (p.c.dim < 64) launch_paged_rows<TYPE, BITS, 64, false, KEYS>(p, s);
   else if (p.c.dim == 128) launch_paged_rows<TYPE, BITS, 128, true, KEYS>(p, s);
   else if (p.c.dim < 128) launch_paged_rows<TYPE, BITS, 128, false, KEYS>(p, s);
+  else if constexpr (KEYS == kBothWide) throw std::logic_error("head size");
   else if (p.c.dim == 256) launch_paged_rows<TYPE, BITS, 256, true, KEYS>(p, s);
   else launch_paged_rows<TYPE, BITS, 256, false, KEYS>(p, s);
 }

@@ -4,11 +4,21 @@
 //
 // with (m1, l1, o1) the maximum, sum and weighted values over the group's shared keys and (m2, l2, o2) those over
 // the sequence's own: the shared keys are read once for the rows of all sequences, which are contiguous.
-// Shared keys, own keys, and the join of all parts.  Own keys, and shared ones with few rows, take
-// the paged attention's kernel; with many rows the matrix cores bound the shared keys:
-//   * a work-group has 128 rows of a key head, a wave 32 of them, and walks 64 keys a step.  The steps' keys and values
-//     stand in LDS in two stages, in 16 bits, each 1024 bytes a fragment of 32 x 32 x 16 MFMA in the order of its lanes: they are
-//     read without a bank conflict, and 8-bit codes are widened once for the four waves;
+// All parts are joined by a kernel behind them.  Own keys take the paged attention's kernel; shared ones
+//   * for up to 16 rows of a group (95 with heads of more than 64 channels), and where heads have more than 128, that
+//     kernel as well, in work-groups of the same launch where the tiles agree.  With few rows the keys' latency counts:
+//     32 rows of 128 channels behind 2048 tokens 15 us so, 18 by 32 rows a wave;
+//   * by 32 rows (shared_rows), in the same launch: each key that L2 gives has twice the rows of that kernel's tiles.
+//     64 sequences of 4 rows a key head behind 8192 tokens, own keys of 20 to 1501, 8 bits: 52 -> 45 us, the kernel 34,
+//     of which the keys' 94 MB are 18 at a copy's rate; 5 groups of 112 rows behind 700 to 6007 tokens in 16 bits 53 -> 37 us;
+//     24 rows of 64 channels behind 1024 tokens 18 -> 13 us;
+//   * with many rows of up to 64 channels behind a long prefix the keys' conversion and L2 bound that: a work-group has 128
+//     rows, a wave 32 of them, and walks 64 keys a step (shared_attn_kernel).  The steps' keys and values stand in LDS in two
+//     stages, in 16 bits, each 1024 bytes a fragment of 32 x 32 x 16 MFMA in the order of its lanes: they are read without a
+//     bank conflict, and 8-bit codes are widened once for the four waves.  1536 rows a key head behind 32000 tokens: 180 us,
+//     0.56 PFLOP/s; behind 16384 120 us in all, 127 by shared_rows, behind 8192 81 and 73.  With 128 channels the accumulators leave two
+//     waves a SIMD and the barriers cost more than the copies save: 768 rows behind 32768 tokens 234 us, 191 by shared_rows.
+// Both:
 //   * S^T = K Q^T with keys in rows in an order of which a lane holds, of a 32-key part, the 16 keys of one granule
 //     (8-bit pages) or two runs of 8 (16-bit): they are operands of O^T = V^T P^T as they are;
 //   * weights, running maxima and scales as in paged_attn.hpp; nothing is masked but pages that hold nothing.
@@ -46,9 +56,9 @@ constexpr int kSharedRows = 128;
 
 }  // namespace
 
-// DP: head size rounded up to 64, 128 or 256; FULL: it is that size.
+// DP: head size rounded up to 64; FULL: it is that size.
 template <int TYPE, int BITS, int DP, bool FULL>
-__global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) shared_attn_kernel(const PagedParams p, int units)
+__global__ void __launch_bounds__(256, 2) shared_attn_kernel(const PagedParams p, int units)
 {
   using T = St<TYPE>;
   typedef typename T::e E;
@@ -73,7 +83,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) shared_attn_kernel(con
   const int seqs = p.groups * c.heads, part = w / seqs;
   w -= part * seqs;
   const int h = w % c.heads;
-  const SharedPart own = shared_part(p, w / c.heads);
+  const SharedPart own = shared_part(p, w / c.heads, 0);
   if (own.keys == 0) return;
   const int c0 = own.c0, rows = (own.c1 - c0) * p.group;
   const int32_t * table = c.table + (long)own.first * c.width;
@@ -302,6 +312,241 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) shared_attn_kernel(con
   }
 }
 
+// 32 rows of a key head, the four waves taking every fourth 32 keys: fragments straight from the cache into registers, in
+// the order of shared_attn_kernel's; what the waves have is joined through LDS.  A tile of 16 rows, as the paged attention
+// has it, reads the shared keys from L2 twice as often, which bounds it (64 sequences of 4 rows a key head behind 8192
+// tokens: 0.27 GB, 11 TB/s).
+template <int TYPE, int BITS, int DP, bool FULL> __device__ __forceinline__ void shared_rows(const PagedParams & p, int block, float * lds)
+{
+  using T = St<TYPE>;
+  typedef typename T::e E;
+  constexpr int EK = BITS == 8 ? 16 : 8;
+  constexpr int KF = DP / (2 * EK), VS = BITS == 8 ? 1 : 2, NB = DP / 32, NS = DP / 16;
+  constexpr int UP = TYPE == kSeqF16 ? 7 : BITS == 8 ? 64 : 0;
+  const CacheParams & c = p.c;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  int w = block / kXcds;
+  const int slot = w % p.shared_slots;
+  w = w / p.shared_slots * kXcds + block % kXcds;
+  const int seqs = p.groups * c.heads, part = w / seqs;
+  if (part >= p.lead) return;
+  w -= part * seqs;
+  const int h = w % c.heads;
+  const SharedPart own = shared_part(p, w / c.heads, 0);
+  if (own.keys == 0) return;
+  const int c0 = own.c0, rows = (own.c1 - c0) * p.group;
+  const int32_t * table = c.table + (long)own.first * c.width;
+  const int lp = 31 - __clz(c.page), last = (own.keys >> lp) - 1;
+  const long page_bytes = (long)c.page * c.dim * (BITS / 8);
+  const int total = own.keys / 64, per = max(p.shared_steps, (total + p.lead - 1) / p.lead);
+  const int t0 = 2 * min(total, part * per), t1 = 2 * min(total, part * per + per);  // 32 keys each
+  const float scale = fmaxf(fabsf(p.scale_log2), 1.2e-38f);
+  const unsigned flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
+  const int mi = col >> 3, mh = col >> 2 & 1, mj = col & 3;
+  const int key_gran = BITS == 8 ? mh : mi >> 1, key_quad = BITS == 8 ? mi : 2 * mh + (mi & 1);
+  const unsigned key_lane = (unsigned)(key_quad * (c.dim / EK) * 64 + mj * 16), gran_bytes = 16u * c.dim * (BITS / 8);
+
+  auto page_at = [&](int t, int gran) { return table[min((32 * t + 16 * gran) >> lp, last)]; };
+  auto valid = [&](int id) { return (unsigned)id < (unsigned)c.pages; };
+  auto granule = [&](int id, int t, int gran) {  // its first byte among the keys, or values, of all pages
+    return ((long)(valid(id) ? id : 0) * c.heads + h) * page_bytes + ((32 * t + 16 * gran) & (c.page - 1)) / 16 * gran_bytes;
+  };
+
+  for (int tile = slot; tile * 32 < rows; tile += p.shared_slots) {
+    const int row = tile * 32 + col;
+    u4v qf[NS];
+    {
+      const int there = min(row, rows - 1), tok = there / p.group;
+      const E * q = static_cast<const E *>(p.q) + (long)(c0 + tok) * p.q_token + (long)(h * p.group + there - tok * p.group) * p.q_head;
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        const int ch = BITS == 8 ? 16 * (2 * (i / 2) + half) + 8 * (i % 2) : 16 * i + 8 * half;
+        qf[i] = *reinterpret_cast<const u4v *>(q + (FULL || ch < c.dim ? ch : 0));
+      }
+    }
+    f16v o[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) o[j] = f16v{};
+    float M = kLowest, L = 0.0f;
+    u4v kf[KF], vf[VS * NB];
+    auto load_k = [&](int t, int id0, int id1) __attribute__((always_inline)) {
+      const uint8_t * k = static_cast<const uint8_t *>(c.kc) + granule(key_gran ? id1 : id0, t, key_gran) + key_lane;
+#pragma unroll
+      for (int i = 0; i < KF; ++i) kf[i] = *reinterpret_cast<const u4v *>(k + (unsigned)(FULL ? 2 * i + half : min(2 * i + half, c.dim / EK - 1)) * 64u);
+    };
+    float ks = 1.0f, vs = 1.0f;
+    auto load_v = [&](int t, int id0, int id1) __attribute__((always_inline)) {
+      if constexpr (BITS == 8) {
+        const int id = half ? id1 : id0;
+        const long page = (long)(valid(id) ? id : 0) * c.heads + h;
+        ks = c.ks[page];
+        vs = c.vs[page];
+        const uint8_t * v = static_cast<const uint8_t *>(c.vc) + granule(id, t, half);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) vf[j] = *reinterpret_cast<const u4v *>(v + (unsigned)(FULL ? 32 * j + col : min(32 * j + col, c.dim - 1)) * 16u);
+      } else {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const uint8_t * v = static_cast<const uint8_t *>(c.vc) + granule(s ? id1 : id0, t, s) + half * c.dim * 16;
+#pragma unroll
+          for (int j = 0; j < NB; ++j) vf[s * NB + j] = *reinterpret_cast<const u4v *>(v + (unsigned)(FULL ? 32 * j + col : min(32 * j + col, c.dim - 1)) * 16u);
+        }
+      }
+    };
+    int id0 = 0, id1 = 0, next0 = 0, next1 = 0;
+    int t = t0 + wave;
+    if (t < t1) {
+      id0 = page_at(t, 0);
+      id1 = page_at(t, 1);
+      const int ahead = min(t + 4, t1 - 1);
+      next0 = page_at(ahead, 0);
+      next1 = page_at(ahead, 1);
+      load_k(t, id0, id1);
+      load_v(t, id0, id1);
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        const int ch = BITS == 8 ? 16 * (2 * (i / 2) + half) + 8 * (i % 2) : 16 * i + 8 * half;
+        qf[i] = FULL || ch < c.dim ? qf[i] ^ flip : u4v{0, 0, 0, 0};
+      }
+    }
+    for (; t < t1; t += 4) {
+      const bool more = t + 4 < t1;
+      f16v s;
+#pragma unroll
+      for (int i = 0; i < KF; ++i) {
+        u4v x = kf[i];
+        if (!FULL && (2 * i + half) * EK >= c.dim) x = u4v{0, 0, 0, 0};
+        if constexpr (BITS == 8) {
+          s = T::mma32(u4v{T::fp8_lo(x[0]), T::fp8_hi(x[0]), T::fp8_lo(x[1]), T::fp8_hi(x[1])}, qf[2 * i], i ? s : f16v{});
+          s = T::mma32(u4v{T::fp8_lo(x[2]), T::fp8_hi(x[2]), T::fp8_lo(x[3]), T::fp8_hi(x[3])}, qf[2 * i + 1], s);
+        } else {
+          s = T::mma32(x, qf[i], i ? s : f16v{});
+        }
+      }
+      const bool ok0 = valid(id0), ok1 = valid(id1), whole = ok0 && ok1;
+      float k1 = ks, v1 = BITS == 8 ? fmaxf(vs, 1e-30f) : 1.0f;
+      const int after = min(t + 8, t1 - 1);
+      if (more) {
+        load_k(t + 4, next0, next1);
+        id0 = next0;
+        id1 = next1;
+        next0 = page_at(after, 0);
+        next1 = page_at(after, 1);
+      }
+      if (!whole) {
+        if (BITS == 8 && !(half ? ok1 : ok0)) k1 = v1 = 1.0f;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[v] = (BITS == 8 ? (half ? ok1 : ok0) : v < 8 ? ok0 : ok1) ? s[v] : -__builtin_inff();
+      }
+      const float mul = BITS == 8 ? fmaxf(scale * k1, 1.2e-38f) : scale, ev = BITS == 8 ? __builtin_amdgcn_logf(v1) : 0.0f;
+      float a = s[0], d = s[1];
+#pragma unroll
+      for (int v = 2; v < 16; v += 4) {
+        a = top_of(a, s[v], s[v + 1]);
+        if (v + 2 < 16) d = top_of(d, s[v + 2], s[v + 3]);
+      }
+      const float top = across32(fmaf(top_of(a, d, d), mul, ev), MaxOp());
+      if (__any(top > M + 8.0f)) {
+        const float m = fmaxf(M, top), e = __builtin_amdgcn_exp2f(M - m);
+        M = m;
+        L *= e;
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) o[j][v] *= e;
+      }
+      const float shift = ev + UP - M;
+      u4v pf[2];
+      float sum = 0.0f, sum2 = 0.0f;
+#pragma unroll
+      for (int v = 0; v < 16; v += 2) {
+        const float e0 = __builtin_amdgcn_exp2f(fmaf(s[v], mul, shift)), e1 = __builtin_amdgcn_exp2f(fmaf(s[v + 1], mul, shift));
+        const unsigned e = pack2<TYPE>(e0, e1);
+        pf[v / 8][v % 8 / 2] = e;
+        if (TYPE == kSeqF16 && BITS == 8) {
+          sum += e0;
+          sum2 += e1;
+        } else {
+          sum = T::add2(e, sum);
+        }
+      }
+      if (BITS == 8)
+        L += __builtin_ldexpf((sum + sum2) * __builtin_amdgcn_rcpf(__builtin_amdgcn_frexp_mantf(v1)), -UP - __builtin_amdgcn_frexp_expf(v1));
+      else L = fmaf(sum, __builtin_ldexpf(1.0f, -UP), L);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        u4v x0, x1;
+        if constexpr (BITS == 8) {
+          u4v x = vf[j];
+          if (!whole && !(half ? ok1 : ok0)) x = u4v{0, 0, 0, 0};  // values of a page that holds nothing may be anything
+          x0 = u4v{T::fp8_lo(x[0]), T::fp8_hi(x[0]), T::fp8_lo(x[1]), T::fp8_hi(x[1])};
+          x1 = u4v{T::fp8_lo(x[2]), T::fp8_hi(x[2]), T::fp8_lo(x[3]), T::fp8_hi(x[3])};
+        } else {
+          x0 = ok0 ? vf[j] : u4v{0, 0, 0, 0};
+          x1 = ok1 ? vf[NB + j] : u4v{0, 0, 0, 0};
+        }
+        o[j] = T::mma32(x0, pf[0], o[j]);
+        o[j] = T::mma32(x1, pf[1], o[j]);
+      }
+      if (more) load_v(t + 4, id0, id1);
+    }
+    L = across32(L, SumOp());
+
+    // ---- the waves' sums are joined as in paged_attn.hpp
+    constexpr int PITCH = DP + 4;
+    f2v * ml = reinterpret_cast<f2v *>(lds + 2 * 32 * PITCH);
+#pragma unroll
+    for (int hw = 2; hw >= 1; hw /= 2) {
+      float * mine = lds + (wave % hw) * 32 * PITCH + col * PITCH + 4 * half;
+      __syncthreads();
+      if (wave >= hw && wave < 2 * hw) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const f4v y = {o[j][4 * i], o[j][4 * i + 1], o[j][4 * i + 2], o[j][4 * i + 3]};
+            *reinterpret_cast<f4v *>(mine + 32 * j + 8 * i) = y;
+          }
+        if (half == 0) ml[(wave % hw) * 32 + col] = f2v{M, L};
+      }
+      __syncthreads();
+      if (wave < hw) {
+        const f2v y = ml[wave * 32 + col];
+        const float m = fmaxf(M, y[0]), a = __builtin_amdgcn_exp2f(M - m), e = __builtin_amdgcn_exp2f(y[0] - m);
+        M = m;
+        L = L * a + y[1] * e;
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const f4v x = *reinterpret_cast<const f4v *>(mine + 32 * j + 8 * i);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) o[j][4 * i + v] = o[j][4 * i + v] * a + x[v] * e;
+          }
+      }
+    }
+    if (wave == 0 && row < rows) {
+      const int tok = row / p.group, head = h * p.group + row - tok * p.group;
+      const long all = (long)c.tokens * p.heads, at = (long)part * all + (long)(c0 + tok) * p.heads + head;
+      if (t0 < t1) {
+        float * out = p.ws + at * c.dim;
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int ch = 32 * j + 8 * i + 4 * half;
+            f4v y = {o[j][4 * i], o[j][4 * i + 1], o[j][4 * i + 2], o[j][4 * i + 3]};
+            if (UP) y *= __builtin_ldexpf(1.0f, -UP);
+            if (FULL || ch < c.dim) *reinterpret_cast<f4v *>(out + ch) = y;
+          }
+      }
+      if (half == 0) reinterpret_cast<f2v *>(p.ws + p.all_parts * all * c.dim)[at] = f2v{M, L};
+    }
+    __syncthreads();  // LDS is read before the next tile's waves write it
+  }
+}
+
 namespace {
 
 template <int TYPE, int BITS, int DP, bool FULL> void launch_shared(const PagedParams & p, hipStream_t s)
@@ -314,17 +559,14 @@ template <int TYPE, int BITS, int DP, bool FULL> void launch_shared(const PagedP
 template <int TYPE, int BITS> void launch_shared_dim(const PagedParams & p, hipStream_t s)
 {
   if (p.c.dim == 64) launch_shared<TYPE, BITS, 64, true>(p, s);
-  else if (p.c.dim < 64) launch_shared<TYPE, BITS, 64, false>(p, s);
-  else if (p.c.dim == 128) launch_shared<TYPE, BITS, 128, true>(p, s);
-  else if (p.c.dim < 128) launch_shared<TYPE, BITS, 128, false>(p, s);
-  else if (p.c.dim == 256) launch_shared<TYPE, BITS, 256, true>(p, s);
-  else launch_shared<TYPE, BITS, 256, false>(p, s);
+  else launch_shared<TYPE, BITS, 64, false>(p, s);
 }
 
 template <int TYPE, int BITS> void launch_prefix_keys(const PrefixParams & p, hipStream_t s)
 {
   if (p.both) {
-    launch_paged_dim<TYPE, BITS, kBothKeys>(p.own, s);
+    if (p.wide) launch_paged_dim<TYPE, BITS, kBothWide>(p.own, s);
+    else launch_paged_dim<TYPE, BITS, kBothKeys>(p.own, s);
     return;
   }
   if (p.own.lead > 0) {

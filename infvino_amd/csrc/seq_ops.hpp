@@ -87,7 +87,8 @@ void launch_paged_bf16(const PagedParams & p, hipStream_t s);  // its bf16 kerne
 struct PrefixParams {
   PagedParams first, own;
   int many = 0;  // shared keys by work-groups of 128 rows
-  int both = 0;  // both kinds of keys in one launch
+  int both = 0;  // both kinds of keys in one launch,
+  int wide = 0;  // shared ones for 32 rows at a time, else as the paged attention does
 };
 size_t prefix_split(PrefixParams & p, int max_new, int max_len, int max_shared);
 void launch_prefix_attention(const PrefixParams & p, hipStream_t s);

@@ -155,6 +155,48 @@ def test_prefix_attention_groups_and_lengths_of_every_kind(bits, hints, heads, k
             row += 1
 
 
+LONG = (0, 0, 16384)  # rows of 512 and more, of up to 64 channels, taken 128 at a time
+PREFIX_LONG = [
+    (8, 64, 2, 64, 64, [20], [1000], [1] * 20, [1 + 3 * i for i in range(20)], LONG),
+    (8, 64, 1, 48, 16, [18, 16], [129, 65], [1] * 34, [1 + i % 5 for i in range(34)], LONG),
+    (16, 64, 2, 64, 64, [20], [1000], [1] * 20, [1 + 3 * i for i in range(20)], LONG),
+    (16, 64, 1, 48, 16, [18, 16], [129, 65], [1] * 34, [1 + i % 5 for i in range(34)], LONG),
+    (8, 64, 1, 16, 128, [33], [16500], [1] * 33, [1] * 33, FEW),
+    (8, 8, 2, 128, 16, [30], [2100], [1] * 30, [1 + i for i in range(30)], FEW),  # 120 rows: 32 at a time
+    (16, 6, 1, 112, 32, [17, 16], [700, 65], [1] * 33, [1 + i for i in range(33)], FEW),
+]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("bits,heads,kv,dim,page,sizes,shared,new,own,hints", PREFIX_LONG)
+def test_prefix_attention_long(t, bits, heads, kv, dim, page, sizes, shared, new, own, hints):
+    g = _gen(dim + len(own))
+    s = Shared(g, t, bits, kv, dim, page, sizes, shared, new, own)
+    q = _randn(g, s.cache.dt, sum(new) + 3, heads, dim)
+    s.check(q, s.run(q, heads, hints=hints))
+
+
+@pytest.mark.parametrize("hints,dim", [(LONG, 64), (FEW, 64), (FEW, 128)])
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("scale", [0.25, -0.25, 0.0])
+def test_prefix_attention_pages_that_hold_nothing(bits, hints, dim, scale):
+    """Among the shared ones, whatever their bytes are; softmax scales of each sign."""
+    g = _gen(31)
+    s = Shared(g, "f16", bits, 1, dim, 16, [12], [400], [1] * 12, [1 + 9 * i for i in range(12)])
+    for i in range(12):
+        s.table[i][3] = -1
+        s.table[i][4] = s.cache.pages
+        s.table[i][17] = 1 << 30
+    q = _randn(g, torch.float16, 12, 64, dim)
+    got = s.run(q, 64, hints=hints, scale=scale)
+    for b, m in enumerate(s.lens):
+        ids = s.table[b][:-(-m // 16)]
+        ks, vs = s.cache.rows([max(0, min(i, s.cache.pages - 1)) for i in ids], m)
+        ok = torch.tensor([0 <= i < s.cache.pages for i in ids], device="cuda").repeat_interleave(16)[:m]
+        r, av, err = seq._attend(q[b:b + 1], ks[ok], vs[ok], torch.tensor([int(ok.sum())], device="cuda"), True, 0, 0, scale)
+        seq._close(got[b:b + 1], r, av, err, s.cache.u, m, vs[ok].abs().max())
+
+
 @pytest.mark.parametrize("hints,heads", [(FEW, 8), (MANY, 64)])
 @pytest.mark.parametrize("bits", [8, 16])
 def test_prefix_attention_odd_values_stay_with_their_rows(bits, hints, heads):
