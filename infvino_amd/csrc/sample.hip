@@ -16,6 +16,10 @@
 // and a last kernel, a work-group a row, finds the cut among the listed ones by digits of their codes, adds
 // them to their pieces' sums, and reads the one piece that u falls in.  Where more than 8192 tokens fall into those
 // bins, as in rows of equal logits, it reads the row itself instead.
+//
+// One row of 131072 fp32 logits: 42 us, four kernels of 26 in all and the gaps between them; a sort of the row in one work-group takes
+// 855.  96 rows 70 us (list 27, bins 21, last 17, top 6), 320 rows of 200000 fp32 logits 269 us (106, 87, 36, 40), of which the
+// bytes are 150 at three passes: the exponentials in 64 bits and the vector unit bound the others.
 #include <algorithm>
 #include <cmath>
 #include <stdexcept>
@@ -800,7 +804,7 @@ size_t sample_split(SampleParams & p)
   p.pieces = (p.vocab + kPiece - 1) / kPiece;
   p.parts = p.per = 0;
   if (p.vocab <= kList || p.rows == 0) return 0;
-  // eight work-groups a CU, of whole pieces
+  // eight work-groups a CU, of whole pieces (320 rows of 200000: 269 us, four 322, sixteen 264; 96 rows 70, 70, 72)
   const int want = std::min(p.pieces, (2048 + p.rows - 1) / p.rows);
   p.per = (p.pieces + want - 1) / want;
   p.parts = (p.pieces + p.per - 1) / p.per;
