@@ -164,6 +164,12 @@ PREFIX_LONG = [
     (8, 64, 1, 16, 128, [33], [16500], [1] * 33, [1] * 33, FEW),
     (8, 8, 2, 128, 16, [30], [2100], [1] * 30, [1 + i for i in range(30)], FEW),  # 120 rows: 32 at a time
     (16, 6, 1, 112, 32, [17, 16], [700, 65], [1] * 33, [1 + i for i in range(33)], FEW),
+    # more groups, and more sequences, than lanes look at together
+    (8, 4, 2, 64, 16, [2] * 70, [64 + 16 * i for i in range(70)], [1 + i % 2 for i in range(140)], [2 + i % 40 for i in range(140)], FEW),
+    (16, 4, 2, 128, 16, [100, 33], [200, 70], [1] * 133, [1 + i % 40 for i in range(133)], FEW),
+    (8, 4, 2, 64, 16, [63, 65], [200, 70], [1] * 128, [1 + i % 40 for i in range(128)], FEW),
+    (8, 4, 2, 64, 16, [1] * 63, [64 + 16 * i for i in range(63)], [1] * 63, [2] * 63, FEW),
+    (8, 4, 2, 64, 16, [1] * 64, [64 + 16 * i for i in range(64)], [1] * 64, [2] * 64, FEW),
 ]
 
 
