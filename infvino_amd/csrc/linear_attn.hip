@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
   float * first = p.ws + ((long)u * p.heads + h) * one;
 
   f16v s[ND];
-  float held = 1.0f;  // fp16: what the column is held times, a power of two, so that the parts below are normal numbers
+  int held = 0;  // fp16: the column is held times 2^held, so that the parts below are normal numbers
   auto state_io = [&](float * at, auto store) __attribute__((always_inline)) {  // channels that are not there: zeros, nowhere
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(at, (short)0, (int)(one * 4), kBufDword3);
 #pragma unroll
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
       for (int v = 0; v < 16; ++v) {
         const int dk = 32 * d + result_row(v, half);
         const unsigned off = dv < p.dim ? (unsigned)(dk * p.dim + dv) * 4u : kBufOOB;  // rows from key_dim on lie behind the end
-        const float x = TYPE == kSeqF16 ? s[d][v] / held : s[d][v];  // by itself: a bit cast of an element is one of the vector's start
+        const float x = TYPE == kSeqF16 ? __builtin_ldexpf(s[d][v], -held) : s[d][v];  // by itself: a bit cast of an element is one of the vector's start
         if (store) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x), r, (int)off, 0, 0);
         else s[d][v] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, (int)off, 0, 0));
       }
@@ -385,6 +385,7 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
     }
     f16v acc[2];
     float fit = 1.0f, back = 1.0f;  // fp16: what brings this lane's column of the state to about 2^14, and what it comes back by
+    float top = 0.0f;               // fp16: the column's largest, as it is held
     auto from_state = [&]() __attribute__((always_inline)) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) acc[t] = f16v{};
@@ -438,7 +439,7 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
         }
         if constexpr (TYPE == kSeqF16) {  // the largest of a row's to about 2^14, so that none overflows and small ones count
           most = across32(most, MaxOp());
-          const int e = min(max(__builtin_amdgcn_frexp_expf(most) - 14, -40), 60);
+          const int e = max(__builtin_amdgcn_frexp_expf(most) - 14, -100);
 #pragma unroll
           for (int i = 0; i < 16; ++i) x[i] = __builtin_ldexpf(x[i], -e);
           if (half == 0) its.unit[s0 / 32][t0 + col] = __builtin_ldexpf(1.0f, e);
@@ -452,16 +453,18 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
     }
     if (wave == 3 && more) decays(c + 1, decay_then);
     if (on) {
+      if constexpr (TYPE == kSeqF16) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) top = fmaxf(top, fabsf(s[d][x]));
+        top = across32(top, MaxOp());
+      }
       if constexpr (OUT) {
         if constexpr (TYPE == kSeqF16) {
-          float most = 0.0f;
-#pragma unroll
-          for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int x = 0; x < 16; ++x) most = fmaxf(most, fabsf(s[d][x]));
-          most = across32(most, MaxOp());
-          fit = __builtin_ldexpf(1.0f, min(max(14 - __builtin_amdgcn_frexp_expf(most), -100), 100));
-          back = 1.0f / (fit * held);
+          const int e = min(14 - __builtin_amdgcn_frexp_expf(top), 100);
+          fit = __builtin_ldexpf(1.0f, e);
+          back = __builtin_ldexpf(1.0f, -e - held);
         }
         from_state();
       }
@@ -494,24 +497,23 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
       lds_barrier();
       if (on) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          float back = 1.0f;
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int z = 0; z <= t; ++z) {  // halves of the keys
-            if constexpr (TYPE == kSeqF16) {
-              const float mine = its.unit[z][32 * t + col], f = back / mine;
+            // fp16: by itself, since neither half's units need hold the state's part or the other half's
+            f16v sum = {};
 #pragma unroll
-              for (int x = 0; x < 16; ++x) acc[t][x] *= f;
-              back = mine;
+            for (int j = 2 * z; j < 2 * z + 2; ++j) {
+              const u4v x = *reinterpret_cast<const u4v *>(P + (32 * t + col) * PP + 16 * j + 8 * half);
+              if constexpr (TYPE == kSeqF16) sum = T::mma32(vf[j], x, sum);
+              else acc[t] = T::mma32(vf[j], x, acc[t]);
             }
+            if constexpr (TYPE == kSeqF16) {
+              const float unit = its.unit[z][32 * t + col];
 #pragma unroll
-            for (int j = 2 * z; j < 2 * z + 2; ++j)
-              acc[t] = T::mma32(vf[j], *reinterpret_cast<const u4v *>(P + (32 * t + col) * PP + 16 * j + 8 * half), acc[t]);
+              for (int x = 0; x < 16; ++x) acc[t][x] = fmaf(sum[x], unit, acc[t][x]);
+            }
           }
-          if constexpr (TYPE == kSeqF16)
-#pragma unroll
-            for (int x = 0; x < 16; ++x) acc[t][x] *= back;
-        }
       }
       if (odd) {
 #pragma unroll
@@ -536,7 +538,8 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
     }
     // the state: values with their decays to the chunk's end in parts of 16 bits, which together have fp32's precision
     if (on) {
-      float a = its.whole[SIDE];
+      float a = its.whole[SIDE], hold = 1.0f;
+      int by = 0;  // fp16: the state is multiplied by a 2^by
       if constexpr (TYPE == kSeqF16) {
         float most = 0.0f;
 #pragma unroll
@@ -546,15 +549,22 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
             const f2v y = unpack2<TYPE>(vf[j][x]), z = *reinterpret_cast<const f2v *>(&its.left[SIDE][16 * j + 8 * half + 2 * x]);
             most = fmaxf(most, fmaxf(fabsf(y[0] * z[0]), fabsf(y[1] * z[1])));
           }
-        most = across32(most, MaxOp());
-        const float next = most > 0.0f ? __builtin_ldexpf(1.0f, min(max(14 - __builtin_amdgcn_frexp_expf(most), -2), 40)) : held;
-        a *= next / held;
+        most = fminf(across32(most, MaxOp()), 3.0e38f);
+        asm volatile("" ::: "memory");  // the decays are read again below: kept, they cost registers that spill
+        // Values with their decays to about 2^14, whether decays are below 1 or above, as far as what the column held before
+        // stays below 2^125: an infinity where it need not be would be a NaN in the second part, or a state that is lost.
+        const int grows = __builtin_amdgcn_frexp_expf(a);
+        int next = min(most > 0.0f ? 14 - __builtin_amdgcn_frexp_expf(most) : 40, 40);
+        if (top > 0.0f) next = min(next, 125 + held - __builtin_amdgcn_frexp_expf(top) - grows);
+        by = grows + next - held;
+        a = __builtin_amdgcn_frexp_mantf(a);
         held = next;
+        hold = __builtin_ldexpf(1.0f, next);
       }
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
-        for (int x = 0; x < 16; ++x) s[d][x] *= a;
+        for (int x = 0; x < 16; ++x) s[d][x] = TYPE == kSeqF16 ? __builtin_ldexpf(s[d][x] * a, by) : s[d][x] * a;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         u4v part[PARTS];
@@ -562,7 +572,10 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           unsigned z[PARTS];
-          split<TYPE>(unpack2<TYPE>(vf[j][x]), (x < 2 ? f2v{l0[2 * x], l0[2 * x + 1]} : f2v{l1[2 * x - 4], l1[2 * x - 3]}) * held, z);
+          f2v left = x < 2 ? f2v{l0[2 * x], l0[2 * x + 1]} : f2v{l1[2 * x - 4], l1[2 * x - 3]};
+          // finite, since it may meet a value of zero
+          if (TYPE == kSeqF16) left = f2v{fminf(left[0] * hold, 3.0e38f), fminf(left[1] * hold, 3.0e38f)};
+          split<TYPE>(unpack2<TYPE>(vf[j][x]), left, z);
 #pragma unroll
           for (int i = 0; i < PARTS; ++i) part[i][x] = z[i];
         }
