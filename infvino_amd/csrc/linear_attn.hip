@@ -302,12 +302,13 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
   };
 
   // Decays of chunk c, by one wave, a row a lane: sums of logarithms in 64 bits, since slow decays add up over thousands
-  // of tokens and differences are taken.  A decay below 2^-256 is 0 whatever it multiplies.
+  // of tokens and differences are taken.  A decay below 2^-4096 is held as that: 0 whatever it multiplies, also after 64 tokens
+  // whose decays are above 1.
   double total = 0.0;
   auto ask_decay = [&](int c) { return g[(long)min(c * kChunk + lane, n - 1) * p.g_token]; };
   auto decays = [&](int c, float log_decay) __attribute__((always_inline)) {
     double x = c * kChunk + lane < n ? (double)log_decay * 1.4426950408889634 : 0.0;
-    x = x < -256.0 ? -256.0 : x;
+    x = x < -4096.0 ? -4096.0 : x;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
       const double y = __shfl_up(x, d);

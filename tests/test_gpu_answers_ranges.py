@@ -95,3 +95,16 @@ def test_scores_past_every_16_bit_number(max_new):
     o, state, _ = x.run(scale=scale, max_new=max_new)
     assert (o[:90, :, 7:20] == 0).all()
     x.check(o, state, scale=scale)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("max_new", [0, 1])
+def test_what_is_forgotten_does_not_grow_again(t, max_new):
+    """A decay of 0, then decays above 1: what was before stays gone."""
+    x = Linear(_gen(64), t, 1, 1, 64, 64, [90])
+    x.state = x.state * 1e30
+    x.v[:] = 0
+    x.g[:], x.g[3] = 0.0, -math.inf
+    x.g[4:64] = 1.3
+    o, state, _ = x.run(scale=1.0, max_new=max_new)
+    assert (o[3:90] == 0).all() and (state[x.to[0]] == 0).all()
