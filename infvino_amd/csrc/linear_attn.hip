@@ -277,7 +277,8 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
   E * o = static_cast<E *>(p.o) + (long)row0 * p.o_token + (long)h * p.o_head + ch0;
   const int chunks = (n + kChunk - 1) / kChunk, width = min(128, p.dim - block * 128);
 
-  // what this lane copies: position pos of a row holds a piece of it; channels and rows that are not there become zeros
+  // what this lane copies: position pos of a row holds a piece of it; channels and rows that are not there become zeros (rows
+  // may lie on top of one another: the buffer's end alone would let in parts of others)
   auto copy = [&](const E * at, long token, int channels, int c, auto pieces, auto order, unsigned char * to) __attribute__((always_inline)) {
     const int rows = min(n - c * kChunk, kChunk);
     const unsigned bytes = (unsigned)((rows - 1) * (int)token + channels) * 2u;
@@ -287,7 +288,7 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
 #pragma unroll
     for (int i = 0; i < pieces / 4; ++i) {
       const int at16 = 64 * (wave + 4 * i) + lane, row = at16 / pieces, ch = (at16 % pieces ^ order(row)) * 8;
-      const unsigned off = ch < channels ? (unsigned)(row * (int)token + ch) * 2u : kBufOOB;
+      const unsigned off = ch < channels && row < rows ? (unsigned)(row * (int)token + ch) * 2u : kBufOOB;
       copy_to_lds(r, off, to + 1024 * (wave + 4 * i));
     }
   };

@@ -108,3 +108,17 @@ def test_what_is_forgotten_does_not_grow_again(t, max_new):
     x.g[4:64] = 1.3
     o, state, _ = x.run(scale=1.0, max_new=max_new)
     assert (o[3:90] == 0).all() and (state[x.to[0]] == 0).all()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("max_new", [0, 1])
+@pytest.mark.parametrize("which", ["k", "v", "kv", "q", "near"])
+def test_rows_on_top_of_one_another(t, max_new, which):
+    """Keys, values and queries broadcast over tokens (a stride of 0), or rows that begin 16 bytes behind one another."""
+    x = Linear(_gen(65), t, 2, 2, 64, 64, [70, 1, 64, 9])
+    n = x.q.shape[0]
+    for name in "qkv" if which == "near" else which:
+        rows = getattr(x, name)
+        setattr(x, name, rows.flatten().as_strided((n, 2, 64), (8, 64, 1)) if which == "near" else rows[:1].expand(n, -1, -1))
+    o, state, _ = x.run(max_new=max_new)
+    x.check(o, state)
