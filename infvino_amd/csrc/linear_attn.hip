@@ -611,7 +611,11 @@ __global__ void __launch_bounds__(256, DK <= 128 ? 2 : 1) linear_chunk_kernel(co
     chunk(c, even);
     if (c + 1 < chunks) chunk(c + 1, odd_one);
   }
-  if (!OUT && wave == 3 && lane == 0 && block == 0) p.decay[(long)u * p.heads + h] = (float)exp2(total);
+  if (!OUT && wave == 3 && lane == 0 && block == 0) {
+    // the decay of thousands of tokens need not be one of fp32's numbers, where what it makes of a state is: 2^e m
+    const double e = fmin(fmax(floor(total), -300.0), 250.0);
+    reinterpret_cast<f2v *>(p.decay)[(long)u * p.heads + h] = f2v{(float)exp2(total - e), (float)e};
+  }
   if (!on) return;
   if constexpr (OUT) {
     if (seg.s == seg.n - 1 && (unsigned)out < (unsigned)p.slots) state_io(p.state + ((long)out * p.heads + h) * one, store);
@@ -633,10 +637,13 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const LinearParams p)
   f4v x = *reinterpret_cast<const f4v *>(at + p.heads * one);
 #pragma unroll 4
   for (int s = 2; s < n; ++s) {
-    const float a = p.decay[(u + s - 1) * p.heads + h];
+    // in two factors, of which each is finite: a state of zeros stays one
+    const f2v decay = reinterpret_cast<const f2v *>(p.decay)[(u + s - 1) * p.heads + h];
+    const int e = (int)decay[1], e0 = e / 2;
+    const float a0 = __builtin_ldexpf(decay[0], e0), a1 = __builtin_ldexpf(1.0f, e - e0);
     f4v y = *reinterpret_cast<const f4v *>(at + s * p.heads * one);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = fmaf(a, x[j], y[j]);
+    for (int j = 0; j < 4; ++j) x[j] = fmaf(a1, a0 * x[j], y[j]);
     *reinterpret_cast<f4v *>(at + s * p.heads * one) = x;
   }
 }
@@ -697,7 +704,7 @@ size_t linear_split(LinearParams & p, int max_new)
     if (seg > cost) break;
   }
   p.seg = best ? (int)best : kMaxSeg;
-  return best ? ((size_t)p.tokens / p.seg + p.batch) * p.heads * ((size_t)p.key_dim * p.dim + 1) * sizeof(float) : 0;
+  return best ? ((size_t)p.tokens / p.seg + p.batch) * p.heads * ((size_t)p.key_dim * p.dim + 2) * sizeof(float) : 0;
 }
 
 void launch_linear_attention(const LinearParams & p, hipStream_t s)

@@ -111,7 +111,7 @@ struct LinearParams {
   // how a call is split, from linear_split
   int seg = 0;                   // tokens of a segment, 0: token by token
   float * ws = nullptr;          // first states of segments [tokens / seg + batch][heads][key_dim][dim], null: one each
-  float * decay = nullptr;       // of whole segments, behind them
+  float * decay = nullptr;       // of whole segments, behind them: a number and a power of two for each
 };
 // Sets the split of a call with at most max_new rows in a sequence; returns the workspace bytes.
 size_t linear_split(LinearParams & p, int max_new);

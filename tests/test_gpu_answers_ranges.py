@@ -54,6 +54,23 @@ def test_growing_decays_in_segments(t, heads, kh, dk, dv, lens):
 
 
 @pytest.mark.parametrize("t", TYPES)
+def test_decays_of_segments_past_fp32(t):
+    """The decay of a segment is below 2^-149, or above 2^128; a state of 2^120 and one of zeros."""
+    x = Linear(_gen(67), t, 1, 1, 64, 80, [2100, 300])
+    x.v[:] = 0
+    x.g[:] = 0
+    x.g[256:512], x.g[600:856] = -0.41, 0.38
+    x.state[0] *= 2.0 ** 120
+    o, state, need = x.run(scale=2.0 ** -122)
+    assert need > 0 and float(state[x.to[0]].abs().max()) > 0
+    x.check(o, state, scale=2.0 ** -122)
+    x.g[:] = 0.38
+    x.state[:] = 0
+    o, state, _ = x.run()
+    assert (o[:2400] == 0).all() and (state == 0).all()
+
+
+@pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("max_new", [0, 1])
 @pytest.mark.parametrize("lens", [[90, 5], [70, 130]])
 def test_values_far_from_states(t, max_new, lens):
