@@ -184,11 +184,12 @@ __device__ __forceinline__ int value_order(int r) { return (r & 3) << 1; }
 
 // 64 x 16 bytes straight into LDS: lane i's from the buffer r at its offset, zeros outside it, to `to` + 16 i.  In
 // assembler, and with barriers that wait for no copy, so that copies stay in flight: the compiler would wait for all of
-// them at a barrier and before each transposing read.
+// them at a barrier and before each transposing read.  Five wait states, which it does not count in assembler: r may have been
+// written by the vector unit just before.
 __device__ __forceinline__ void copy_to_lds(u4v r, unsigned off, void * to)
 {
 #if defined(__HIP_DEVICE_COMPILE__)
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
                :
                : "v"(off), "s"(r), "s"((unsigned)(unsigned long)(lds_ptr *)to)
                : "memory", "m0");
