@@ -655,8 +655,7 @@ template <int TYPE, int DK> void launch_linear_chunks(const LinearParams & p, hi
 {
   const int blocks = (p.dim + 127) / 128;
   const int units = p.tokens / p.seg + p.batch;
-  const long keys = (long)units * (p.heads / p.group);
-  const dim3 grid((unsigned)((keys + kXcds - 1) / kXcds * kXcds * p.group * blocks)), blk(256);
+  const dim3 grid((unsigned)linear_wgs(p)), blk(256);
   if (p.ws) {
     hipLaunchKernelGGL((linear_chunk_kernel<TYPE, DK, false>), grid, blk, 0, s, p, units, blocks);
     const int parts = (p.key_dim * p.dim + 1023) / 1024;
@@ -674,7 +673,7 @@ template <int TYPE> void launch_linear_type(const LinearParams & p, hipStream_t 
     return;
   }
   const int blocks = (p.dim + 31) / 32;
-  const dim3 grid((unsigned)((long)p.batch * p.heads * blocks)), blk(kStepThreads);
+  const dim3 grid((unsigned)linear_wgs(p)), blk(kStepThreads);
   if (p.key_dim <= 64) hipLaunchKernelGGL((linear_step_kernel<TYPE, 32, 2>), grid, blk, 0, s, p, blocks);
   else if (p.key_dim <= 128) hipLaunchKernelGGL((linear_step_kernel<TYPE, 32, 4>), grid, blk, 0, s, p, blocks);
   else hipLaunchKernelGGL((linear_step_kernel<TYPE, 32, 8>), grid, blk, 0, s, p, blocks);
@@ -706,6 +705,13 @@ size_t linear_split(LinearParams & p, int max_new)
   }
   p.seg = best ? (int)best : kMaxSeg;
   return best ? ((size_t)p.tokens / p.seg + p.batch) * p.heads * ((size_t)p.key_dim * p.dim + 2) * sizeof(float) : 0;
+}
+
+long linear_wgs(const LinearParams & p)
+{
+  if (p.seg == 0) return (long)p.batch * p.heads * ((p.dim + 31) / 32);
+  const long keys = ((long)p.tokens / p.seg + p.batch) * (p.heads / p.group);
+  return (keys + kXcds - 1) / kXcds * kXcds * p.group * ((p.dim + 127) / 128);
 }
 
 void launch_linear_attention(const LinearParams & p, hipStream_t s)

@@ -48,6 +48,19 @@ size_t paged_split(PagedParams & p, int max_new, int max_len)
   return (size_t)p.parts * c.tokens * p.heads * (c.dim + 2) * sizeof(float);
 }
 
+long paged_wgs(const PagedParams & p, long seqs)
+{
+  return (seqs * p.c.heads * p.parts + kXcds - 1) / kXcds * kXcds * p.row_slots;
+}
+
+JoinSplit join_split(const PagedParams & p)
+{
+  // a lot for every two parts where lanes allow it, and where rows alone do not fill the chip many times over
+  const long rows = (long)p.c.tokens * p.heads;
+  const int lanes = p.c.dim / 4, lots = rows < 1L << 23 ? std::max(1, std::min(p.parts / 2, 256 / lanes)) : 1, per = 256 / (lanes * lots);
+  return JoinSplit{lots, per, (rows + per - 1) / per};
+}
+
 void launch_paged_attention(const PagedParams & p, hipStream_t s)
 {
   if (p.c.type == kSeqF16) launch_paged_type<kSeqF16>(p, s);

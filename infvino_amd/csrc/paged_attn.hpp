@@ -585,9 +585,9 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attn_kernel(cons
 
 // Joins the parts of a row.  dim / 4 lanes have 4 channels each of every lots-th part, with a running
 // maximum; the lots of a row meet in LDS.  A part that had no keys for the row left a sum of zero, and its
-// values are not read.
+// values are not read.  first: the launch's first row.
 template <int TYPE>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p, int lots)
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p, int lots, long first)
 {
   typedef typename St<TYPE>::e E;
   __shared__ __attribute__((aligned(16))) float sum[256 * 4];
@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedParams p, in
   const CacheParams & c = p.c;
   const int lanes = c.dim / 4, tid = threadIdx.x, at = tid / lanes, ch = 4 * (tid - at * lanes);
   const int per = 256 / (lanes * lots), lot = at / per, sub = at - lot * per;  // rows of a work-group
-  const long n = (long)c.tokens * p.heads, row = (long)blockIdx.x * per + sub;
+  const long n = (long)c.tokens * p.heads, row = first + (long)blockIdx.x * per + sub;
   const int token = (int)(row / p.heads), head = (int)(row - (long)token * p.heads);
   // rows of no sequence stay as they are
   const bool on = lot < lots && row < n && token >= c.cu[0] && token < c.cu[c.batch];
@@ -646,9 +646,9 @@ template <int TYPE, int BITS, int DP, bool FULL, int QT, int WK, int KEYS> void 
   auto kern = paged_attn_kernel<TYPE, BITS, DP, FULL, QT, WK, KEYS>;
   const size_t own = (size_t)(WK / 2) * (4 / WK) * 16 * QT * (DP + 4 + 2) * sizeof(float), wide = (size_t)2 * 32 * (DP + 4 + 2) * sizeof(float);
   const size_t lds = KEYS == kBothWide ? std::max(own, wide) : own;
-  const long units = (long)(KEYS == kSharedKeys ? p.groups : p.c.batch) * p.c.heads * p.parts;
-  const dim3 grid((unsigned)((units + kXcds - 1) / kXcds * kXcds * p.row_slots + (KEYS == kBothKeys || KEYS == kBothWide ? p.shared_wgs : 0))), blk(256);
-  hipLaunchKernelGGL(kern, grid, blk, lds, s, p, (int)units);
+  const long seqs = KEYS == kSharedKeys ? p.groups : p.c.batch;
+  const dim3 grid((unsigned)(paged_wgs(p, seqs) + (KEYS == kBothKeys || KEYS == kBothWide ? p.shared_wgs : 0))), blk(256);
+  hipLaunchKernelGGL(kern, grid, blk, lds, s, p, (int)(seqs * p.c.heads * p.parts));
 }
 
 template <int TYPE, int BITS, int DP, bool FULL, int KEYS> void launch_paged_rows(const PagedParams & p, hipStream_t s)
@@ -677,11 +677,9 @@ template <int TYPE, int BITS, int KEYS = kAllKeys> void launch_paged_dim(const P
 
 template <int TYPE> void launch_paged_join(const PagedParams & p, hipStream_t s)
 {
-  // a lot for every two parts where lanes allow it, and where a launch holds the work-groups (fewer than 2^24)
-  const long rows = (long)p.c.tokens * p.heads;
-  const int lanes = p.c.dim / 4, lots = rows < 1L << 23 ? std::max(1, std::min(p.parts / 2, 256 / lanes)) : 1, per = 256 / (lanes * lots);
-  const dim3 grid((unsigned)((rows + per - 1) / per));
-  hipLaunchKernelGGL((paged_join_kernel<TYPE>), grid, dim3(256), 0, s, p, lots);
+  const JoinSplit j = join_split(p);
+  for (long first = 0; first < j.wgs; first += kJoinWgs)
+    hipLaunchKernelGGL((paged_join_kernel<TYPE>), dim3((unsigned)std::min(j.wgs - first, kJoinWgs)), dim3(256), 0, s, p, j.lots, first * j.per);
 }
 
 template <int TYPE> void launch_paged_type(const PagedParams & p, hipStream_t s)

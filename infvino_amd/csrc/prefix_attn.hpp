@@ -551,9 +551,8 @@ namespace {
 
 template <int TYPE, int BITS, int DP, bool FULL> void launch_shared(const PagedParams & p, hipStream_t s)
 {
-  const long units = (long)p.groups * p.c.heads * p.parts;
-  const dim3 grid((unsigned)((units + kXcds - 1) / kXcds * kXcds * p.row_slots));
-  hipLaunchKernelGGL((shared_attn_kernel<TYPE, BITS, DP, FULL>), grid, dim3(256), 0, s, p, (int)units);
+  const dim3 grid((unsigned)paged_wgs(p, p.groups));
+  hipLaunchKernelGGL((shared_attn_kernel<TYPE, BITS, DP, FULL>), grid, dim3(256), 0, s, p, p.groups * p.c.heads * p.parts);
 }
 
 template <int TYPE, int BITS> void launch_shared_dim(const PagedParams & p, hipStream_t s)

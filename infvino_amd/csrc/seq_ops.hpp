@@ -80,6 +80,15 @@ struct PagedParams {
 // Sets the split of a call with at most max_new new tokens and max_len cached ones in a
 // sequence (bounds that only steer the split); returns the workspace bytes.
 size_t paged_split(PagedParams & p, int max_new, int max_len);
+// Work-groups of 256 lanes over the keys of `seqs` sequences or groups.  A launch holds fewer than 2^24.
+long paged_wgs(const PagedParams & p, long seqs);
+// Rows are joined `per` a work-group, by `lots` lots of lanes each, in launches of at most kJoinWgs (a millisecond's work).
+struct JoinSplit {
+  int lots, per;
+  long wgs;
+};
+constexpr long kJoinWgs = 1L << 20;
+JoinSplit join_split(const PagedParams & p);
 void launch_paged_attention(const PagedParams & p, hipStream_t s);
 void launch_paged_bf16(const PagedParams & p, hipStream_t s);  // its bf16 kernels, built by themselves
 
@@ -115,6 +124,7 @@ struct LinearParams {
 };
 // Sets the split of a call with at most max_new rows in a sequence; returns the workspace bytes.
 size_t linear_split(LinearParams & p, int max_new);
+long linear_wgs(const LinearParams & p);  // of a launch over segments, or over states
 void launch_linear_attention(const LinearParams & p, hipStream_t s);
 
 struct SampleParams {
