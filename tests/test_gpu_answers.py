@@ -79,7 +79,7 @@ class Shared:
         seq._check_paged(self.cache, q, o, self.new, self.lens, self.table, 0, 0, scale)
 
 
-FEW, MANY = (0, 0, 0), (0, 0, 8192)  # hints; the latter has rows of 512 and more taken 128 at a time
+FEW, MANY = (0, 0, 0), (0, 0, 8192)  # hints; the latter is more than these tables hold, and is cut to that
 PREFIX = [  # bits, heads, kv heads, dim, page, sizes, shared, new, own, hints
     (8, 8, 2, 128, 16, [4], [200], [1] * 4, [1, 2, 17, 70], FEW),
     (8, 8, 2, 128, 16, [1], [64], [1], [1], FEW),
@@ -155,7 +155,7 @@ def test_prefix_attention_groups_and_lengths_of_every_kind(bits, hints, heads, k
             row += 1
 
 
-LONG = (0, 0, 16384)  # rows of 512 and more, of up to 64 channels, taken 128 at a time
+LONG = (0, 0, 16384)  # as MANY: rows are taken 128 at a time where tables hold as much (test_gpu_prefix_rows.py)
 PREFIX_LONG = [
     (8, 64, 2, 64, 64, [20], [1000], [1] * 20, [1 + 3 * i for i in range(20)], LONG),
     (8, 64, 1, 48, 16, [18, 16], [129, 65], [1] * 34, [1 + i % 5 for i in range(34)], LONG),

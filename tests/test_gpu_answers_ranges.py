@@ -139,3 +139,15 @@ def test_rows_on_top_of_one_another(t, max_new, which):
         setattr(x, name, rows.flatten().as_strided((n, 2, 64), (8, 64, 1)) if which == "near" else rows[:1].expand(n, -1, -1))
     o, state, _ = x.run(max_new=max_new)
     x.check(o, state)
+
+
+def test_the_same_call_gives_the_same_bits():
+    """Chunks, segments and single tokens, again and again."""
+    for t in TYPES:
+        for heads, kh, dk, dv, lens, max_new in ((4, 2, 128, 128, [65, 0, 1, 63, 2], 0), (2, 1, 128, 96, [1500, 40, 700], 0), (3, 3, 48, 80, [130, 17], 1),
+                                                 (2, 2, 256, 64, [900, 1025], 0)):
+            x = Linear(_gen(66), t, heads, kh, dk, dv, lens)
+            first = x.run(max_new=max_new)
+            for _ in range(5):
+                again = x.run(max_new=max_new)
+                assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
