@@ -688,11 +688,10 @@ size_t linear_split(LinearParams & p, int max_new)
   p.seg = 0;
   if (max_new <= 16) return 0;
   // Rounds of work-groups, two a CU (one above 128 key channels), times the tokens of each, for sequences of the same length
-  // or the longest one.  Segments cost a second pass over keys and values, and their first states.
+  // or the longest one.
   const long cap = p.key_dim <= 128 ? 512 : 256, wgs = (long)p.heads * ((p.dim + 127) / 128), mean = std::max(1, p.tokens / p.batch);
   auto rounds = [&](long units) { return (units * wgs + cap - 1) / cap; };
-  const long whole = std::max(rounds(p.batch) * mean, (long)max_new);
-  long best = 0, cost = whole * 10 / 17;
+  long best = 0, cost = std::max(rounds(p.batch) * mean, (long)max_new);
   // a launch holds fewer than 2^24 work-groups
   const long least = std::max<long>(256, ((long)p.tokens * wgs >> 22) / kChunk * kChunk + kChunk);
   for (long seg = least; seg < max_new; seg += std::max<long>(kChunk, seg / 16 / kChunk * kChunk)) {
@@ -703,6 +702,12 @@ size_t linear_split(LinearParams & p, int max_new)
     }
     if (seg > cost) break;
   }
+  // Segments cost a second pass over keys and values, and their first states: 0.7 of the outputs' time.  A second work-group on a
+  // CU takes 0.72 of another's time where it shares one, so whole sequences that give each CU one are left whole (32
+  // heads of 128 x 128, us, whole and in segments: 8 of 4096 tokens 325 and 385, 8 of 2048 167 and 207, 4 of 4096 283 and 212, one
+  // of 4096 281 and 82, of 512 42 and 41, of 300 28 and 40; 16 ragged ones of 16 heads of 64 x 96, 301 to 4099 tokens, 208 and 189).
+  auto busy = [&](long units) { return cap == 512 ? std::max(1.0, 0.86 * (double)(units * wgs) / 256.0) : (double)rounds(units); };
+  if (best && 1.7 * busy(p.batch * ((mean + best - 1) / best)) * (double)best >= std::max(busy(p.batch) * (double)mean, (double)max_new)) best = 0;
   p.seg = best ? (int)best : kMaxSeg;
   return best ? ((size_t)p.tokens / p.seg + p.batch) * p.heads * ((size_t)p.key_dim * p.dim + 2) * sizeof(float) : 0;
 }

@@ -5,6 +5,7 @@ import subprocess
 import pytest
 
 import infvino_amd as ia
+from infvino_amd import ops
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CLANG = "/opt/rocm/llvm/bin/clang++"
@@ -21,3 +22,11 @@ def test_launches_hold_their_work_groups(tmp_path):
     r = subprocess.run([exe], capture_output=True, text=True, timeout=300)
     print(r.stdout[-500:], r.stderr[-4000:])
     assert r.returncode == 0 and "0 failures" in r.stdout
+
+
+def test_long_sequences_are_cut_where_they_leave_compute_units_idle():
+    """Segments cost a second pass over keys and values: none where whole sequences give each CU a work-group (measured on both
+    sides beside linear_split)."""
+    for batch, tokens, cut in ((8, 4096, False), (8, 2048, False), (6, 4096, False), (12, 4096, False), (4, 4096, True), (1, 4096, True), (1, 768, True), (1, 300, False)):
+        d = ops.linear_attention_desc(ops.BF16, 32, 32, 128, 128, 0.1, batch, max_new=tokens)
+        assert (ops.linear_attention_workspace(d, batch, batch * tokens) > 0) == cut, (batch, tokens)
