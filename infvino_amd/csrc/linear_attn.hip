@@ -683,10 +683,13 @@ template <int TYPE> void launch_linear_type(const LinearParams & p, hipStream_t 
 
 size_t linear_split(LinearParams & p, int max_new)
 {
-  // token by token a state is read and written once as well, and 16 tokens of it cost less than a chunk's start,
-  // whose products take 64 rows whatever there is
+  // Token by token a state is read and written once as well, and a few tokens of it cost less than a chunk's start, whose
+  // products take 64 rows whatever there is.  The sides meet between 3 and 10 tokens, by sizes of states (96 sequences, us, token by token
+  // and in a chunk: 32 heads of 128 x 128 4 tokens 94 and 97, 6 111 and 99, 8 132 and 99, 16 207 and 104; 48 heads of
+  // 128 x 64 6 85 and 109, 10 114 and 109; 8 heads of 256 x 64 6 43 and 49, 8 52 and 49; 16 heads of 256 x 256 3 303 and 240;
+  // one sequence of 32 heads of 128 x 128 8 10.4 and 11.2, 16 16.5 and 11.2).
   p.seg = 0;
-  if (max_new <= 16) return 0;
+  if (max_new <= 6) return 0;
   // Rounds of work-groups, two a CU (one above 128 key channels), times the tokens of each, for sequences of the same length
   // or the longest one.
   const long cap = p.key_dim <= 128 ? 512 : 256, wgs = (long)p.heads * ((p.dim + 127) / 128), mean = std::max(1, p.tokens / p.batch);
