@@ -378,7 +378,8 @@ int ivh_linear_attention_workspace(const ivh_linear_attn_desc * d, int batch, in
    state.  A sequence without rows hands its state on.  g: natural logarithms of the decays, fp32; -infinity
    forgets what was before (but no infinity or NaN in it).  Decays may be above 1: rows
    are taken up to 64 at a time, so exp of a sum of g over up to 64 rows in a row, and what it makes of a value, a score
-   (q . k) and a state, have to be within fp32's range.  q, k, v rows start at multiples of 16 bytes, o's too.
+   (q . k) and a state, have to be within fp32's range.  q, k, v rows start at multiples of 16 bytes, o's too;
+   tokens of q, k and v lie less than 2^23 elements apart (0, or less than a row, for operands that tokens share).
    Infinities and NaN reach only the rows from theirs on.  o and state must not overlap an operand. */
 int ivh_linear_attention(const ivh_linear_attn_desc * d, const void * q, const void * k, const void * v, const float * g,
                          const int32_t * cu, const int32_t * from, const int32_t * to, float * state, void * o, int batch,

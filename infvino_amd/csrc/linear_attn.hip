@@ -5,21 +5,27 @@
 // Few new tokens (the recurrence): a state is read, taken through its tokens in registers, and
 // written, 8 key_dim dim bytes of HBM for 4 key_dim dim operations a token: HBM bounds it.  A
 // work-group has `DV` value channels of one head: a thread 4 of them and every (1024 / DV)-th key channel.  The sums
-// over the key channels meet by lane exchanges and through LDS, which two copies of keep at one barrier a
-// token.  96 sequences of 32 heads of 128 x 128, a token each: 83 us, 4.8 TB/s.
+// over the key channels meet by lane exchanges and through LDS, two barriers a token; two copies of what LDS holds keep the next token's
+// rows from waiting for the last one's sums.  96 sequences of 32 heads of 128 x 128, a token each: 84 us, 4.8 TB/s.
 //
 // Many (chunks of 64 rows): with b_t the sum of the chunk's g up to t,
 //
 //   o_t = scale (e^(b_t) q_t S0 + sum_{s <= t} e^(b_t - b_s) (q_t k_s) v_s),  S' = e^(b_63) S0 + sum_s e^(b_63 - b_s) k_s^T v_s
 //
 // are matrix products.  A work-group has up to 128 value channels of a head, a wave 32 of them and all key channels: the state
-// stays in a wave's accumulators, S0 enters the first product in two 16-bit parts, and values with their decays enter the
-// last in three bf16 or two fp16 parts, so that states keep the precision of fp32 products.  Chunks follow one another, which leaves
+// stays in a wave's accumulators, and values with their decays enter the last in three bf16 or two fp16 parts, so that states, which
+// hand their errors on, keep the precision of fp32 products.  What only an output sees is held to fewer bits: S0 enters the first
+// product in two 16-bit parts (16 bits in bf16, off by 2^-17, a 512th of half a step of the output; a third part would be half of that
+// product's matrix work again), and scores are rounded to the storage type once, as the weights of the softmax
+// attention are (off by half a step each, independently, where the output's own rounding is half a step of the sum): an operand
+// of the matrix cores has 16 bits.  fp16's range is too small for states, values with decays and scores: columns of the first two and
+// rows of the last are held times powers of two, which follow what they meet.  Chunks follow one another, which leaves
 // little to hide latency behind: the next chunk's rows come by LDS DMA while this one is worked on, over barriers that do not
 // wait for them.  A long sequence is cut into segments: what each adds to a state that begins with
 // nothing, the first states from those, then the outputs of all at once.  It costs a second pass over keys and
-// values and pays where sequences do not fill the chip.  Ragged prompts 93 us (states 25, join 5, outputs 74 in a
-// trace), a long one 224 (69 to 84, 11, 132 to 165); one segment each in place of that 4240 us and 17160 by single tokens.
+// values and pays where sequences do not fill the chip.  Ragged prompts of 16 heads of 64 x 96 in fp16 93 us (in a trace the median of
+// states is 28.6, of the join 5.4, of outputs 65.5), a long one of 32 heads of 128 x 128 225 (at best 70, 10 and 136; in a trace, whose calls
+// follow one another less closely, medians of 87, 12 and 176); by single tokens 4240 and 17160.
 #include <algorithm>
 #include <cmath>
 #include <stdexcept>

@@ -18,7 +18,7 @@ size_t prefix_split(PrefixParams & p, int max_new, int max_len, int max_shared)
   if (p.own.groups > 0) {
     p.first.c.batch = p.own.groups;
     const long tokens = (c.tokens + p.own.groups - 1) / p.own.groups, rows = tokens * p.own.group;
-    // measured on both sides in prefix_attn.hpp
+    // both sides of each bound are in prefix_attn.hpp
     p.many = c.dim <= 64 && rows >= 512 && max_shared >= 16384;
     p.wide = !p.many && (c.dim <= 64 ? rows > 16 : c.dim <= 128 && rows >= 96);
     if (p.many || p.wide) {

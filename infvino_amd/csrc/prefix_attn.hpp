@@ -6,22 +6,28 @@
 // the sequence's own: the shared keys are read once for the rows of all sequences, which are contiguous.
 // All parts are joined by a kernel behind them.  Own keys take the paged attention's kernel; shared ones
 //   * for up to 16 rows of a group (95 with heads of more than 64 channels), and where heads have more than 128, that
-//     kernel as well, in work-groups of the same launch where the tiles agree.  With few rows the keys' latency counts:
-//     32 rows of 128 channels behind 2048 tokens 15 us so, 18 by 32 rows a wave;
+//     kernel as well, in work-groups of the same launch where the tiles agree.  With few rows the keys' latency counts.  8 key
+//     heads, 8 bits, so and by 32 rows a wave: 128 channels behind 8192 tokens 48 rows 16.0 and 17.1 us, 96 19.8 and 20.1, 128 22.2 and
+//     21.4 (behind 1024 15.3 and 17.5, 16.0 and 17.1 with 96 and 128 rows); 64 channels behind 1024 16 rows 13.4 and 13.4, 24 19.5 and 13.3;
 //   * by 32 rows (shared_rows), in the same launch: each key that L2 gives has twice the rows of that kernel's tiles.
-//     64 sequences of 4 rows a key head behind 8192 tokens, own keys of 20 to 1501, 8 bits: 52 -> 45 us, the kernel 34,
+//     64 sequences of 4 rows a key head behind 8192 tokens, own keys of 20 to 1501, 8 bits: 52 -> 44 us, the kernel 38 to 39,
 //     of which the keys' 94 MB are 18 at a copy's rate; 5 groups of 112 rows behind 700 to 6007 tokens in 16 bits 53 -> 37 us;
 //     24 rows of 64 channels behind 1024 tokens 18 -> 13 us;
 //   * with many rows of up to 64 channels behind a long prefix the keys' conversion and L2 bound that: a work-group has 128
 //     rows, a wave 32 of them, and walks 64 keys a step (shared_attn_kernel).  The steps' keys and values stand in LDS in two
 //     stages, in 16 bits, each 1024 bytes a fragment of 32 x 32 x 16 MFMA in the order of its lanes: they are read without a
 //     bank conflict, and 8-bit codes are widened once for the four waves.  1536 rows a key head behind 32000 tokens: 180 us,
-//     0.56 PFLOP/s; behind 16384 120 us in all, 127 by shared_rows, behind 8192 81 and 73.  With 128 channels the accumulators leave two
-//     waves a SIMD and the barriers cost more than the copies save: 768 rows behind 32768 tokens 234 us, 191 by shared_rows.
+//     0.56 PFLOP/s; behind 16384 120 us in all, 127 by shared_rows, behind 8192 81 and 73.  Where the sides meet, 8 key heads, so and by
+//     shared_rows, 8 and 16 bits: behind 16384 512 rows 56 and 55, 63 and 69 us, 384 rows 49 and 47, 53 and 53, 1024 88 and 98, 95 and 126;
+//     behind 8192 512 rows 44 and 33, 49 and 40, 1024 61 and 54, 67 and 68; behind 32768 256 rows 52 and 55, 58 and 69.  With 128 channels
+//     the accumulators leave two waves a SIMD and the barriers cost more than the copies save: 768 rows behind 32768 tokens 234
+//     us, 191 by shared_rows.
 // Both:
 //   * S^T = K Q^T with keys in rows in an order of which a lane holds, of a 32-key part, the 16 keys of one granule
 //     (8-bit pages) or two runs of 8 (16-bit): they are operands of O^T = V^T P^T as they are;
-//   * weights, running maxima and scales as in paged_attn.hpp; nothing is masked but pages that hold nothing.
+//   * weights, running maxima and scales as in paged_attn.hpp: weights are rounded to 16 bits for the second product, half a step each
+//     and independently (outputs are 5 to 20 % further from 64 bits than with fp32 weights), since an operand of the matrix cores has
+//     no more, and the sum is that of the rounded ones; nothing is masked but pages that hold nothing.
 #pragma once
 
 #include "paged_attn.hpp"

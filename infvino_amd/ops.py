@@ -171,7 +171,8 @@ def prefix_attention(d: PrefixAttentionDesc, q, kc, vc, ks, vs, cu, lens, table,
 
 def linear_attention_desc(type, heads, key_heads, key_dim, dim, scale, slots, q=None, k=None, v=None, o=None, g=None,
                           max_new=0) -> LinearAttentionDesc:
-    """g: strides of the decays, dense [tokens][heads] by default; (0, 1): one for each head."""
+    """g: strides of the decays, dense [tokens][heads] by default; (0, 1): one for each head.  Tokens of q, k and v lie less than
+    2^23 elements apart."""
     dk, dv = (key_heads * key_dim, key_dim), (heads * dim, dim)
     q, k, v, o, g = q or dk, k or dk, v or dv, o or dv, g or (heads, 1)
     return LinearAttentionDesc(type, heads, key_heads, key_dim, dim, scale, slots, q[0], q[1], k[0], k[1], v[0], v[1], o[0], o[1],
